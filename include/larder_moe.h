@@ -490,6 +490,53 @@ int lmoe_quantize_q4_0(const void *w, int wdtype, long long rows, int cols, uint
  * Q4_K test and benchmark packs (configuration 5). */
 int lmoe_quantize_q4_k(const void *w, int wdtype, long long rows, int cols, uint8_t *out, void *stream);
 
+/* ---- attention of the trunk's rows ----
+ * Rows are packed: [T][heads][D] with strides in elements between rows and between heads, channels dense; sequence b's rows
+ * are cu[b] .. cu[b + 1] (int32 [B + 1], cu NULL: row b alone, T == B). Rows of no sequence come back zero where a call
+ * returns rows. Alignment of 16 bytes is asked of rows, heads and codes unless said otherwise.
+ *
+ * lmoe_rope_rows: rotary positions (route_cuda.py:549-591's rotation): the first 2 n_freq of a head's D channels (D <= 1024)
+ * in pairs (i, i + n_freq), or (2 i, 2 i + 1) where interleaved: gain (u cos a - w sin a, w cos a + u sin a), a = positions[t]
+ * freq[i] (positions int32, or int64 where positions64; freq float64 radians). Any dtype, alignment and strides; out may be x. */
+int lmoe_rope_rows(const void *x, int dtype, long long x_row, long long x_head, const void *positions, int positions64,
+                   const double *freq, int n_freq, int T, int heads, int D, int interleaved, float gain, void *out,
+                   long long out_row, long long out_head, void *stream);
+
+/* The paged 8-bit cache: codes e4m3 [pages][heads][page][D] and scales float32 [pages][heads], of keys and of values; page 32,
+ * 64 or 128 tokens, D 64, 128 or 256. table [B][width] int32: a sequence's pages in order; an entry outside [0, pages), and
+ * places past the table, hold nothing. lens [B]: a sequence's tokens, the call's rows being the last ones. No counterpart in
+ * the reference, whose cache is its MLX arrays.
+ * lmoe_kv_append: k (rotated by its places as lmoe_rope_rows does) and v into the pages. The scale of a page's head is the
+ * least power of two >= 2^-100 with largest finite |x| <= 448 scale; where the page held tokens before, the larger of that and
+ * its old one, and the held codes are restated. Infinities and NaN are written as NaN. q (optional) [T][q_heads][D] rotated
+ * into q_out [T][q_heads][D] dense; k_out (optional) [T][heads][D] dense gets the rotated keys in dtype. n_freq % 8 == 0
+ * (% 4 where interleaved), 0: no rotation. A page is written for one sequence of the call only.
+ * lmoe_kv_read: rows cu[b] .. cu[b + 1] of k_out / v_out [total][heads][D] get sequence b's first tokens, code times scale.
+ * lmoe_kv_attend: out [T][q_heads][D] = softmax(scale q k^T) v in float16 / bfloat16, row r of a sequence's n over its first
+ * lens - n + r + 1 tokens (none: zero). most_rows / longest: about the most rows / tokens of a sequence (any value is sound;
+ * they size the launch). workspace: lmoe_kv_attend_workspace_bytes of the same numbers, 16-byte aligned. B <= 65535. */
+int lmoe_kv_append(const void *q, long long q_row, long long q_head, int q_heads, const void *k, long long k_row,
+                   long long k_head, const void *v, long long v_row, long long v_head, int dtype, int T, int heads, int D,
+                   const int *cu, const int *lens, int B, const int *table, int width, uint8_t *k_codes, float *k_scale,
+                   uint8_t *v_codes, float *v_scale, int pages, int page, const double *freq, int n_freq, int interleaved,
+                   float gain, void *q_out, void *k_out, void *stream);
+int lmoe_kv_read(const uint8_t *k_codes, const float *k_scale, const uint8_t *v_codes, const float *v_scale, int pages, int page,
+                 int heads, int D, const int *table, int width, const int *cu, int B, int total, void *k_out, void *v_out,
+                 int dtype, void *stream);
+size_t lmoe_kv_attend_workspace_bytes(int T, int q_heads, int heads, int D, int B, int most_rows, int longest);
+int lmoe_kv_attend(const void *q, int dtype, long long q_row, long long q_head, int T, int q_heads, int heads, int D,
+                   const int *cu, const int *lens, int B, const int *table, int width, const uint8_t *k_codes,
+                   const float *k_scale, const uint8_t *v_codes, const float *v_scale, int pages, int page, int most_rows,
+                   int longest, float scale, void *workspace, size_t workspace_bytes, void *out, void *stream);
+
+/* Attention over whole prompts, causal: q [T][q_heads][D], k and v [U][heads][D] (float16 or bfloat16; q_heads a multiple of
+ * heads; D 64, 128 or 256), sequence b's rows cu[b] .. cu[b + 1] of q over keys cu_k[b] .. cu_k[b + 1]: the last row sees all of
+ * them, each one before it one fewer (none: zero). out [T][q_heads][D] dense, in dtype. Rows of k and v are less than 2^23
+ * elements apart. The reference runs its trunk's prompt attention on MLX (cpu_ext/cpu_kern.cpp:493-659 is its CPU form). */
+int lmoe_prompt_attend(const void *q, long long q_row, long long q_head, const void *k, long long k_row, long long k_head,
+                       const void *v, long long v_row, long long v_head, int dtype, int T, int U, int q_heads, int heads, int D,
+                       const int *cu, const int *cu_k, int B, float scale, void *out, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

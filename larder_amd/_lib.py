@@ -105,6 +105,14 @@ SIGNATURES = {
     "lmoe_qmv_swiglu_rows": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P]),
     "lmoe_quantize_q4_0": (_I, [_P, _I, _LL, _I, _P, _P]),
     "lmoe_quantize_q4_k": (_I, [_P, _I, _LL, _I, _P, _P]),
+    "lmoe_rope_rows": (_I, [_P, _I, _LL, _LL, _P, _I, _P, _I, _I, _I, _I, _I, _F, _P, _LL, _LL, _P]),
+    "lmoe_kv_append": (_I, [_P, _LL, _LL, _I, _P, _LL, _LL, _P, _LL, _LL, _I, _I, _I, _I, _P, _P, _I, _P, _I, _P, _P, _P, _P,
+                            _I, _I, _P, _I, _I, _F, _P, _P, _P]),
+    "lmoe_kv_read": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _P, _I, _P, _I, _I, _P, _P, _I, _P]),
+    "lmoe_kv_attend_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I]),
+    "lmoe_kv_attend": (_I, [_P, _I, _LL, _LL, _I, _I, _I, _I, _P, _P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _F, _P, _SZ,
+                            _P, _P]),
+    "lmoe_prompt_attend": (_I, [_P, _LL, _LL, _P, _LL, _LL, _P, _LL, _LL, _I, _I, _I, _I, _I, _I, _P, _P, _I, _F, _P, _P]),
 }
 
 _LIB = None

@@ -1,0 +1,39 @@
+// What the kernels of the trunk's attention share (rope.hip, attend.hip, prompt.hip): the place of a packed row in its
+// sequence, the cos / sin of a position, matrix-core fragments.
+#pragma once
+#include "grouped.h"
+
+namespace lmoe {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// The largest b < B with first(cu[b], b) <= t, by one wavefront (-1 if there is none); first never falls with b where cu
+// does not. 64 sequences a step. Whatever cu holds, the result is in [-1, B).
+template <typename F>
+__device__ __forceinline__ int last_at(const int *cu, int B, int t, F &&first) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+  for (int b0 = 0; b0 < B; b0 += 64) {
+    const int b = b0 + lane;
+    const unsigned long long le = __ballot(b < B && first(cu[b < B ? b : B - 1], b) <= (long long)t);
+    n += __popcll(le);
+    if (le != ~0ull) break;
+  }
+  return n - 1;
+}
+
+// A sequence's rows [row0, row0 + n) of T packed ones: cu[b] .. cu[b + 1], or row b alone where cu is null. Offsets past
+// the rows that there are (or that fall) leave an empty sequence, never a row out of bounds.
+__device__ __forceinline__ void seq_rows(const int *cu, int b, int T, int *row0, int *n) {
+  if (!cu) {
+    *row0 = b;
+    *n = b < T ? 1 : 0;
+    return;
+  }
+  const int a = cu[b], e = min(cu[b + 1], T);
+  *row0 = a;
+  *n = a < 0 || e <= a ? 0 : e - a;
+}
+
+}  // namespace lmoe

@@ -3,6 +3,7 @@
     qmv_fits(x, w, scales, group_size, bits, mode, biases)   route_cuda.py:516-522
     qmv_rows(x, w, scales, biases, group_size)               route_cuda.py:525-541 (lmoe_qmv_rows)
     shared_expert_rows(x, gate, up, down)                    mlx_lm's shared_expert MLP on qmv_rows projections
+    attention_rows(x, qkv, out, cache, table, lens, ...)     mlx_lm's attention on qmv_rows projections and the paged cache
 
 qmv_rows gives every row of x the bits of the reference's kernel (MLX 0.32.4's one-row qmv arithmetic: bf16
 weights, bf16 fused multiply-add slots, a float32 slot sum and lane butterfly), reading the weights once a pass.
@@ -11,9 +12,10 @@ bfloat16 [N, K / G].
 """
 import torch
 
+from . import attention
 from ._lib import call, ptr, stream
 
-__all__ = ["qmv_fits", "qmv_rows", "shared_expert_rows"]
+__all__ = ["attention_rows", "qmv_fits", "qmv_rows", "shared_expert_rows"]
 
 
 def qmv_fits(x, w, scales, group_size, bits, mode, biases):
@@ -59,3 +61,36 @@ def shared_expert_rows(x, gate, up, down):
     h = torch.empty_like(g)
     call("lmoe_swiglu_bf16", ptr(g), ptr(u), g.numel(), ptr(h), stream())
     return qmv_rows(h, *down)
+
+
+def attention_rows(x, qkv, out, cache, table, lens, cu=None, freq=None, interleaved=False, gain=1.0, prompt=None,
+                   most_rows=None, longest=None):
+    """The trunk's attention of x [T, H] bf16 (larder_amd.attention's packed rows): out(attend(rotate(qkv(x)))), with qkv and
+    out (w, scales, biases, group_size) 4-bit affine weights run through qmv_rows, qkv's output the query heads, then the key
+    heads, then the value heads of the cache's width. The rows' keys and values are written to the cache, then read by
+
+      prompt None              the newest rows of each sequence over its cached tokens (attend_rows; most_rows, longest its)
+      prompt True              sequences that begin with this call, over the call's own keys and values (prompt_rows)
+      prompt (cu_k, total)     later chunks of prompts: over all the cached tokens, lens of each, total in all, cu_k int32
+                               [sequences + 1] where each begins (read_rows, prompt_rows)
+    """
+    heads, width = cache.k.shape[1], cache.k.shape[3]
+    y = qmv_rows(x, *qkv)
+    t, q_heads = y.shape[0], y.shape[1] // width - 2 * heads
+    if q_heads <= 0 or y.shape[1] % width:
+        raise ValueError(f"attention_rows: {y.shape[1]} outputs are not query heads and {heads} key and value heads of {width}")
+    q, k, v = y.view(t, -1, width).split([q_heads, heads, heads], 1)
+    whole = prompt is True
+    if whole and cu is None:
+        raise ValueError("attention_rows: a prompt's rows need their offsets cu")
+    q, k = attention.append_rows(cache, q, k, v, table, lens, cu=cu, freq=freq, interleaved=interleaved, gain=gain, keys=whole)
+    if prompt is None:
+        o = attention.attend_rows(q, cache, table, lens, cu=cu, most_rows=most_rows, longest=longest)
+    elif whole:
+        o = attention.prompt_rows(q, k, v, cu)
+    else:
+        if cu is None:
+            raise ValueError("attention_rows: a prompt's rows need their offsets cu")
+        cu_k, total = prompt
+        o = attention.prompt_rows(q, *attention.read_rows(cache, table, cu_k, total, dtype=x.dtype), cu, cu_k=cu_k)
+    return qmv_rows(o.reshape(t, q_heads * width), *out)

@@ -1,0 +1,149 @@
+"""The host side of the trunk's attention without a GPU: rotary frequencies, the entry points' refusals, their workspace, and
+how a call's pages are dealt to workgroups."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from larder_amd import _lib, attention
+
+
+def test_rotary_freq():
+    f, gain = attention.rotary_freq(8, 10000.0, device="cpu")
+    assert torch.equal(f, 10000.0 ** (-torch.arange(4, dtype=torch.float64) / 4)) and gain == 1.0
+    g, _ = attention.rotary_freq(8, 10000.0, "linear", 4.0, device="cpu")
+    assert torch.equal(g, f / 4)
+    g, _ = attention.rotary_freq(8, 10000.0, "ntk", 4.0, device="cpu")
+    assert g[0] == 1.0 and math.isclose(float(g[-1]), float(f[-1]) / 4, rel_tol=1e-12)  # the slowest interpolated
+    f, _ = attention.rotary_freq(128, 10000.0, device="cpu")
+    g, gain = attention.rotary_freq(128, 10000.0, "yarn", 8.0, 4096, device="cpu")
+    assert math.isclose(gain, 0.1 * math.log(8) + 1)
+    turns = 4096 * f / (2 * math.pi)
+    assert torch.allclose(g[turns > 40], f[turns > 40]) and torch.allclose(g[turns < 0.8], f[turns < 0.8] / 8)
+    assert ((g <= f) & (g >= f / 8)).all() and (torch.diff(g) < 0).all()
+    # factor 1: f keep + f (1 - keep), three roundings of 2^-53
+    assert torch.allclose(attention.rotary_freq(128, 10000.0, "yarn", 1.0, 4096, device="cpu")[0], f, rtol=2.0 ** -51, atol=0)
+
+
+@pytest.mark.parametrize("kw", [dict(width=7), dict(width=0), dict(width=8, factor=0.5), dict(width=8, kind="yarn"),
+                                dict(width=8, kind="other")])
+def test_rotary_freq_refuses(kw):
+    with pytest.raises(ValueError):
+        attention.rotary_freq(**kw, device="cpu")
+
+
+def test_tensors_off_the_gpu_are_refused():
+    x, i = torch.zeros(1, 1, 64, dtype=torch.float16), torch.zeros(1, dtype=torch.int32)
+    cache = attention.KVCache.empty(1, 1, 64, device="cpu")
+    freq = torch.zeros(32, dtype=torch.float64)
+    cu = torch.tensor([0, 1], dtype=torch.int32)
+    for call in (lambda: attention.rope_rows(x, i, freq), lambda: attention.append_rows(cache, x, x, x, i[None], i),
+                 lambda: attention.attend_rows(x, cache, i[None], i), lambda: attention.read_rows(cache, i[None], cu, 1),
+                 lambda: attention.prompt_rows(x, x, x, cu)):
+        with pytest.raises(ValueError, match="GPU"):
+            call()
+
+
+P = ctypes.c_void_p(16)  # never dereferenced: every call below is refused while its arguments are checked
+ODD = ctypes.c_void_p(24)
+
+
+def refused(L, code, word, name, *args):
+    rc = getattr(L, name)(*args, None)
+    assert rc == code and word in L.lmoe_error(), (rc, L.lmoe_error())
+
+
+def test_entry_points_refuse(built_lib):
+    L = built_lib
+
+    def rope(x=P, dt=1, st=64, pos=P, freq=P, n=32, T=2, h=1, D=64, out=P):
+        return x, dt, st, 64, pos, 0, freq, n, T, h, D, 0, 1.0, out, 64, 64
+
+    refused(L, _lib.EINVAL, b"dtype", "lmoe_rope_rows", *rope(dt=3))
+    refused(L, _lib.ESHAPE, b"pairs", "lmoe_rope_rows", *rope(n=33))
+    refused(L, _lib.ESHAPE, b"heads of", "lmoe_rope_rows", *rope(D=1026))
+    refused(L, _lib.ESHAPE, b"rows", "lmoe_rope_rows", *rope(T=-1))
+    refused(L, _lib.EINVAL, b"null", "lmoe_rope_rows", *rope(pos=None))
+    refused(L, _lib.EINVAL, b"null", "lmoe_rope_rows", *rope(freq=None))
+    assert L.lmoe_rope_rows(*rope(T=0, x=None), None) == 0
+
+    def append(q=P, k=P, v=P, dt=1, T=2, heads=1, D=64, cu=P, B=1, width=1, pages=1, page=64, n=32, inter=0, st=128, codes=P,
+               q_out=P):
+        return (q, st, 64, 1, k, st, 64, v, st, 64, dt, T, heads, D, cu, P, B, P, width, codes, P, P, P, pages, page, P, n, inter,
+                1.0, q_out, None)
+
+    refused(L, _lib.EINVAL, b"dtype", "lmoe_kv_append", *append(dt=7))
+    refused(L, _lib.ESHAPE, b"channels", "lmoe_kv_append", *append(D=96, n=0))
+    refused(L, _lib.ESHAPE, b"tokens", "lmoe_kv_append", *append(page=16))
+    refused(L, _lib.ESHAPE, b"pairs", "lmoe_kv_append", *append(n=12))
+    refused(L, _lib.ESHAPE, b"pairs", "lmoe_kv_append", *append(n=6, inter=1))
+    refused(L, _lib.ESHAPE, b"pairs", "lmoe_kv_append", *append(n=40))
+    refused(L, _lib.ESHAPE, b"offsets", "lmoe_kv_append", *append(cu=None))
+    refused(L, _lib.ESHAPE, b"pages", "lmoe_kv_append", *append(pages=0))
+    refused(L, _lib.EINVAL, b"null", "lmoe_kv_append", *append(k=None))
+    refused(L, _lib.EINVAL, b"null", "lmoe_kv_append", *append(q_out=None))
+    refused(L, _lib.EALIGN, b"aligned", "lmoe_kv_append", *append(k=ODD))
+    refused(L, _lib.EALIGN, b"aligned", "lmoe_kv_append", *append(st=68))
+    refused(L, _lib.EALIGN, b"aligned", "lmoe_kv_append", *append(codes=ODD))
+    assert L.lmoe_kv_append(*append(T=0), None) == 0
+
+    def read(pages=1, page=64, heads=1, D=64, B=1, total=2, k=P, dt=1):
+        return P, P, P, P, pages, page, heads, D, P, 1, P, B, total, k, P, dt
+
+    refused(L, _lib.EINVAL, b"dtype", "lmoe_kv_read", *read(dt=9))
+    refused(L, _lib.ESHAPE, b"rows", "lmoe_kv_read", *read(total=-1))
+    refused(L, _lib.ESHAPE, b"channels", "lmoe_kv_read", *read(D=32))
+    refused(L, _lib.EINVAL, b"null", "lmoe_kv_read", *read(k=None))
+    refused(L, _lib.EALIGN, b"aligned", "lmoe_kv_read", *read(k=ODD))
+
+    def attend(q=P, dt=1, st=64, T=2, qh=2, h=1, D=64, cu=P, B=1, pages=1, page=64, most=1, longest=8192, ws=P, wsb=1 << 30):
+        return (q, dt, st, 64, T, qh, h, D, cu, P, B, P, 1, P, P, P, P, pages, page, most, longest, 0.125, ws, wsb, P)
+
+    refused(L, _lib.EINVAL, b"dtype", "lmoe_kv_attend", *attend(dt=0))
+    refused(L, _lib.ESHAPE, b"query heads", "lmoe_kv_attend", *attend(qh=3, h=2))
+    refused(L, _lib.ESHAPE, b"channels", "lmoe_kv_attend", *attend(D=192))
+    refused(L, _lib.ESHAPE, b"tokens", "lmoe_kv_attend", *attend(page=256))
+    refused(L, _lib.ESHAPE, b"sequences", "lmoe_kv_attend", *attend(B=65536))
+    refused(L, _lib.ESHAPE, b"sequences", "lmoe_kv_attend", *attend(longest=0))
+    refused(L, _lib.ESHAPE, b"offsets", "lmoe_kv_attend", *attend(cu=None))
+    refused(L, _lib.EINVAL, b"null", "lmoe_kv_attend", *attend(q=None))
+    refused(L, _lib.EALIGN, b"aligned", "lmoe_kv_attend", *attend(st=65))
+    refused(L, _lib.EWORKSPACE, b"workspace", "lmoe_kv_attend", *attend(wsb=16))
+    refused(L, _lib.EWORKSPACE, b"workspace", "lmoe_kv_attend", *attend(ws=None))
+
+    def prompt(q=P, k=P, st=64, kst=64, dt=1, T=2, U=2, qh=1, h=1, D=64, cu=P, B=1):
+        return q, st, 64, k, kst, 64, P, 64, 64, dt, T, U, qh, h, D, cu, P, B, 0.125, P
+
+    refused(L, _lib.EINVAL, b"dtype", "lmoe_prompt_attend", *prompt(dt=0))
+    refused(L, _lib.ESHAPE, b"channels", "lmoe_prompt_attend", *prompt(D=80))
+    refused(L, _lib.ESHAPE, b"query heads", "lmoe_prompt_attend", *prompt(qh=3, h=2))
+    refused(L, _lib.ESHAPE, b"sequence", "lmoe_prompt_attend", *prompt(B=0))
+    refused(L, _lib.EINVAL, b"null", "lmoe_prompt_attend", *prompt(cu=None))
+    refused(L, _lib.EALIGN, b"aligned", "lmoe_prompt_attend", *prompt(q=ODD))
+    refused(L, _lib.ESHAPE, b"apart", "lmoe_prompt_attend", *prompt(kst=1 << 23))
+    assert L.lmoe_prompt_attend(*prompt(T=0), None) == 0
+
+
+def test_attend_workspace(built_lib):
+    need = built_lib.lmoe_kv_attend_workspace_bytes
+    assert need(1, 16, 16, 128, 1, 1, 100) == 0                      # one chunk: nothing to join
+    assert need(1, 32, 4, 128, 1, 1, 8192) % (32 * 130 * 4) == 0 and need(1, 32, 4, 128, 1, 1, 8192) > 0
+    assert need(1, 3, 2, 128, 1, 1, 8192) == 0                       # refused shapes ask for nothing
+
+
+@pytest.mark.parametrize("unit,spare", [(32, 2), (64, 2), (128, 2), (128, 1)])
+def test_every_page_and_tile_has_a_workgroup(unit, spare):
+    """Sequence b's workgroups begin at cu[b] // unit + spare b. With spare 2 that is room for every page that its rows can
+    touch, wherever they begin in the first (k_append); with spare 1 for every tile of unit rows (k_prompt)."""
+    rng = np.random.default_rng(unit + spare)
+    for _ in range(200):
+        n = rng.choice([0, 1, 2, unit - 1, unit, unit + 1, 3 * unit + 5], 8)
+        cu = np.concatenate([[0], np.cumsum(n)])
+        first = cu // unit + spare * np.arange(9)
+        for b in range(8):
+            start = rng.integers(0, unit) if spare == 2 else 0
+            touched = 0 if n[b] == 0 else (start + n[b] - 1) // unit - start // unit + 1
+            assert touched <= first[b + 1] - first[b]
+        assert first[8] == cu[8] // unit + spare * 8                  # what the host launches
