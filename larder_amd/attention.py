@@ -20,6 +20,7 @@ n + r. table int32 [sequences, width] lists each sequence's pages in order; entr
 page outside the cache (or the table) holds nothing: no token is written there and none is seen. Sequences may share pages
 they only read; a page that a call writes to belongs to one of them.
 """
+import functools
 import math
 from typing import NamedTuple
 
@@ -93,82 +94,99 @@ def rotary_freq(width, base=10000.0, kind="default", factor=1.0, original=None, 
 
 
 # ---- arguments -------------------------------------------------------------------------------------------------
+# A decode step's calls take the host longer than the GPU, so these checks are plain comparisons, and what a refusal says is
+# put together only once there is one.
 
-def _p(t):
-    return None if t is None else t.data_ptr()
-
-
-def _check(fn, ok, why):
-    if not ok:
-        raise ValueError(f"{fn}: {why}")
+_CODES = (torch.float8_e4m3fn, torch.uint8)
+_HALVES = (torch.float16, torch.bfloat16)
 
 
-def _same_device(fn, first, *others):
-    dev = first.device
-    _check(fn, first.is_cuda, "tensors must live on the GPU")
+def _refuse(fn, why):
+    raise ValueError(f"{fn}: {why}")
+
+
+def _device(fn, first, *others):
+    """The index of the one device that every tensor (None: skipped) lives on."""
+    dev = first.get_device()
+    if dev < 0:
+        _refuse(fn, "tensors must live on the GPU")
     for t in others:
-        _check(fn, t is None or t.device == dev, "tensors on different devices")
+        if t is not None and t.get_device() != dev:
+            _refuse(fn, "tensors on different devices")
     return dev
 
 
 def _rows(fn, name, x, heads=None, width=None, rows=None):
-    """A [T, heads, width] tensor the kernels can read (its last axis dense, 16-byte aligned rows), copied if it is not."""
-    _check(fn, x.dim() == 3, f"{name} is [rows, heads, width]")
-    _check(fn, (heads is None or x.shape[1] == heads) and (width is None or x.shape[2] == width)
-           and (rows is None or x.shape[0] == rows), f"{name} is {tuple(x.shape)}")
-    st, size = x.stride(), x.element_size()
-    if st[2] != 1 or (st[0] * size) % 16 or (st[1] * size) % 16 or x.data_ptr() % 16:
+    """(x, row stride, head stride): a [rows, heads, width] tensor the kernels can read (its last axis dense, 16-byte aligned
+    rows and heads), copied if it is not."""
+    if x.dim() != 3:
+        _refuse(fn, f"{name} is [rows, heads, width], not {tuple(x.shape)}")
+    r, h, w = x.shape
+    if (heads is not None and h != heads) or (width is not None and w != width) or (rows is not None and r != rows):
+        _refuse(fn, f"{name} is [{r}, {h}, {w}]")
+    s0, s1, s2 = x.stride()
+    mask = 3 if x.element_size() == 4 else 7
+    if s2 != 1 or s0 & mask or s1 & mask or x.data_ptr() & 15:
         x = x.contiguous()
-        if x.data_ptr() % 16:
+        if x.data_ptr() & 15:
             x = x.clone()
-    return x
+        s0, s1, s2 = x.stride()
+    return x, s0, s1
 
 
-def _ints(fn, name, t, *shape):
-    _check(fn, t.dtype == torch.int32 and t.dim() == len(shape) and all(s is None or s == d for s, d in zip(shape, t.shape)),
-           f"{name} is int32 {list(shape)}, not {t.dtype} {list(t.shape)}")
+def _ints(fn, name, t, n):
+    """int32 [n], dense."""
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != n:
+        _refuse(fn, f"{name} is int32 [{n}], not {t.dtype} {list(t.shape)}")
     return t if t.is_contiguous() else t.contiguous()
 
 
 def _sequences(fn, cu, lens, table, rows):
-    """(cu, lens, table, sequences) checked; lens may be None (read_rows)."""
-    n = table.shape[0] if table.dim() == 2 else -1
-    table = _ints(fn, "table", table, n, None)
-    _check(fn, table.shape[1] > 0, "a table without pages")
+    """(cu, lens, table, sequences, table width) checked; lens may be None (read_rows)."""
+    if table.dtype is not torch.int32 or table.dim() != 2 or table.shape[1] == 0:
+        _refuse(fn, f"table is int32 [sequences, pages], not {table.dtype} {list(table.shape)}")
+    n, width = table.shape
+    if not table.is_contiguous():
+        table = table.contiguous()
     if lens is not None:
         lens = _ints(fn, "lens", lens, n)
-    if cu is None:
-        _check(fn, rows == n, f"{rows} rows of {n} sequences need their offsets cu")
-    else:
+    if cu is not None:
         cu = _ints(fn, "cu", cu, n + 1)
-    return cu, lens, table, n
+    elif rows != n:
+        _refuse(fn, f"{rows} rows of {n} sequences need their offsets cu")
+    return cu, lens, table, n, width
 
 
 def _cache(fn, cache):
     k, ks, v, vs = cache
-    _check(fn, k.dim() == 4 and k.dtype in (torch.float8_e4m3fn, torch.uint8) and v.dtype == k.dtype and v.shape == k.shape,
-           "the cache's codes are float8_e4m3fn [pages, heads, page, width]")
-    _check(fn, ks.dtype == torch.float32 and vs.dtype == torch.float32 and ks.shape == k.shape[:2] and vs.shape == k.shape[:2],
-           "the cache's scales are float32 [pages, heads]")
-    _check(fn, k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous(),
-           "the cache's tensors must be contiguous")
-    return k.shape
+    shape = k.shape
+    if len(shape) != 4 or k.dtype not in _CODES or v.dtype is not k.dtype or v.shape != shape:
+        _refuse(fn, "the cache's codes are float8_e4m3fn [pages, heads, page, width]")
+    if ks.dtype is not torch.float32 or vs.dtype is not torch.float32 or ks.shape != shape[:2] or vs.shape != shape[:2]:
+        _refuse(fn, "the cache's scales are float32 [pages, heads]")
+    if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+        _refuse(fn, "the cache's tensors must be contiguous")
+    return (*shape, k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr())
 
 
 def _freq(fn, freq, width):
-    if freq is None:
-        return None, 0
-    _check(fn, freq.dtype == torch.float64 and freq.dim() == 1 and 2 * freq.numel() <= width,
-           "freq is float64 [pairs], two channels a pair")
-    return freq if freq.is_contiguous() else freq.contiguous(), freq.numel()
+    if freq is None or freq.dtype is not torch.float64 or freq.dim() != 1 or 2 * freq.shape[0] > width:
+        _refuse(fn, "freq is float64 [pairs], two channels a pair")
+    return freq if freq.is_contiguous() else freq.contiguous()
 
 
-def _on(dev, go):
-    """go(stream) with dev as the current device."""
-    if dev.index == torch.cuda.current_device():
-        return go(stream())
+def _launch(dev, name, *args):
+    """call(name, *args, stream) with dev as the current device."""
+    if dev == torch.cuda.current_device():
+        return call(name, *args, stream())
     with torch.cuda.device(dev):
-        return go(stream())
+        return call(name, *args, stream())
+
+
+# the workspace of a call is a function of its sizes alone
+@functools.lru_cache(maxsize=1024)
+def _attend_workspace(*sizes):
+    return _lib.lib().lmoe_kv_attend_workspace_bytes(*sizes)
 
 
 # ---- the calls -------------------------------------------------------------------------------------------------
@@ -179,26 +197,26 @@ def rope_rows(x, positions, freq, interleaved=False, gain=1.0, out=None):
     (2 i, 2 i + 1) where interleaved, multiplied by gain; the other channels as they are. float32 inside, one rounding.
     out: a tensor of x's shape and type, which may be x; rows of any strides with a dense last axis."""
     fn = "rope_rows"
-    _check(fn, x.dim() == 3, "x is [rows, heads, width]")
+    if x.dim() != 3:
+        _refuse(fn, "x is [rows, heads, width]")
     t, heads, width = x.shape
     dt = dcode(x.dtype)
-    _check(fn, positions.dim() == 1 and positions.shape[0] == t and positions.dtype in (torch.int32, torch.int64),
-           "positions is int32 or int64 [rows]")
-    freq, pairs = _freq(fn, freq, width)
-    _check(fn, freq is not None, "no frequencies")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 1 or positions.shape[0] != t:
+        _refuse(fn, "positions is int32 or int64 [rows]")
+    freq = _freq(fn, freq, width)
     if out is None:
         out = torch.empty((t, heads, width), dtype=x.dtype, device=x.device)
-    _check(fn, out.shape == x.shape and out.dtype == x.dtype and (width == 1 or out.stride(2) == 1),
-           "out has x's shape and type and a dense last axis")
-    dev = _same_device(fn, x, positions, freq, out)
-    if x.stride(2) != 1 and width > 1:
+    elif out.shape != x.shape or out.dtype is not x.dtype or (width > 1 and out.stride(2) != 1):
+        _refuse(fn, "out has x's shape and type and a dense last axis")
+    dev = _device(fn, x, positions, freq, out)
+    if width > 1 and x.stride(2) != 1:
         x = x.contiguous()
-    positions = positions if positions.is_contiguous() else positions.contiguous()
-    if x.numel() == 0:
-        return out
-    _on(dev, lambda st: call("lmoe_rope_rows", _p(x), dt, x.stride(0), x.stride(1), _p(positions),
-                             int(positions.dtype == torch.int64), _p(freq), pairs, t, heads, width, int(bool(interleaved)),
-                             float(gain), _p(out), out.stride(0), out.stride(1), st))
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    if x.numel():
+        _launch(dev, "lmoe_rope_rows", x.data_ptr(), dt, x.stride(0), x.stride(1), positions.data_ptr(),
+                positions.dtype is torch.int64, freq.data_ptr(), freq.shape[0], t, heads, width, bool(interleaved), gain,
+                out.data_ptr(), out.stride(0), out.stride(1))
     return out
 
 
@@ -208,30 +226,37 @@ def append_rows(cache, q, k, v, table, lens, cu=None, freq=None, interleaved=Fal
     the rotated k in its own type, as prompt_rows reads it (else None). float16, bfloat16 or float32. len(freq) is a multiple
     of 8 (of 4 where interleaved). The cache's tensors are written in place."""
     fn = "append_rows"
-    pages, heads, page, width = _cache(fn, cache)
+    pages, heads, page, width, *codes = _cache(fn, cache)
+    k, k_row, k_head = _rows(fn, "k", k, heads, width)
     t = k.shape[0]
-    k, v = _rows(fn, "k", k, heads, width), _rows(fn, "v", v, heads, width, t)
-    _check(fn, v.dtype == k.dtype and (q is None or q.dtype == k.dtype), "q, k and v have one type")
+    v, v_row, v_head = _rows(fn, "v", v, heads, width, t)
+    dtype = k.dtype
+    dt = dcode(dtype)
+    if v.dtype is not dtype or (q is not None and q.dtype is not dtype):
+        _refuse(fn, "q, k and v have one type")
+    cu, lens, table, n, room = _sequences(fn, cu, lens, table, t)
+    pairs = 0
+    if freq is not None:
+        freq = _freq(fn, freq, width)
+        pairs = freq.shape[0]
+    dev = _device(fn, k, v, q, table, lens, cu, freq, *cache)
+    q_in = q_out = k_out = None
+    q_heads = q_row = q_head = 0
     if q is not None:
-        q = _rows(fn, "q", q, None, width, t)
-    dt = dcode(k.dtype)
-    cu, lens, table, n = _sequences(fn, cu, lens, table, t)
-    freq, pairs = _freq(fn, freq, width)
-    dev = _same_device(fn, k, v, q, table, lens, cu, freq, *cache)
-    q_out = q
-    if q is not None and pairs:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    turned = q if pairs else None
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=dev) if keys else None
+        q, q_row, q_head = _rows(fn, "q", q, None, width, t)
+        q_out = q
+        if pairs:
+            q_heads, q_in = q.shape[1], q.data_ptr()
+            q_out = torch.empty((t, q_heads, width), dtype=dtype, device=q.device)
+    if keys:
+        k_out = torch.empty((t, heads, width), dtype=dtype, device=k.device)
     if t and n:
-        qs = turned.stride() if turned is not None else (0, 0)
-        _on(dev, lambda st: call(
-            "lmoe_kv_append", _p(turned), qs[0], qs[1], q.shape[1] if q is not None else 0, _p(k), k.stride(0), k.stride(1),
-            _p(v), v.stride(0), v.stride(1), dt, t, heads, width, _p(cu), _p(lens), n, _p(table), table.shape[1],
-            _p(cache[0]), _p(cache[1]), _p(cache[2]), _p(cache[3]), pages, page, _p(freq), pairs, int(bool(interleaved)),
-            float(gain), _p(q_out) if turned is not None else None, _p(k_out), st))
+        _launch(dev, "lmoe_kv_append", q_in, q_row, q_head, q_heads, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, dt,
+                t, heads, width, None if cu is None else cu.data_ptr(), lens.data_ptr(), n, table.data_ptr(), room, *codes, pages,
+                page, None if freq is None else freq.data_ptr(), pairs, bool(interleaved), gain,
+                None if q_in is None else q_out.data_ptr(), None if k_out is None else k_out.data_ptr())
     elif t:
-        q_out = q_out if turned is None else q_out.zero_()
+        q_out = q_out if q_in is None else q_out.zero_()
         k_out = k_out if k_out is None else k_out.zero_()
     return q_out, k_out
 
@@ -240,15 +265,16 @@ def read_rows(cache, table, cu, total, dtype=torch.bfloat16):
     """(k, v) [total, heads, width] in dtype: the first cu[b + 1] - cu[b] tokens of every sequence, codes times scale, rounded
     once (bfloat16 holds them exactly): the history that the rows of a later prompt chunk see, for prompt_rows."""
     fn = "read_rows"
-    pages, heads, page, width = _cache(fn, cache)
+    pages, heads, page, width, *codes = _cache(fn, cache)
     dt = dcode(dtype)
-    _check(fn, cu is not None, "no offsets cu")
-    cu, _, table, n = _sequences(fn, cu, None, table, total)
-    dev = _same_device(fn, cache[0], *cache[1:], table, cu)
-    k, v = (torch.empty((total, heads, width), dtype=dtype, device=dev) for _ in range(2))
+    if cu is None:
+        _refuse(fn, "no offsets cu")
+    cu, _, table, n, room = _sequences(fn, cu, None, table, total)
+    dev = _device(fn, *cache, table, cu)
+    k, v = (torch.empty((total, heads, width), dtype=dtype, device=table.device) for _ in range(2))
     if total:
-        _on(dev, lambda st: call("lmoe_kv_read", _p(cache[0]), _p(cache[1]), _p(cache[2]), _p(cache[3]), pages, page, heads,
-                                 width, _p(table), table.shape[1], _p(cu), n, total, _p(k), _p(v), dt, st))
+        _launch(dev, "lmoe_kv_read", *codes, pages, page, heads, width, table.data_ptr(), room, cu.data_ptr(), n, total,
+                k.data_ptr(), v.data_ptr(), dt)
     return k, v
 
 
@@ -260,25 +286,26 @@ def attend_rows(q, cache, table, lens, cu=None, most_rows=None, longest=None, sc
     most_rows and longest size the launch: about the most rows of a sequence (1 without cu, else T / sequences) and tokens of
     one (the table's room). Any values give the same sums in another order."""
     fn = "attend_rows"
-    pages, heads, page, width = _cache(fn, cache)
-    q = _rows(fn, "q", q, None, width)
-    t, q_heads = q.shape[0], q.shape[1]
-    _check(fn, q.dtype in (torch.float16, torch.bfloat16), f"q is float16 or bfloat16, not {q.dtype}")
-    _check(fn, q_heads > 0 and q_heads % heads == 0, f"{q_heads} query heads over {heads} key heads")
-    cu, lens, table, n = _sequences(fn, cu, lens, table, t)
-    dev = _same_device(fn, q, table, lens, cu, *cache)
-    out = torch.empty((t, q_heads, width), dtype=q.dtype, device=dev)
+    pages, heads, page, width, *codes = _cache(fn, cache)
+    q, q_row, q_head = _rows(fn, "q", q, None, width)
+    t, q_heads, _ = q.shape
+    dtype = q.dtype
+    if dtype not in _HALVES:
+        _refuse(fn, f"q is float16 or bfloat16, not {dtype}")
+    if q_heads == 0 or q_heads % heads:
+        _refuse(fn, f"{q_heads} query heads over {heads} key heads")
+    cu, lens, table, n, room = _sequences(fn, cu, lens, table, t)
+    dev = _device(fn, q, table, lens, cu, *cache)
+    out = torch.empty((t, q_heads, width), dtype=dtype, device=q.device)
     if not t or not n:
         return out.zero_()
-    most = int(most_rows) if most_rows is not None else 1 if cu is None else -(-t // n)
-    room = table.shape[1] * page
-    long = min(int(longest), room) if longest is not None else room
-    need = _lib.lib().lmoe_kv_attend_workspace_bytes(t, q_heads, heads, width, n, max(most, 1), max(long, 1))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _on(dev, lambda st: call(
-        "lmoe_kv_attend", _p(q), dcode(q.dtype), q.stride(0), q.stride(1), t, q_heads, heads, width, _p(cu), _p(lens), n,
-        _p(table), table.shape[1], _p(cache[0]), _p(cache[1]), _p(cache[2]), _p(cache[3]), pages, page, max(most, 1),
-        max(long, 1), float(width ** -0.5 if scale is None else scale), _p(ws), need, _p(out), st))
+    most = max(1, int(most_rows)) if most_rows is not None else 1 if cu is None else -(-t // n)
+    long = room * page if longest is None else max(1, min(int(longest), room * page))
+    need = _attend_workspace(t, q_heads, heads, width, n, most, long)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _launch(dev, "lmoe_kv_attend", q.data_ptr(), dcode(dtype), q_row, q_head, t, q_heads, heads, width,
+            None if cu is None else cu.data_ptr(), lens.data_ptr(), n, table.data_ptr(), room, *codes, pages, page, most, long,
+            width ** -0.5 if scale is None else scale, None if ws is None else ws.data_ptr(), need, out.data_ptr())
     return out
 
 
@@ -288,26 +315,31 @@ def prompt_rows(q, k, v, cu, cu_k=None, scale=None):
     The last row sees all of its sequence's keys, each row before it one fewer; a row that sees none is zero. scale is
     width^-0.5 if None."""
     fn = "prompt_rows"
-    q = _rows(fn, "q", q)
+    q, q_row, q_head = _rows(fn, "q", q)
     t, q_heads, width = q.shape
-    k = _rows(fn, "k", k, None, width)
-    u, heads = k.shape[0], k.shape[1]
-    v = _rows(fn, "v", v, heads, width, u)
-    _check(fn, q.dtype in (torch.float16, torch.bfloat16) and k.dtype == q.dtype and v.dtype == q.dtype,
-           "q, k and v are all float16 or all bfloat16")
-    _check(fn, width in (64, 128, 256), f"heads of {width} channels (64, 128 and 256 are served)")
-    _check(fn, heads > 0 and q_heads > 0 and q_heads % heads == 0, f"{q_heads} query heads over {heads} key heads")
-    _check(fn, cu.dim() == 1 and cu.shape[0] > 0, "cu is int32 [sequences + 1]")
-    cu = _ints(fn, "cu", cu, None)
-    n = cu.shape[0] - 1
-    _check(fn, cu_k is not None or u == t, f"{t} rows over {u} keys need their offsets cu_k")
-    cu_k = cu if cu_k is None else _ints(fn, "cu_k", cu_k, n + 1)
-    dev = _same_device(fn, q, k, v, cu, cu_k)
-    out = torch.empty((t, q_heads, width), dtype=q.dtype, device=dev)
+    k, k_row, k_head = _rows(fn, "k", k, None, width)
+    u, heads, _ = k.shape
+    v, v_row, v_head = _rows(fn, "v", v, heads, width, u)
+    dtype = q.dtype
+    if dtype not in _HALVES or k.dtype is not dtype or v.dtype is not dtype:
+        _refuse(fn, "q, k and v are all float16 or all bfloat16")
+    if width not in (64, 128, 256):
+        _refuse(fn, f"heads of {width} channels (64, 128 and 256 are served)")
+    if heads == 0 or q_heads == 0 or q_heads % heads:
+        _refuse(fn, f"{q_heads} query heads over {heads} key heads")
+    n = cu.shape[0] - 1 if cu.dim() == 1 else -1
+    if n < 0:
+        _refuse(fn, "cu is int32 [sequences + 1]")
+    cu = _ints(fn, "cu", cu, n + 1)
+    if cu_k is not None:
+        cu_k = _ints(fn, "cu_k", cu_k, n + 1)
+    elif u != t:
+        _refuse(fn, f"{t} rows over {u} keys need their offsets cu_k")
+    dev = _device(fn, q, k, v, cu, cu_k)
+    out = torch.empty((t, q_heads, width), dtype=dtype, device=q.device)
     if not t or not n:
         return out.zero_()
-    _on(dev, lambda st: call(
-        "lmoe_prompt_attend", _p(q), q.stride(0), q.stride(1), _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1),
-        dcode(q.dtype), t, u, q_heads, heads, width, _p(cu), _p(cu_k), n, float(width ** -0.5 if scale is None else scale),
-        _p(out), st))
+    _launch(dev, "lmoe_prompt_attend", q.data_ptr(), q_row, q_head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
+            dcode(dtype), t, u, q_heads, heads, width, cu.data_ptr(), (cu if cu_k is None else cu_k).data_ptr(), n,
+            width ** -0.5 if scale is None else scale, out.data_ptr())
     return out

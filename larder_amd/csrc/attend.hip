@@ -422,6 +422,7 @@ extern "C" int lmoe_kv_attend(const void *q, int dtype, long long q_row, long lo
   LMOE_REQUIRE(pages > 0 && width > 0, LMOE_ESHAPE, "%s: %d pages, a table of %d", fn, pages, width);
   if (T == 0) return 0;
   LMOE_REQUIRE(B > 0 && (cu || T == B), LMOE_ESHAPE, "%s: %d rows of %d sequences need their offsets", fn, T, B);
+  LMOE_REQUIRE(scale > 0.0f && scale < INFINITY, LMOE_EINVAL, "%s: scale %g", fn, double(scale));
   LMOE_REQUIRE(q && lens && table && k_codes && k_scale && v_codes && v_scale && out, LMOE_EINVAL, "%s: null pointer", fn);
   LMOE_REQUIRE(aligned16(q) && q_row % 8 == 0 && q_head % 8 == 0 && aligned16(k_codes) && aligned16(v_codes) && aligned16(out),
                LMOE_EALIGN, "%s: rows and codes must be 16-byte aligned", fn);

@@ -12,7 +12,7 @@
 //                      keys' scores of one row (lane & 31), the other 16 in lane ^ 32;
 //   out^T += V^T P^T   B = eight of those weights as they lie (keys 4 h + i and 8 + 4 h + i, h = lane >> 5); A = the same
 //                      keys' values of one channel, by LDS loads that transpose (ds_read_b64_tr_b16).
-// Weights are rounded to the inputs' type for the matrix cores (float16: times 2^15, so that those down to 2^-29 of a row's
+// Weights are rounded to the inputs' type for the matrix cores (float16: times 2^11, so that those down to 2^-25 of a row's
 // largest keep all their bits), and what a row is divided by is the float32 sum of the rounded weights.
 //
 // Values that a row must not see are multiplied by a weight of zero; where one is not finite in a tile that some row does
@@ -32,6 +32,14 @@ struct PromptArgs {
   int T, U, B, q_heads, heads, tiles;
 };
 
+// A weight is 2^(score - maximum in use + kLift), the maximum lagging at most kLag: float16 weights reach 2^15 at most, and
+// one 2^-25 of the largest is still a normal number
+template <bool BF>
+constexpr float kLift = BF ? 0.0f : 11.0f;
+template <bool BF>
+constexpr float kLag = BF ? 8.0f : 4.0f;
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
@@ -57,9 +65,8 @@ __device__ __forceinline__ int v_pair(int r, int p) {
 template <bool BF>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (BF) {
-    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
     typedef float f2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, bf2));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, bf16x2));
   } else {
     return __builtin_bit_cast(uint32_t, h2_t{_Float16(a), _Float16(b)});
   }
@@ -68,32 +75,38 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 template <bool BF>
 __device__ __forceinline__ float add2(uint32_t pair, float a) {
   if constexpr (BF)
-    return a + (__uint_as_float(pair << 16) + __uint_as_float(pair & 0xffff0000u));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), __builtin_bit_cast(bf16x2, 0x3f803f80u), a, false);
   else
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2_t, pair), h2_t{1.0f, 1.0f}, a, false);
 }
 
-// Fragment words of values: those not finite taken out (set to zero), and as ones in pos (NaN, +inf) and neg (NaN, -inf)
-template <bool BF>
-__device__ __forceinline__ bool take_bad(u32x4 &f, u32x4 &pos, u32x4 &neg) {
-  constexpr uint32_t INF = BF ? 0x7f80u : 0x7c00u, ONE = BF ? 0x3f80u : 0x3c00u;
-  bool any = false;
+// Values that are not finite in a tile that some row does not see whole: one thread a key and 32 channels. They are set to zero
+// in LDS and noted in two words of bits, pos (NaN, +inf) and neg (NaN, -inf); false if there are none.
+template <int D, bool BF>
+__device__ __forceinline__ bool take_bad(uint8_t *vt, int row, int c32, uint32_t *pos, uint32_t *neg) {
+  constexpr uint32_t INF = BF ? 0x7f80u : 0x7c00u;
+  uint32_t up = 0, down = 0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    pos[e] = neg[e] = 0;
+  for (int j = 0; j < 4; ++j) {
+    u32x4 *at = reinterpret_cast<u32x4 *>(vt + row * D * 2 + v_pair<D>(row, 2 * c32 + (j >> 1)) * 32 + (j & 1) * 16);
+    u32x4 w = *at;
+    bool any = false;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t v = (f[e] >> (16 * h)) & 0xffffu, mag = v & 0x7fffu;
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t x = (w[e >> 1] >> (16 * (e & 1))) & 0xffffu, mag = x & 0x7fffu;
       if (mag >= INF) {
+        const bool nan = mag > INF, minus = x >> 15;
         any = true;
-        const bool nan = mag > INF, minus = v >> 15;
-        if (nan || !minus) pos[e] |= ONE << (16 * h);
-        if (nan || minus) neg[e] |= ONE << (16 * h);
-        f[e] &= ~(0xffffu << (16 * h));
+        if (nan || !minus) up |= 1u << (8 * j + e);
+        if (nan || minus) down |= 1u << (8 * j + e);
+        w[e >> 1] &= ~(0xffffu << (16 * (e & 1)));
       }
     }
+    if (any) *at = w;
   }
-  return any;
+  *pos = up;
+  *neg = down;
+  return (up | down) != 0;
 }
 
 template <int D, int BN, bool BF>
@@ -101,6 +114,7 @@ __global__ void __launch_bounds__(256) k_prompt(PromptArgs a) {
   constexpr int MT = BN / 32, KS = D / 16, DT = D / 32, COPIES = BN * D / 512 / 4;
   constexpr int kTileBytes = BN * D * 2;
   extern __shared__ uint8_t lds[];  // [2 stages][K tile, V tile]
+  __shared__ uint32_t marks[512];   // of take_bad: [pos, neg][key][32 channels]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
   // heads of one XCD are neighbours (they share key heads in its L2); later tiles, which see more keys, go first
   const int slot = blockIdx.x % a.q_heads, task = a.tiles - 1 - int(blockIdx.x) / a.q_heads;
@@ -152,13 +166,21 @@ __global__ void __launch_bounds__(256) k_prompt(PromptArgs a) {
   };
   f32x16 o[DT] = {};
   float m = -INFINITY, l = 0.0f;
+  // a transposing load: 16 lanes take 4 keys x 16 channels, lane i of them gets channel i of the 4
+  const int vrow = 4 * h + ((lane & 15) >> 2), vpair = (lane >> 4) & 1, vbyte = (lane & 3) * 8;
   if (keys > 0) fetch(0, 0);
   for (int at = 0, stage = 0; at < keys; at += BN, stage ^= 1) {
     wait_vm<0>();
     barrier_lds();  // the tile is there, and the other stage has been read
     if (at + BN < keys) fetch(at + BN, stage ^ 1);
-    if (at >= wave_keys) continue;
     const uint8_t *kt = lds + stage * 2 * kTileBytes, *vt = kt + kTileBytes;
+    bool bad = false;
+    if (at + BN > first + off + 1) {  // the workgroup's first row does not see all of it
+      const int row = threadIdx.x / (D / 32), c32 = threadIdx.x % (D / 32);
+      if (row < BN) bad = take_bad<D, BF>(const_cast<uint8_t *>(vt), row, c32, &marks[threadIdx.x], &marks[256 + threadIdx.x]);
+      bad = __syncthreads_or(bad);
+    }
+    if (at >= wave_keys) continue;
     f32x16 s[MT] = {};
 #pragma unroll
     for (int j = 0; j < KS; ++j)
@@ -167,36 +189,39 @@ __global__ void __launch_bounds__(256) k_prompt(PromptArgs a) {
         const int row = 32 * t + r;
         s[t] = mfma32<BF>(*reinterpret_cast<const u32x4 *>(kt + row * D * 2 + k_chunk<D>(row, 2 * j + h) * 16), qf[j], s[t]);
       }
-    const bool edge = at + BN > all;
+    if (at + BN > all) {
+      const int left = opaque(sees - at - 4 * h);  // opaque: a branch, not 64 selects in every tile
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (32 * t + 8 * (e >> 2) + (e & 3) >= left) s[t][e] = -INFINITY;
+    }
     float top = -INFINITY;
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        s[t][e] *= a.scale;
-        if (edge && at + 32 * t + 8 * (e >> 2) + 4 * h + (e & 3) >= sees) s[t][e] = -INFINITY;
-        top = fmaxf(top, s[t][e]);
-      }
-    top = fmaxf(top, lane_xor32(top));
-    if (__any(top > m)) {
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[t][e]);
+    top = fmaxf(top, lane_xor32(top)) * a.scale;
+    // The maximum in use may lag by kLag octaves, so that most tiles leave the sums as they are
+    if (__any(top > m + kLag<BF>)) {
       const float to = fmaxf(m, top), keep = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
       m = to;
       l *= keep;
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] *= keep;
     }
-    const float lift = m == -INFINITY ? 0.0f : m - (BF ? 0.0f : 15.0f);
+    const float lift = m == -INFINITY ? 0.0f : kLift<BF> - m;
     u32x4 p[MT * 2];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const uint32_t w = pack2<BF>(__builtin_amdgcn_exp2f(s[t][2 * e] - lift), __builtin_amdgcn_exp2f(s[t][2 * e + 1] - lift));
+        const uint32_t w = pack2<BF>(__builtin_amdgcn_exp2f(fmaf(s[t][2 * e], a.scale, lift)),
+                                     __builtin_amdgcn_exp2f(fmaf(s[t][2 * e + 1], a.scale, lift)));
         l = add2<BF>(w, l);
         p[2 * t + (e >> 2)][e & 3] = w;
       }
-    // a transposing load: 16 lanes take 4 keys x 16 channels, lane i of them gets channel i of the 4
-    const int vrow = 4 * h + ((lane & 15) >> 2), vpair = (lane >> 4) & 1, vbyte = (lane & 3) * 8;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -206,30 +231,24 @@ __global__ void __launch_bounds__(256) k_prompt(PromptArgs a) {
         for (int x = 0; x < 2; ++x) {
           const int row = 16 * ks + 8 * x + vrow;
           const uint8_t *src = vt + row * D * 2 + v_pair<D>(row, 2 * d + vpair) * 32 + vbyte;
-          const s16x4 g = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(src));
-          const u32x2 g2 = __builtin_bit_cast(u32x2, g);
-          f[2 * x] = g2.x, f[2 * x + 1] = g2.y;
-        }
-        if (edge) {
-          u32x4 pos, neg;
-          if (__any(take_bad<BF>(f, pos, neg))) {
-            constexpr uint32_t ONE = BF ? 0x3f80u : 0x3c00u;
-            u32x4 seen;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int place = at + 16 * ks + 8 * (e >> 1) + 4 * h + 2 * (e & 1);
-              seen[e] = (place < sees ? ONE : 0) | (place + 1 < sees ? ONE << 16 : 0);
-            }
-            const f32x16 up = mfma32<BF>(pos, seen, f32x16{}), down = mfma32<BF>(neg, seen, f32x16{});
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              if (up[e] > 0.0f) o[d][e] += INFINITY;
-              if (down[e] > 0.0f) o[d][e] -= INFINITY;
-            }
-          }
+          const u32x2 g = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(src)));
+          f[2 * x] = g.x, f[2 * x + 1] = g.y;
         }
         o[d] = mfma32<BF>(f, p[ks], o[d]);
       }
+    if (bad) {
+      for (int j = 0; j < BN; ++j)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const uint32_t up = at + j < sees ? marks[j * DT + d] >> (4 * h) : 0, down = at + j < sees ? marks[256 + j * DT + d] >> (4 * h) : 0;
+          if (!__any((up | down) != 0)) continue;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if (up >> (8 * (e >> 2) + (e & 3)) & 1) o[d][e] += INFINITY;
+            if (down >> (8 * (e >> 2) + (e & 3)) & 1) o[d][e] -= INFINITY;
+          }
+        }
+    }
   }
   l += lane_xor32(l);
   if (first + 32 * wave + r >= nq) return;
@@ -259,6 +278,7 @@ extern "C" int lmoe_prompt_attend(const void *q, long long q_row, long long q_he
   LMOE_REQUIRE(T >= 0 && U >= 0 && B >= 0, LMOE_ESHAPE, "%s: %d rows, %d keys, %d sequences", fn, T, U, B);
   if (T == 0) return 0;
   LMOE_REQUIRE(B > 0, LMOE_ESHAPE, "%s: %d rows of no sequence", fn, T);
+  LMOE_REQUIRE(scale > 0.0f && scale < INFINITY, LMOE_EINVAL, "%s: scale %g", fn, double(scale));
   LMOE_REQUIRE(q && out && cu && cu_k && ((k && v) || U == 0), LMOE_EINVAL, "%s: null pointer", fn);
   LMOE_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && q_row % 8 == 0 && q_head % 8 == 0 &&
                    k_row % 8 == 0 && k_head % 8 == 0 && v_row % 8 == 0 && v_head % 8 == 0,

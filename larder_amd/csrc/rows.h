@@ -20,7 +20,7 @@ __device__ __forceinline__ int last_at(const int *cu, int B, int t, F &&first) {
     n += __popcll(le);
     if (le != ~0ull) break;
   }
-  return n - 1;
+  return __builtin_amdgcn_readfirstlane(n - 1);
 }
 
 // A sequence's rows [row0, row0 + n) of T packed ones: cu[b] .. cu[b + 1], or row b alone where cu is null. Offsets past
