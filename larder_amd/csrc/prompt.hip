@@ -22,6 +22,7 @@
 namespace lmoe {
 
 constexpr int kPromptRows = 128;
+constexpr int kAhead = 2;
 
 struct PromptArgs {
   const uint16_t *q, *k, *v;
@@ -56,10 +57,11 @@ template <int D>
 __device__ __forceinline__ int k_chunk(int r, int c) {
   return D == 64 ? c ^ ((r >> 1) & 7) : c ^ (r & 15);
 }
-// 32-byte chunk pair p of value row r: the eight rows that a transposing load takes lie in different banks
+// 32-byte chunk pair p of value row r: what 32 lanes of a transposing load take (two neighbouring pairs of four rows) lies in
+// different banks
 template <int D>
 __device__ __forceinline__ int v_pair(int r, int p) {
-  return D == 64 ? p ^ ((r >> 1) & 3) : p ^ (r & 7);
+  return D == 64 ? p ^ (r & 2) : p ^ ((r & 3) << 1) ^ ((r >> 2) & 1);
 }
 
 template <bool BF>
@@ -142,38 +144,80 @@ __global__ void __launch_bounds__(256) k_prompt(PromptArgs a) {
   const int wave_keys = min(first + 32 * wave + 31, nq - 1) + off + 1;  // what its last row sees
   const int kv = head / (a.q_heads / a.heads);
 
+  const uint32_t base = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)lds));
+  // copy i of this wavefront: 64 chunks of 16 bytes, in LDS order; the rows' chunks are permuted on the global side
+  auto fetch_k = [&](int at, int stage) {
+    const uint16_t *k = a.k + size_t(key0 + at) * a.k_row + size_t(kv) * a.k_head;
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+      const int j = (wave * COPIES + i) * 64 + lane, row = j / (D / 8), c = j % (D / 8);
+      dma<16>(k, uint32_t(min(row, nk - 1 - at)) * uint32_t(a.k_row * 2) + k_chunk<D>(row, c) * 16,
+              base + stage * kTileBytes + (wave * COPIES + i) * 1024);
+    }
+  };
+  auto fetch_v = [&](int at, int stage) {
+    const uint16_t *v = a.v + size_t(key0 + at) * a.v_row + size_t(kv) * a.v_head;
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+      const int j = (wave * COPIES + i) * 64 + lane, row = j / (D / 8), c = j % (D / 8);
+      dma<16>(v, uint32_t(min(row, nk - 1 - at)) * uint32_t(a.v_row * 2) + (v_pair<D>(row, c >> 1) * 2 + (c & 1)) * 16,
+              base + (2 + stage) * kTileBytes + (wave * COPIES + i) * 1024);
+    }
+  };
+  if (keys > 0) fetch_k(0, 0);
   u32x4 qf[KS];
   {
     const uint16_t *q = a.q + size_t(row0 + mine) * a.q_row + size_t(head) * a.q_head + 8 * h;
 #pragma unroll
     for (int j = 0; j < KS; ++j) qf[j] = *reinterpret_cast<const u32x4 *>(q + 16 * j);
   }
-  const uint32_t base = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)lds));
-  // copy i of this wavefront: 64 chunks of 16 bytes, in LDS order; the rows' chunks are permuted on the global side
-  auto fetch = [&](int at, int stage) {
-    const uint16_t *k = a.k + size_t(key0 + at) * a.k_row + size_t(kv) * a.k_head;
-    const uint16_t *v = a.v + size_t(key0 + at) * a.v_row + size_t(kv) * a.v_head;
-    const int most = nk - 1 - at;
-#pragma unroll
-    for (int i = 0; i < COPIES; ++i) {
-      const int j = (wave * COPIES + i) * 64 + lane, row = j / (D / 8), c = j % (D / 8);
-      const int from = min(row, most);
-      dma<16>(k, uint32_t(from) * uint32_t(a.k_row * 2) + k_chunk<D>(row, c) * 16,
-              base + stage * 2 * kTileBytes + (wave * COPIES + i) * 1024);
-      dma<16>(v, uint32_t(from) * uint32_t(a.v_row * 2) + (v_pair<D>(row, c >> 1) * 2 + (c & 1)) * 16,
-              base + (stage * 2 + 1) * kTileBytes + (wave * COPIES + i) * 1024);
-    }
-  };
   f32x16 o[DT] = {};
   float m = -INFINITY, l = 0.0f;
   // a transposing load: 16 lanes take 4 keys x 16 channels, lane i of them gets channel i of the 4
   const int vrow = 4 * h + ((lane & 15) >> 2), vpair = (lane >> 4) & 1, vbyte = (lane & 3) * 8;
-  if (keys > 0) fetch(0, 0);
+  auto k_frag = [&](const uint8_t *kt, int t, int j) {
+    const int row = 32 * t + r;
+    return *reinterpret_cast<const u32x4 *>(kt + row * D * 2 + k_chunk<D>(row, 2 * j + h) * 16);
+  };
+  auto v_frag = [&](const uint8_t *vt, int d, int ks) {
+    u32x4 f;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int row = 16 * ks + 8 * x + vrow;
+      const uint8_t *src = vt + row * D * 2 + v_pair<D>(row, 2 * d + vpair) * 32 + vbyte;
+      const u32x2 g = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(src)));
+      f[2 * x] = g.x, f[2 * x + 1] = g.y;
+    }
+    return f;
+  };
+  auto largest = [](const f32x16 (&x)[MT]) {
+    float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) y[e & 3] = fmaxf(y[e & 3], x[t][e]);
+    return fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+  };
+  f32x16 s[MT] = {};  // the scores of the tile at hand
+  // The compiler's own wait for q, here: it does not see the copies, and one left to the loop would wait for them too
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  if (keys > 0) {
+    wait_vm<0>();
+    barrier_lds();
+    fetch_v(0, 0);
+    if (BN < keys) fetch_k(BN, 1);
+#pragma unroll
+    for (int j = 0; j < KS; ++j)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) s[t] = mfma32<BF>(k_frag(lds, t, j), qf[j], s[t]);
+  }
+  float top = largest(s);
   for (int at = 0, stage = 0; at < keys; at += BN, stage ^= 1) {
     wait_vm<0>();
-    barrier_lds();  // the tile is there, and the other stage has been read
-    if (at + BN < keys) fetch(at + BN, stage ^ 1);
-    const uint8_t *kt = lds + stage * 2 * kTileBytes, *vt = kt + kTileBytes;
+    barrier_lds();  // this tile's values and the next one's keys are there, and what they replace has been read
+    if (at + BN < keys) fetch_v(at + BN, stage ^ 1);
+    if (at + 2 * BN < keys) fetch_k(at + 2 * BN, stage);
+    const uint8_t *kt = lds + (stage ^ 1) * kTileBytes, *vt = lds + (2 + stage) * kTileBytes;
     bool bad = false;
     if (at + BN > first + off + 1) {  // the workgroup's first row does not see all of it
       const int row = threadIdx.x / (D / 32), c32 = threadIdx.x % (D / 32);
@@ -181,14 +225,6 @@ __global__ void __launch_bounds__(256) k_prompt(PromptArgs a) {
       bad = __syncthreads_or(bad);
     }
     if (at >= wave_keys) continue;
-    f32x16 s[MT] = {};
-#pragma unroll
-    for (int j = 0; j < KS; ++j)
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const int row = 32 * t + r;
-        s[t] = mfma32<BF>(*reinterpret_cast<const u32x4 *>(kt + row * D * 2 + k_chunk<D>(row, 2 * j + h) * 16), qf[j], s[t]);
-      }
     if (at + BN > all) {
       const int left = opaque(sees - at - 4 * h);  // opaque: a branch, not 64 selects in every tile
 #pragma unroll
@@ -196,12 +232,20 @@ __global__ void __launch_bounds__(256) k_prompt(PromptArgs a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if (32 * t + 8 * (e >> 2) + (e & 3) >= left) s[t][e] = -INFINITY;
+      top = largest(s);
     }
-    float top = -INFINITY;
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[t][e]);
+    // The matrix products of a tile: the next tile's scores, then this one's output, their fragments read kAhead products ahead
+    constexpr int NM = MT * KS, NV = MT * 2 * DT, NP = MT * 8;
+    u32x4 ring[kAhead + 1];
+    auto frag = [&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      if constexpr (i < NM)
+        ring[i % (kAhead + 1)] = k_frag(kt, i % MT, i / MT);
+      else if constexpr (i < NM + NV)
+        ring[i % (kAhead + 1)] = v_frag(vt, (i - NM) % DT, (i - NM) / DT);
+    };
+    static_for<0, kAhead>([&](auto ic) { frag(ic); });
+    __builtin_amdgcn_sched_barrier(0);
     top = fmaxf(top, lane_xor32(top)) * a.scale;
     // The maximum in use may lag by kLag octaves, so that most tiles leave the sums as they are
     if (__any(top > m + kLag<BF>)) {
@@ -212,30 +256,50 @@ __global__ void __launch_bounds__(256) k_prompt(PromptArgs a) {
       for (int d = 0; d < DT; ++d) o[d] *= keep;
     }
     const float lift = m == -INFINITY ? 0.0f : kLift<BF> - m;
+    // Past the last tile the next scores are of whatever LDS holds, and unused. The vector unit's work goes between the
+    // products, in the order that leaves no instruction waiting for the one before it: a slot's pairs of weights get their
+    // exponentials, the slot before's are packed, the one before that's are summed. Half of the output products go among
+    // them (their weights are ready by then), and the next scores' maximum goes among the other half.
+    constexpr int NS = NM + NV / 2 - 2, NR = NM + NV - NS;  // slots with exponentials, and with the maximum
+    static_assert((NM - 1) * NP / NS >= 4 && (NM + NV / 2 - 1) * NP / NS >= NP, "an output product before its weights");
+    f32x16 next[MT] = {};
     u32x4 p[MT * 2];
+    float part[2] = {l, 0.0f}, peak[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, ex[NP][2];
+    auto each = [&](auto slot, auto f) {  // the pairs of a slot
+      constexpr int i = decltype(slot)::value;
+      if constexpr (i >= 0 && i < NS) static_for<i * NP / NS, (i + 1) * NP / NS>(f);
+    };
+    static_for<0, NM + NV>([&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      frag(IC<i + kAhead>{});
+      if constexpr (i < NM)
+        next[i % MT] = mfma32<BF>(ring[i % (kAhead + 1)], qf[i / MT], next[i % MT]);
+      else
+        o[(i - NM) % DT] = mfma32<BF>(ring[i % (kAhead + 1)], p[(i - NM) / DT], o[(i - NM) % DT]);
+      each(IC<i>{}, [&](auto ec) {
+        constexpr int e = decltype(ec)::value, u = e / 8, x = e % 8;
+        ex[e][0] = __builtin_amdgcn_exp2f(fmaf(s[u][2 * x], a.scale, lift));
+        ex[e][1] = __builtin_amdgcn_exp2f(fmaf(s[u][2 * x + 1], a.scale, lift));
+      });
+      each(IC<i - 1>{}, [&](auto ec) {
+        constexpr int e = decltype(ec)::value;
+        p[e / 4][e & 3] = pack2<BF>(ex[e][0], ex[e][1]);
+      });
+      each(IC<i - 2>{}, [&](auto ec) {
+        constexpr int e = decltype(ec)::value;
+        part[e & 1] = add2<BF>(p[e / 4][e & 3], part[e & 1]);
+      });
+      if constexpr (i >= NS)
+        static_for<(i - NS) * NP * 2 / NR, (i - NS + 1) * NP * 2 / NR>([&](auto ec) {
+          constexpr int e = decltype(ec)::value;
+          peak[(e >> 1) & 3] = fmaxf(peak[(e >> 1) & 3], next[e / 16][e % 16]);
+        });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    l = part[0] + part[1];
+    top = fmaxf(fmaxf(peak[0], peak[1]), fmaxf(peak[2], peak[3]));
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t w = pack2<BF>(__builtin_amdgcn_exp2f(fmaf(s[t][2 * e], a.scale, lift)),
-                                     __builtin_amdgcn_exp2f(fmaf(s[t][2 * e + 1], a.scale, lift)));
-        l = add2<BF>(w, l);
-        p[2 * t + (e >> 2)][e & 3] = w;
-      }
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int ks = 0; ks < MT * 2; ++ks) {
-        u32x4 f;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int row = 16 * ks + 8 * x + vrow;
-          const uint8_t *src = vt + row * D * 2 + v_pair<D>(row, 2 * d + vpair) * 32 + vbyte;
-          const u32x2 g = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(src)));
-          f[2 * x] = g.x, f[2 * x + 1] = g.y;
-        }
-        o[d] = mfma32<BF>(f, p[ks], o[d]);
-      }
+    for (int t = 0; t < MT; ++t) s[t] = next[t];
     if (bad) {
       for (int j = 0; j < BN; ++j)
 #pragma unroll
