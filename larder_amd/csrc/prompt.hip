@@ -5,7 +5,7 @@
 // One pass over the keys with a running maximum m. Bound by the matrix cores (4 width products a visible pair) beside the
 // exponentials on the vector unit.
 //
-// A workgroup takes 128 rows of one head, a wavefront 32 of them; keys come 64 (width 256: 32) at a time, global -> LDS
+// A workgroup takes 128 rows of one head, a wavefront 32 of them; keys come 64 at a time, global -> LDS
 // without registers, the next tile's copies in flight under the present one's products. Products are written so that
 // nothing has to change lanes between them:
 //   scores^T = K Q^T   A = 32 keys (lane & 31) x 16 channels from LDS, B = Q^T from registers: a lane ends with 16 of 32
@@ -21,8 +21,8 @@
 
 namespace lmoe {
 
-constexpr int kPromptRows = 128;
-constexpr int kAhead = 2;
+constexpr int kPromptRows = 128, kPromptKeys = 64;  // a workgroup's rows, and keys a tile
+constexpr int kAhead = 3;  // products that a fragment is read ahead of its own
 
 struct PromptArgs {
   const uint16_t *q, *k, *v;
@@ -73,6 +73,11 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return __builtin_bit_cast(uint32_t, h2_t{_Float16(a), _Float16(b)});
   }
 }
+// One wavefront-wide copy of 16 bytes a lane, from voff in what the descriptor covers, to LDS address lds + 16 lane
+__device__ __forceinline__ void dma_rows(u32x4 rows, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rows), "s"(lds) : "memory");
+}
+
 // a + the pair's two values
 template <bool BF>
 __device__ __forceinline__ float add2(uint32_t pair, float a) {
@@ -111,12 +116,22 @@ __device__ __forceinline__ bool take_bad(uint8_t *vt, int row, int c32, uint32_t
   return (up | down) != 0;
 }
 
-template <int D, int BN, bool BF>
-__global__ void __launch_bounds__(256) k_prompt(PromptArgs a) {
-  constexpr int MT = BN / 32, KS = D / 16, DT = D / 32, COPIES = BN * D / 512 / 4;
+// Whether every output product's weights are packed a slot before it: NM score products, NV output products over NP pairs of
+// weights, DT channel tiles, pairs spread over NS slots and packed one slot later
+constexpr bool weights_in_time(int NM, int NV, int NP, int DT, int NS) {
+  for (int k = 0; k < NV; ++k) {
+    const int slots = NM + k - 1 < NS ? NM + k - 1 : NS;
+    if (slots * NP / NS < 4 * (k / DT + 1)) return false;
+  }
+  return true;
+}
+
+template <int D, bool BF>
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_prompt(PromptArgs a) {
+  constexpr int BN = kPromptKeys, MT = BN / 32, KS = D / 16, DT = D / 32, COPIES = BN * D / 512 / 4;
   constexpr int kTileBytes = BN * D * 2;
   extern __shared__ uint8_t lds[];  // [2 stages][K tile, V tile]
-  __shared__ uint32_t marks[512];   // of take_bad: [pos, neg][key][32 channels]
+  __shared__ uint32_t marks[2 * BN * DT];   // of take_bad: [pos, neg][key][32 channels]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
   // heads of one XCD are neighbours (they share key heads in its L2); later tiles, which see more keys, go first
   const int slot = blockIdx.x % a.q_heads, task = a.tiles - 1 - int(blockIdx.x) / a.q_heads;
@@ -140,29 +155,36 @@ __global__ void __launch_bounds__(256) k_prompt(PromptArgs a) {
   const int off = nk - nq;                                  // row i sees keys 0 .. i + off
   const int keys = off + min(first + kPromptRows, nq);      // what the workgroup's last row sees
   const int mine = min(first + 32 * wave + r, nq - 1), sees = mine + off + 1;
-  const int all = first + 32 * wave + off + 1;              // what every row of the wavefront sees
-  const int wave_keys = min(first + 32 * wave + 31, nq - 1) + off + 1;  // what its last row sees
+  const int all = first + 32 * wave + off + 1;  // what every row of the wavefront sees
   const int kv = head / (a.q_heads / a.heads);
 
   const uint32_t base = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)lds));
-  // copy i of this wavefront: 64 chunks of 16 bytes, in LDS order; the rows' chunks are permuted on the global side
-  auto fetch_k = [&](int at, int stage) {
-    const uint16_t *k = a.k + size_t(key0 + at) * a.k_row + size_t(kv) * a.k_head;
+  // Copy i of this wavefront: 64 chunks of 16 bytes in LDS order; the rows' chunks are permuted on the global side. A tile's
+  // copies go through a descriptor that ends with the sequence's last key: rows past it are not read.
+  uint32_t k_off[COPIES], v_off[COPIES];
 #pragma unroll
-    for (int i = 0; i < COPIES; ++i) {
-      const int j = (wave * COPIES + i) * 64 + lane, row = j / (D / 8), c = j % (D / 8);
-      dma<16>(k, uint32_t(min(row, nk - 1 - at)) * uint32_t(a.k_row * 2) + k_chunk<D>(row, c) * 16,
-              base + stage * kTileBytes + (wave * COPIES + i) * 1024);
-    }
+  for (int i = 0; i < COPIES; ++i) {
+    const int j = (wave * COPIES + i) * 64 + lane, row = j / (D / 8), c = j % (D / 8);
+    k_off[i] = uint32_t(row) * uint32_t(a.k_row * 2) + k_chunk<D>(row, c) * 16;
+    v_off[i] = uint32_t(row) * uint32_t(a.v_row * 2) + (v_pair<D>(row, c >> 1) * 2 + (c & 1)) * 16;
+  }
+  auto tile_of_rows = [&](const uint16_t *p, long long stride, int at) {
+    const uint64_t from = reinterpret_cast<uint64_t>(p + (long long)min(at, nk) * stride);
+    const long long bytes = at < nk ? ((nk - 1 - at) * stride + D) * 2 : 0;
+    return u32x4{uint32_t(from), uint32_t(from >> 32) & 0xffffu, uint32_t(min(bytes, 1ll << 31)), 0x00020000u};
+  };
+  const uint16_t *k_rows = a.k + size_t(key0) * a.k_row + size_t(kv) * a.k_head;
+  const uint16_t *v_rows = a.v + size_t(key0) * a.v_row + size_t(kv) * a.v_head;
+  const uint32_t to = base + wave * COPIES * 1024;
+  auto fetch_k = [&](int at, int stage) {
+    const u32x4 rows = tile_of_rows(k_rows, a.k_row, at);
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) dma_rows(rows, k_off[i], to + stage * kTileBytes + i * 1024);
   };
   auto fetch_v = [&](int at, int stage) {
-    const uint16_t *v = a.v + size_t(key0 + at) * a.v_row + size_t(kv) * a.v_head;
+    const u32x4 rows = tile_of_rows(v_rows, a.v_row, at);
 #pragma unroll
-    for (int i = 0; i < COPIES; ++i) {
-      const int j = (wave * COPIES + i) * 64 + lane, row = j / (D / 8), c = j % (D / 8);
-      dma<16>(v, uint32_t(min(row, nk - 1 - at)) * uint32_t(a.v_row * 2) + (v_pair<D>(row, c >> 1) * 2 + (c & 1)) * 16,
-              base + (2 + stage) * kTileBytes + (wave * COPIES + i) * 1024);
-    }
+    for (int i = 0; i < COPIES; ++i) dma_rows(rows, v_off[i], to + (2 + stage) * kTileBytes + i * 1024);
   };
   if (keys > 0) fetch_k(0, 0);
   u32x4 qf[KS];
@@ -205,26 +227,32 @@ __global__ void __launch_bounds__(256) k_prompt(PromptArgs a) {
     wait_vm<0>();
     barrier_lds();
     fetch_v(0, 0);
-    if (BN < keys) fetch_k(BN, 1);
+    fetch_k(BN, 1);
 #pragma unroll
     for (int j = 0; j < KS; ++j)
 #pragma unroll
       for (int t = 0; t < MT; ++t) s[t] = mfma32<BF>(k_frag(lds, t, j), qf[j], s[t]);
   }
   float top = largest(s);
-  for (int at = 0, stage = 0; at < keys; at += BN, stage ^= 1) {
+  // one tile: its scores s become next, the following tile's. Called with the two in turn, so that nothing is moved.
+  auto step = [&](int at, auto stage_c, f32x16 (&s)[MT], f32x16 (&next)[MT]) {
+    constexpr int stage = decltype(stage_c)::value;
     wait_vm<0>();
     barrier_lds();  // this tile's values and the next one's keys are there, and what they replace has been read
-    if (at + BN < keys) fetch_v(at + BN, stage ^ 1);
-    if (at + 2 * BN < keys) fetch_k(at + 2 * BN, stage);
+    const u32x4 k_tile = tile_of_rows(k_rows, a.k_row, at + 2 * BN), v_tile = tile_of_rows(v_rows, a.v_row, at + BN);
+    auto copy = [&](int i) {  // copy i of the next tile's values and of the keys after that
+      if (i < COPIES)
+        dma_rows(v_tile, v_off[i], to + (2 + (stage ^ 1)) * kTileBytes + i * 1024);
+      else
+        dma_rows(k_tile, k_off[i - COPIES], to + stage * kTileBytes + (i - COPIES) * 1024);
+    };
     const uint8_t *kt = lds + (stage ^ 1) * kTileBytes, *vt = lds + (2 + stage) * kTileBytes;
     bool bad = false;
     if (at + BN > first + off + 1) {  // the workgroup's first row does not see all of it
-      const int row = threadIdx.x / (D / 32), c32 = threadIdx.x % (D / 32);
-      if (row < BN) bad = take_bad<D, BF>(const_cast<uint8_t *>(vt), row, c32, &marks[threadIdx.x], &marks[256 + threadIdx.x]);
+      for (int i = threadIdx.x; i < BN * DT; i += 256)
+        bad |= take_bad<D, BF>(const_cast<uint8_t *>(vt), i / DT, i % DT, &marks[i], &marks[BN * DT + i]);
       bad = __syncthreads_or(bad);
     }
-    if (at >= wave_keys) continue;
     if (at + BN > all) {
       const int left = opaque(sees - at - 4 * h);  // opaque: a branch, not 64 selects in every tile
 #pragma unroll
@@ -261,10 +289,9 @@ __global__ void __launch_bounds__(256) k_prompt(PromptArgs a) {
     // exponentials, the slot before's are packed, the one before that's are summed. Half of the output products go among
     // them (their weights are ready by then), and the next scores' maximum goes among the other half.
     constexpr int NS = NM + NV / 2 - 2, NR = NM + NV - NS;  // slots with exponentials, and with the maximum
-    static_assert((NM - 1) * NP / NS >= 4 && (NM + NV / 2 - 1) * NP / NS >= NP, "an output product before its weights");
-    f32x16 next[MT] = {};
     u32x4 p[MT * 2];
     float part[2] = {l, 0.0f}, peak[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, ex[NP][2];
+    static_assert(weights_in_time(NM, NV, NP, DT, NS), "an output product before its weights");
     auto each = [&](auto slot, auto f) {  // the pairs of a slot
       constexpr int i = decltype(slot)::value;
       if constexpr (i >= 0 && i < NS) static_for<i * NP / NS, (i + 1) * NP / NS>(f);
@@ -272,8 +299,9 @@ __global__ void __launch_bounds__(256) k_prompt(PromptArgs a) {
     static_for<0, NM + NV>([&](auto ic) {
       constexpr int i = decltype(ic)::value;
       frag(IC<i + kAhead>{});
+      if constexpr (i % 2 == 0 && i < 4 * COPIES) copy(i / 2);
       if constexpr (i < NM)
-        next[i % MT] = mfma32<BF>(ring[i % (kAhead + 1)], qf[i / MT], next[i % MT]);
+        next[i % MT] = mfma32<BF>(ring[i % (kAhead + 1)], qf[i / MT], i < MT ? f32x16{} : next[i % MT]);
       else
         o[(i - NM) % DT] = mfma32<BF>(ring[i % (kAhead + 1)], p[(i - NM) / DT], o[(i - NM) % DT]);
       each(IC<i>{}, [&](auto ec) {
@@ -298,13 +326,11 @@ __global__ void __launch_bounds__(256) k_prompt(PromptArgs a) {
     });
     l = part[0] + part[1];
     top = fmaxf(fmaxf(peak[0], peak[1]), fmaxf(peak[2], peak[3]));
-#pragma unroll
-    for (int t = 0; t < MT; ++t) s[t] = next[t];
     if (bad) {
       for (int j = 0; j < BN; ++j)
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          const uint32_t up = at + j < sees ? marks[j * DT + d] >> (4 * h) : 0, down = at + j < sees ? marks[256 + j * DT + d] >> (4 * h) : 0;
+          const uint32_t up = at + j < sees ? marks[j * DT + d] >> (4 * h) : 0, down = at + j < sees ? marks[BN * DT + j * DT + d] >> (4 * h) : 0;
           if (!__any((up | down) != 0)) continue;
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -313,7 +339,14 @@ __global__ void __launch_bounds__(256) k_prompt(PromptArgs a) {
           }
         }
     }
+  };
+  f32x16 other[MT];
+  for (int at = 0; at < keys; at += 2 * BN) {
+    step(at, IC<0>{}, s, other);
+    if (at + BN >= keys) break;
+    step(at + BN, IC<1>{}, other, s);
   }
+  wait_vm<0>();  // the last tiles' copies (of nothing) land before the LDS is another workgroup's
   l += lane_xor32(l);
   if (first + 32 * wave + r >= nq) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -354,15 +387,15 @@ extern "C" int lmoe_prompt_attend(const void *q, long long q_row, long long q_he
   PromptArgs a = {static_cast<const uint16_t *>(q), static_cast<const uint16_t *>(k), static_cast<const uint16_t *>(v), q_row,
                   q_head, k_row, k_head, v_row, v_head, cu, cu_k, static_cast<uint16_t *>(out), scale * 1.4426950408889634f, T, U,
                   B, q_heads, heads, int(tiles)};
-  auto go = [&](auto kernel, int bn) -> int {
-    const size_t lds = size_t(bn) * D * 2 * 4;
+  auto go = [&](auto kernel) -> int {
+    const size_t lds = size_t(kPromptKeys) * D * 2 * 4;
     if (const int rc = allow_lds(kernel, lds, fn)) return rc;
     launch(kernel, dim3(unsigned(tiles * q_heads)), dim3(256), lds, (hipStream_t)stream, a);
     LMOE_LAUNCHED(fn);
     return 0;
   };
   const bool bf = dtype == LMOE_BF16;
-  if (D == 64) return bf ? go(k_prompt<64, 64, true>, 64) : go(k_prompt<64, 64, false>, 64);
-  if (D == 128) return bf ? go(k_prompt<128, 64, true>, 64) : go(k_prompt<128, 64, false>, 64);
-  return bf ? go(k_prompt<256, 32, true>, 32) : go(k_prompt<256, 32, false>, 32);
+  if (D == 64) return bf ? go(k_prompt<64, true>) : go(k_prompt<64, false>);
+  if (D == 128) return bf ? go(k_prompt<128, true>) : go(k_prompt<128, false>);
+  return bf ? go(k_prompt<256, true>) : go(k_prompt<256, false>);
 }
