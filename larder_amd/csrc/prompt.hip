@@ -92,7 +92,15 @@ __device__ __forceinline__ float add2(uint32_t pair, float a) {
 template <int D, bool BF>
 __device__ __forceinline__ bool take_bad(uint8_t *vt, int row, int c32, uint32_t *pos, uint32_t *neg) {
   constexpr uint32_t INF = BF ? 0x7f80u : 0x7c00u;
-  uint32_t up = 0, down = 0;
+  uint32_t up = 0, down = 0, any_bad = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {  // a half word's magnitude of INF or more carries into its sign bit
+    const u32x4 w = *reinterpret_cast<const u32x4 *>(vt + row * D * 2 + v_pair<D>(row, 2 * c32 + (j >> 1)) * 32 + (j & 1) * 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) any_bad |= (w[e] & 0x7fff7fffu) + (0x8000u - INF) * 0x10001u;
+  }
+  *pos = *neg = 0;
+  if (!(any_bad & 0x80008000u)) return false;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     u32x4 *at = reinterpret_cast<u32x4 *>(vt + row * D * 2 + v_pair<D>(row, 2 * c32 + (j >> 1)) * 32 + (j & 1) * 16);
@@ -113,7 +121,7 @@ __device__ __forceinline__ bool take_bad(uint8_t *vt, int row, int c32, uint32_t
   }
   *pos = up;
   *neg = down;
-  return (up | down) != 0;
+  return true;
 }
 
 // Whether every output product's weights are packed a slot before it: NM score products, NV output products over NP pairs of
@@ -186,7 +194,11 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_prompt(PromptArgs a) 
 #pragma unroll
     for (int i = 0; i < COPIES; ++i) dma_rows(rows, v_off[i], to + (2 + stage) * kTileBytes + i * 1024);
   };
-  if (keys > 0) fetch_k(0, 0);
+  if (keys > 0) {
+    fetch_k(0, 0);
+    fetch_v(0, 0);
+    fetch_k(BN, 1);
+  }
   u32x4 qf[KS];
   {
     const uint16_t *q = a.q + size_t(row0 + mine) * a.q_row + size_t(head) * a.q_head + 8 * h;
@@ -226,8 +238,6 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_prompt(PromptArgs a) 
   if (keys > 0) {
     wait_vm<0>();
     barrier_lds();
-    fetch_v(0, 0);
-    fetch_k(BN, 1);
 #pragma unroll
     for (int j = 0; j < KS; ++j)
 #pragma unroll
