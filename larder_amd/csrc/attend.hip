@@ -16,9 +16,11 @@
 // 2^-29 of the row's largest keeps all eleven bits (a long context under one token that stands out lives there). The scales
 // multiply float32 sums.
 //
-// A workgroup is four wavefronts, taking turns at the 32-token tiles of one chunk of one sequence; they join in LDS, and
-// where a sequence has more than one chunk a second kernel joins those. Chunks have one length, so ragged sequences give
-// equal workgroups; those past a sequence's end leave at once.
+// All of a call's work lies on one line of units of 128 tokens (one 32-token tile for each of a workgroup's four wavefronts):
+// sequence by sequence, in it each tile of 16 rows and key head, in that the sequence's units in order. As many workgroups as
+// the GPU holds at once take equal stretches of the line, whatever the sequences' lengths. A workgroup finishes the items
+// that lie in its stretch whole; the two that may reach over its ends go to its two places in the workspace, and a second
+// kernel joins those. Where sequences are short, each is one unit and there is nothing to join.
 #include "rows.h"
 
 namespace lmoe {
@@ -26,17 +28,83 @@ namespace lmoe {
 constexpr int kAttendWaves = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
+constexpr int kUnit = 32 * kAttendWaves;  // tokens
+// A weight is 2^(score - maximum in use + kLift), the maximum lagging at most kLag behind
+constexpr float kLift = 11.0f, kLag = 4.0f;
+
 struct AttendArgs {
   const void *q;
   long long q_row, q_head;
   const uint8_t *kc, *vc;
   const float *ks, *vs;
   const int *table, *lens, *cu;
-  void *out;        // [T][q_heads][D]
-  float *part;      // [T q_heads][chunks] of D sums, then [T q_heads][chunks] of {maximum, weight}; null: one chunk
-  float scale;      // times log2 e
-  int T, B, q_heads, heads, page_shift, pages, width, group, row_tiles, chunk, chunks;
+  void *out;    // [T][q_heads][D]
+  float *part;  // [workgroups][2] of [16 rows][D] sums and [16 rows] of {maximum, weight}; null: an item is one unit
+  float scale;  // times log2 e
+  int T, B, q_heads, heads, page_shift, pages, width, group, groups;  // groups: workgroups of k_attend
 };
+
+// A sequence's share of the line
+struct Share {
+  int row0, n, len, tiles, units;  // rows, tokens, tiles of 16 (row, query head of the group) pairs, units an item
+  __device__ __forceinline__ long long total(int heads) const { return (long long)tiles * heads * units; }
+};
+__device__ __forceinline__ Share share_of(const AttendArgs &a, int b) {
+  Share s;
+  seq_rows(a.cu, b, a.T, &s.row0, &s.n);
+  s.len = a.lens[b];
+  s.tiles = (s.n * a.group + 15) >> 4;
+  s.units = a.part ? (min(max(s.len, 1), a.width << a.page_shift) + kUnit - 1) / kUnit : 1;
+  return s;
+}
+
+// The line's length and, by one wavefront, where sequence `until` (or that of unit `unit`) begins on it
+__device__ __forceinline__ long long wave_scan(long long v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const long long u = __shfl_up(v, d);
+    if ((threadIdx.x & 63) >= d) v += u;
+  }
+  return v;
+}
+__device__ __forceinline__ long long lane_i64(long long v, int l) {
+  const uint32_t lo = __builtin_amdgcn_readlane(uint32_t(v), l), hi = __builtin_amdgcn_readlane(uint32_t(v >> 32), l);
+  return (long long)(uint64_t(hi) << 32 | lo);
+}
+__device__ __forceinline__ long long line_length(const AttendArgs &a) {
+  long long sum = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int b = b0 + (threadIdx.x & 63);
+    sum += lane_i64(wave_scan(b < a.B ? share_of(a, b).total(a.heads) : 0), 63);
+  }
+  return sum;
+}
+// the sequence that has unit `unit` (of a line longer than that), and where it begins
+__device__ __forceinline__ int sequence_of(const AttendArgs &a, long long unit, long long *begins) {
+  long long base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int b = b0 + (threadIdx.x & 63);
+    const long long own = b < a.B ? share_of(a, b).total(a.heads) : 0, sum = wave_scan(own);
+    const unsigned long long past = __ballot(base + sum > unit);
+    if (past) {
+      const int l = __ffsll(past) - 1;
+      *begins = base + lane_i64(sum - own, l);
+      return __builtin_amdgcn_readfirstlane(b0 + l);
+    }
+    base += lane_i64(sum, 63);
+  }
+  *begins = base;
+  return a.B;
+}
+// where sequence `which` begins
+__device__ __forceinline__ long long begin_of(const AttendArgs &a, int which) {
+  long long base = 0;
+  for (int b0 = 0; b0 < which; b0 += 64) {
+    const int b = b0 + (threadIdx.x & 63);
+    base += lane_i64(wave_scan(b < which ? share_of(a, b).total(a.heads) : 0), 63);
+  }
+  return base;
+}
 
 template <bool BF>
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
@@ -55,11 +123,8 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
 }
 
-// whether one of a word's four codes is NaN
-__device__ __forceinline__ bool nan_code(uint32_t w) {
-  const uint32_t m = ~w & 0x7f7f7f7fu;  // a NaN's byte is zero here, and no byte has its top bit
-  return ((m - 0x01010101u) & ~m & 0x80808080u) != 0;
-}
+// 0x80 in the place of each of a word's four codes that is NaN
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ~((~w & 0x7f7f7f7fu) + 0x7f7f7f7fu) & 0x80808080u; }
 
 // One wavefront's raw codes of 32 tokens of a head
 template <int D>
@@ -106,44 +171,67 @@ __device__ __forceinline__ void v_fragments(const uint32_t (&a)[8], u32x4 (&f)[4
 }
 
 template <int D>
-__device__ __forceinline__ void zero_rows(const AttendArgs &a, int head, int from, int to) {
-  const int per = a.group * D / 8;
-  for (long long i = threadIdx.x; i < (long long)(to - from) * per; i += 64 * kAttendWaves) {
-    const int row = int(i / per), j = int(i - (long long)row * per);
-    *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(a.out) + (size_t(from + row) * a.q_heads + head * a.group) * D +
-                               j * 8) = u32x4{};
-  }
+__device__ __forceinline__ void zero_rows(const AttendArgs &a, int from, int to) {
+  const long long per = (long long)a.q_heads * D / 8;
+  u32x4 *out = reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(a.out) + size_t(from) * a.q_heads * D);
+  for (long long i = threadIdx.x; i < (to - from) * per; i += 64 * kAttendWaves) out[i] = u32x4{};
 }
 
+template <bool BF>
+__device__ __forceinline__ void store4(void *out, size_t at, f32x4 v, float weight) {
+  const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
+  u32x2 w;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    w[j] = BF ? uint32_t(f32_to_bf16(v[2 * j] * inv)) | uint32_t(f32_to_bf16(v[2 * j + 1] * inv)) << 16
+              : __builtin_bit_cast(uint32_t, h2_t{_Float16(v[2 * j] * inv), _Float16(v[2 * j + 1] * inv)});
+  *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(out) + at) = w;
+}
+
+template <int D>
+constexpr int kPlace = 16 * (D + 2);  // floats of a place in the workspace
+
 template <int D, bool BF>
-__global__ void __launch_bounds__(64 * kAttendWaves) k_attend(AttendArgs a) {
+__global__ void __launch_bounds__(64 * kAttendWaves, D == 256 ? 2 : 3) k_attend(AttendArgs a) {
   constexpr int NC = D / 64, NT = D / 16;  // 64-channel groups, 16-channel tiles
   extern __shared__ float lds[];           // [wave][16 rows][D] sums, then [wave][16] maxima, [wave][16] weights
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-  const int head = blockIdx.y / a.row_tiles, b = blockIdx.z;
-  int row0, n;
-  seq_rows(a.cu, b, a.T, &row0, &n);
-  if (!a.part && blockIdx.y % a.row_tiles == 0 && a.cu) {
-    // rows before the first sequence or behind the last one come back zero (the joining kernel does it where there is one)
-    const int from = b == 0 ? 0 : a.T, to = b == 0 ? min(max(a.cu[0], 0), a.T) : a.T;
-    zero_rows<D>(a, head, from, to);
-    if (b == a.B - 1) zero_rows<D>(a, head, min(max(a.cu[a.B], 0), a.T), a.T);
+  if (blockIdx.x == 0 && a.cu) {  // rows before the first sequence or behind the last one come back zero
+    zero_rows<D>(a, 0, min(max(a.cu[0], 0), a.T));
+    zero_rows<D>(a, min(max(a.cu[a.B], 0), a.T), a.T);
   }
-  const int rows = n * a.group, page_tokens = 1 << a.page_shift, len = a.lens[b];
-  const int begin = blockIdx.x * a.chunk;
-  // the row tiles and the last chunk go on past what the caller said of the longest sequence and the most rows
-  for (int rt = blockIdx.y - head * a.row_tiles; 16 * rt < rows; rt += a.row_tiles) {
+  const long long line = line_length(a);
+  long long at_unit = line * blockIdx.x / a.groups;
+  const long long stop_unit = line * (blockIdx.x + 1) / a.groups;
+  if (at_unit >= stop_unit) return;
+  const long long first_unit = at_unit;
+  long long base;
+  int b = sequence_of(a, at_unit, &base);
+  Share s = share_of(a, b);
+  const int page_tokens = 1 << a.page_shift;
+  const size_t head_bytes = size_t(page_tokens) * D, page_bytes = head_bytes * a.heads;
+
+  while (at_unit < stop_unit) {
+    while (at_unit >= base + s.total(a.heads)) {  // on to the next sequence that has rows
+      base += s.total(a.heads);
+      s = share_of(a, ++b);
+    }
+    const int item = int((at_unit - base) / s.units), unit0 = int((at_unit - base) - (long long)item * s.units);
+    const int units = int(min((long long)(s.units - unit0), stop_unit - at_unit));
+    const int rt = item / a.heads, head = item - rt * a.heads, rows = s.n * a.group;
+    const bool whole = units == s.units;
     const int last = min(16 * rt + 15, rows - 1) / a.group;
-    int end = len - n + last + 1;  // this workgroup's tokens: [begin, end)
-    if (int(blockIdx.x) + 1 < a.chunks) end = min(end, begin + a.chunk);
-    if (begin >= end && a.part) continue;
+    // this stretch's tokens [begin, end): an item's last unit ends with what its last row sees
+    const int begin = unit0 * kUnit;
+    int end = s.len - s.n + last + 1;
+    if (unit0 + units < s.units) end = min(end, begin + units * kUnit);
     // the lane's row: query row `mine` of the sequence, seeing the first `sees` places; every row sees those below `all`
     const int flat = min(16 * rt + r, rows - 1), mine = flat / a.group, sub = flat - mine * a.group;
-    const int sees = len - n + mine + 1, all = len - n + (16 * rt) / a.group + 1;
+    const int sees = s.len - s.n + mine + 1, all = s.len - s.n + (16 * rt) / a.group + 1;
 
     u32x4 qf[2 * NC];
     {
-      const uint16_t *q = static_cast<const uint16_t *>(a.q) + size_t(row0 + mine) * a.q_row +
+      const uint16_t *q = static_cast<const uint16_t *>(a.q) + size_t(s.row0 + mine) * a.q_row +
                           size_t(head * a.group + sub) * a.q_head + 16 * g;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
@@ -153,8 +241,8 @@ __global__ void __launch_bounds__(64 * kAttendWaves) k_attend(AttendArgs a) {
     }
     f32x4 o[NT] = {};
     float m = -INFINITY, l = 0.0f;
-    const int first = begin / 32 + wave, stop = (max(end, begin) + 31) / 32, tiles = max(0, (stop - first + 3) / 4);
-    const size_t head_bytes = size_t(page_tokens) * D, page_bytes = head_bytes * a.heads;
+    uint8_t *marks = reinterpret_cast<uint8_t *>(lds + wave * 16 * D);
+    const int first = begin / 32 + wave, tiles = max(0, ((max(end, begin) + 31) / 32 - first + 3) / 4);
 
     for (int t0 = 0; t0 < tiles; t0 += 64) {
       // the pages and scales of this wavefront's next 64 tiles, one a lane
@@ -175,62 +263,69 @@ __global__ void __launch_bounds__(64 * kAttendWaves) k_attend(AttendArgs a) {
         const int place = (first + 4 * (t0 + i)) * 32 & (page_tokens - 1);
         load_codes<D>(c, a.kc, a.vc, size_t(page) * page_bytes + size_t(head) * head_bytes + size_t(place) * D, lane);
       };
-      Codes<D> next;
-      fetch(next, 0);
-      for (int i = 0; i < nt; ++i) {
-        Codes<D> c = next;
-        if (i + 1 < nt) fetch(next, i + 1);
+      auto work = [&](Codes<D> &c, int i) {
         const int at = (first + 4 * (t0 + i)) * 32;
-        const bool there = __builtin_amdgcn_readlane(number, i) >= 0;
+        const bool held = __builtin_amdgcn_readlane(number, i) >= 0;
         const float k_scale = lane_value(ks, i) * a.scale, v_scale = lane_value(vs, i);
-        if (!there) continue;
-        f32x4 s[2] = {};
+        f32x4 sc[2] = {};
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int j = 0; j < NC; ++j) {
             const u32x4 w = c.k[h][j];
-            s[h] = mfma16<BF>(u32x4{codes2<BF, false>(w.x), codes2<BF, true>(w.x), codes2<BF, false>(w.y), codes2<BF, true>(w.y)},
-                              qf[2 * j], s[h]);
-            s[h] = mfma16<BF>(u32x4{codes2<BF, false>(w.z), codes2<BF, true>(w.z), codes2<BF, false>(w.w), codes2<BF, true>(w.w)},
-                              qf[2 * j + 1], s[h]);
+            sc[h] = mfma16<BF>(
+                u32x4{codes2<BF, false>(w.x), codes2<BF, true>(w.x), codes2<BF, false>(w.y), codes2<BF, true>(w.y)}, qf[2 * j],
+                sc[h]);
+            sc[h] = mfma16<BF>(
+                u32x4{codes2<BF, false>(w.z), codes2<BF, true>(w.z), codes2<BF, false>(w.w), codes2<BF, true>(w.w)},
+                qf[2 * j + 1], sc[h]);
           }
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3] * k_scale;
-        const bool edge = at + 32 > all || at + 32 > end;  // some row does not see all of the tile
+        for (int e = 0; e < 8; ++e) x[e] = sc[e >> 2][e & 3] * k_scale;
         bool poison = false;
-        if (edge) {
-          bool bad = false;
+        if (!held || at + 32 > all || at + 32 > end) {  // some row does not see all of the tile
+          const int there = opaque(held ? end - at - 4 * g : 0), left = min(there, sees - at - 4 * g);
+          uint32_t bad = 0;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const int place = at + 4 * g + (e & 3) + 16 * (e >> 2);
-            if (place >= min(sees, end)) x[e] = -INFINITY;
+            const int place = (e & 3) + 16 * (e >> 2);
+            if (place >= left) x[e] = -INFINITY;
             // places past the last row's: whatever the page holds there must not reach a product (0 NaN is NaN)
 #pragma unroll
             for (int w = 0; w < NC; ++w) {
-              if (place >= end) c.v[e][w] = 0;
-              bad |= nan_code(c.v[e][w]);
+              if (place >= there) c.v[e][w] = 0;
+              bad |= nan_codes(c.v[e][w]);
             }
           }
-          poison = __any(bad);
+          poison = __any(bad != 0);
+          if (poison) {  // NaN among tokens that not every row sees: taken out, and noted in LDS by token and four channels
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+              for (int w = 0; w < NC; ++w) {
+                const uint32_t z = nan_codes(c.v[e][w]) >> 7;
+                c.v[e][w] &= ~(z * 0xffu);
+                marks[(4 * g + (e & 3) + 16 * (e >> 2)) * (D / 4) + r * NC + w] = uint8_t(z | z >> 7 | z >> 14 | z >> 21);
+              }
+          }
         }
         float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
         top = fmaxf(top, lane_xor16(top));
         top = fmaxf(top, lane_xor32(top));
-        if (__any(top > m)) {
+        if (__any(top > m + kLag)) {
           const float to = fmaxf(m, top), keep = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
           m = to;
           l *= keep;
 #pragma unroll
           for (int d = 0; d < NT; ++d) o[d] *= keep;
         }
-        const float off = m == -INFINITY ? 0.0f : m - 15.0f;
+        const float lift = m == -INFINITY ? 0.0f : kLift - m;
         u32x4 p;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const h2_t w = {_Float16(__builtin_amdgcn_exp2f(x[2 * e] - off)), _Float16(__builtin_amdgcn_exp2f(x[2 * e + 1] - off))};
-          l = __builtin_amdgcn_fdot2(w, h2_t{1.0f, 1.0f}, l, false);  // the rounded weights: their sum is what they are divided by
+          const h2_t w = {_Float16(__builtin_amdgcn_exp2f(x[2 * e] + lift)), _Float16(__builtin_amdgcn_exp2f(x[2 * e + 1] + lift))};
+          l = __builtin_amdgcn_fdot2(w, h2_t{1.0f, 1.0f}, l, false);  // the rounded weights' sum is what the row is divided by
           p[e] = __builtin_bit_cast(uint32_t, w);
         }
 #pragma unroll
@@ -240,33 +335,44 @@ __global__ void __launch_bounds__(64 * kAttendWaves) k_attend(AttendArgs a) {
           for (int e = 0; e < 8; ++e) v[e] = c.v[e][w];
           u32x4 f[4];
           v_fragments(v, f);
-          if (poison) {  // a NaN among tokens that not every row sees: it goes to the rows that see it alone
-            u32x4 seen;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              seen[e] = (x[2 * e] == -INFINITY ? 0u : 0x3c00u) | (x[2 * e + 1] == -INFINITY ? 0u : 0x3c000000u);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              u32x4 mark;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t lo = f[j][e] & 0x7fffu, hi = f[j][e] & 0x7fff0000u;
-                mark[e] = (lo > 0x7c00u ? 0x3c00u : 0u) | (hi > 0x7c000000u ? 0x3c000000u : 0u);
-                if (lo > 0x7c00u) f[j][e] &= 0xffff0000u;
-                if (hi > 0x7c000000u) f[j][e] &= 0x0000ffffu;
-              }
-              const f32x4 hit = mfma16<false>(mark, seen, f32x4{});
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (hit[e] > 0.0f) o[4 * w + j][e] = NAN;
-            }
-          }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const f32x4 y = mfma16<false>(f[j], p, f32x4{});
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[4 * w + j][e] = fmaf(y[e], v_scale, o[4 * w + j][e]);
           }
+        }
+        if (poison) {  // and given to the rows that do see them
+          for (int place = 0; place < 32; ++place)
+#pragma unroll
+            for (int i = 0; i < 4 * NC; ++i) {
+              const uint32_t z = at + place < sees ? marks[place * (D / 4) + (4 * g + i / NC) * NC + i % NC] : 0;
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (z >> j & 1) o[4 * (i % NC) + j][i / NC] = NAN;
+            }
+        }
+      };
+      if constexpr (D < 256) {  // two sets of codes in turn, so that none is moved; at width 256 there are no registers for that
+        Codes<D> one, two;
+        fetch(one, 0);
+        int i = 0;
+        for (; i + 2 < nt; i += 2) {
+          fetch(two, i + 1);
+          work(one, i);
+          fetch(one, i + 2);
+          work(two, i + 1);
+        }
+        if (i + 1 < nt) fetch(two, i + 1);
+        work(one, i);
+        if (i + 1 < nt) work(two, i + 1);
+      } else {
+        Codes<D> next;
+        fetch(next, 0);
+        for (int i = 0; i < nt; ++i) {
+          Codes<D> c = next;
+          if (i + 1 < nt) fetch(next, i + 1);
+          work(c, i);
         }
       }
     }
@@ -283,9 +389,10 @@ __global__ void __launch_bounds__(64 * kAttendWaves) k_attend(AttendArgs a) {
       }
     if (g == 0) tops[wave * 16 + r] = m, weights[wave * 16 + r] = l;
     __syncthreads();
+    float *place = whole ? nullptr : a.part + (size_t(blockIdx.x) * 2 + (at_unit == first_unit ? 0 : 1)) * kPlace<D>;
     for (int i = threadIdx.x; i < 16 * (D / 4); i += 64 * kAttendWaves) {
       const int row = i / (D / 4), d = (i - row * (D / 4)) * 4, fl = 16 * rt + row;
-      if (fl >= rows) continue;
+      if (fl >= rows) break;
       float top = tops[row];
 #pragma unroll
       for (int w = 1; w < kAttendWaves; ++w) top = fmaxf(top, tops[w * 16 + row]);
@@ -299,101 +406,106 @@ __global__ void __launch_bounds__(64 * kAttendWaves) k_attend(AttendArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = fmaf(y[e], f, v[e]);
       }
-      const int qr = fl / a.group, h = head * a.group + (fl - qr * a.group);
-      const size_t line = size_t(row0 + qr) * a.q_heads + h;
-      if (a.part) {
-        *reinterpret_cast<f32x4 *>(a.part + (line * a.chunks + blockIdx.x) * D + d) = v;
-        if (d == 0)
-          *reinterpret_cast<float2 *>(a.part + size_t(a.T) * a.q_heads * a.chunks * D + (line * a.chunks + blockIdx.x) * 2) =
-              float2{top, weight};
+      if (whole) {
+        const int qr = fl / a.group, h = head * a.group + (fl - qr * a.group);
+        store4<BF>(a.out, (size_t(s.row0 + qr) * a.q_heads + h) * D + d, v, weight);
       } else {
-        const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
-        const uint32_t two[2] = {
-            BF ? uint32_t(f32_to_bf16(v[0] * inv)) | uint32_t(f32_to_bf16(v[1] * inv)) << 16
-               : __builtin_bit_cast(uint32_t, h2_t{_Float16(v[0] * inv), _Float16(v[1] * inv)}),
-            BF ? uint32_t(f32_to_bf16(v[2] * inv)) | uint32_t(f32_to_bf16(v[3] * inv)) << 16
-               : __builtin_bit_cast(uint32_t, h2_t{_Float16(v[2] * inv), _Float16(v[3] * inv)})};
-        *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + line * D + d) = u32x2{two[0], two[1]};
+        *reinterpret_cast<f32x4 *>(place + row * D + d) = v;
+        if (d == 0) *reinterpret_cast<float2 *>(place + 16 * D + 2 * row) = float2{top, weight};
       }
     }
     __syncthreads();
+    at_unit += units;
   }
 }
 
-// One workgroup a query row and head: its sequence's chunks, the same ones as k_attend wrote, joined in order
+// One workgroup a query row and head: where more than one workgroup of k_attend had its item, their places joined in order
 template <int D, bool BF>
-__global__ void __launch_bounds__(256) k_attend_join(AttendArgs a) {
-  constexpr int LANES = D / 4, GROUPS = 256 / LANES;  // threads over the channels, and over the chunks
-  __shared__ float sums[GROUPS][D];
-  __shared__ float weights[GROUPS];
-  const int line = blockIdx.x, row = line / a.q_heads;
+__global__ void __launch_bounds__(512) k_attend_join(AttendArgs a) {
+  constexpr int LANES = D / 4, PARTS = 512 / LANES;  // threads over the channels, and over the places
+  __shared__ float sums[PARTS][D];
+  __shared__ float weights[PARTS];
+  const int row = blockIdx.x / a.q_heads, qh = blockIdx.x - row * a.q_heads, head = qh / a.group;
   const int b = a.cu ? last_at(a.cu, a.B, row, [](int c, int) { return (long long)c; }) : row;
-  int row0 = 0, n = 0;
-  if (b >= 0) seq_rows(a.cu, b, a.T, &row0, &n);
-  const int r = row - row0;
-  // the chunks that k_attend worked: those below the end of the row's tile of 16
-  int chunks = 0;
-  if (r < n) {
-    const int flat = r * a.group + (line - row * a.q_heads) % a.group;
-    const int last = min((flat | 15), n * a.group - 1) / a.group;
-    chunks = min(a.chunks, max(0, (a.lens[b] - n + last + 1 + a.chunk - 1) / a.chunk));
-  }
-  const float2 *ml = reinterpret_cast<const float2 *>(a.part + size_t(a.T) * a.q_heads * a.chunks * D) + size_t(line) * a.chunks;
+  if (b < 0 || b >= a.B) return;
+  const Share s = share_of(a, b);
+  if (row >= s.row0 + s.n) return;
+  const int flat = (row - s.row0) * a.group + (qh - head * a.group), rt = flat >> 4;
+  const long long line = line_length(a), from = begin_of(a, b) + (long long)(rt * a.heads + head) * s.units, to = from + s.units;
+  // the workgroups that have its first and its last unit
+  const int w0 = int(((from + 1) * a.groups - 1) / line), w1 = int((to * a.groups - 1) / line);
+  if (w0 == w1) return;
+  const int skip = line * w0 / a.groups < from ? 1 : 0;  // it was not the first thing that workgroup w0 did
+  auto place = [&](int w) { return a.part + (size_t(w) * 2 + (w == w0 ? skip : 0)) * kPlace<D>; };
+  const int in = flat & 15;
   float top = -INFINITY;
-  for (int i = threadIdx.x & 63; i < chunks; i += 64) top = fmaxf(top, ml[i].x);
+  for (int w = w0 + (threadIdx.x & 63); w <= w1; w += 64) top = fmaxf(top, place(w)[16 * D + 2 * in]);
   top = wave_max(top);
-  const int grp = threadIdx.x / LANES, d = (threadIdx.x - grp * LANES) * 4;
+  const int part = threadIdx.x / LANES, d = (threadIdx.x - part * LANES) * 4;
   f32x4 v = {};
   float weight = 0.0f;
-  for (int i = grp; i < chunks; i += GROUPS) {
-    const float2 c = ml[i];
-    if (c.y == 0.0f) continue;  // the row sees nothing of it (the largest weight seen is 2^15; one that is NaN goes on)
-    const float f = c.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(c.x - top);
-    const f32x4 y = *reinterpret_cast<const f32x4 *>(a.part + (size_t(line) * a.chunks + i) * D + d);
+#pragma unroll 4
+  for (int w = w0 + part; w <= w1; w += PARTS) {
+    const float2 c = *reinterpret_cast<const float2 *>(place(w) + 16 * D + 2 * in);
+    const f32x4 y = *reinterpret_cast<const f32x4 *>(place(w) + in * D + d);
+    // a place that the row sees nothing of weighs 0 (what is seen weighs 2^kLift at most, 2^(kLift - kLag) at least; NaN goes on)
+    const float f = c.y == 0.0f ? 0.0f : c.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(c.x - top);
     weight = fmaf(c.y, f, weight);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = fmaf(y[e], f, v[e]);
   }
-  *reinterpret_cast<f32x4 *>(&sums[grp][d]) = v;
-  if (d == 0) weights[grp] = weight;
+  *reinterpret_cast<f32x4 *>(&sums[part][d]) = v;
+  if (d == 0) weights[part] = weight;
   __syncthreads();
   if (threadIdx.x >= LANES) return;
 #pragma unroll
-  for (int j = 1; j < GROUPS; ++j) {
-    const f32x4 y = *reinterpret_cast<const f32x4 *>(&sums[j][d]);
+  for (int j = 1; j < PARTS; ++j) {
     weight += weights[j];
-    v += y;
+    v += *reinterpret_cast<const f32x4 *>(&sums[j][d]);
   }
-  const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
-  uint16_t *out = static_cast<uint16_t *>(a.out) + size_t(line) * D + d;
-  u32x2 w;
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-    w[j] = BF ? uint32_t(f32_to_bf16(v[2 * j] * inv)) | uint32_t(f32_to_bf16(v[2 * j + 1] * inv)) << 16
-              : __builtin_bit_cast(uint32_t, h2_t{_Float16(v[2 * j] * inv), _Float16(v[2 * j + 1] * inv)});
-  *reinterpret_cast<u32x2 *>(out) = w;
+  store4<BF>(a.out, size_t(blockIdx.x) * D + d, v, weight);
 }
 
-// The tokens a chunk: the longest that gives 1,024 workgroups (four a CU), within 128 (a tile for each wavefront) and 2,048
-static int attend_chunk(int B, int heads, int row_tiles, int longest) {
-  int chunk = 2048;
-  while (chunk > 128 && (long long)B * heads * row_tiles * ((longest + chunk - 1) / chunk) < 1024) chunk >>= 1;
-  return chunk;
+// Sequences of up to 512 tokens (four tiles a wavefront) are one unit each: joining would cost what splitting gains
+constexpr int kShort = 512;
+
+struct AttendPlan {
+  int groups;    // workgroups
+  bool split;    // items of more than one unit
+  size_t bytes;  // workspace
+};
+
+// The workgroups that the GPU holds at once, but no more than there can be units of work
+template <int D>
+static int attend_resident() {
+  static const int n = [] {
+    int dev = 0, cus = 0, per = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+        hipOccupancyMaxActiveBlocksPerMultiprocessor(&per, k_attend<D, true>, 64 * kAttendWaves,
+                                                     size_t(kAttendWaves) * 16 * (D + 2) * sizeof(float)) != hipSuccess)
+      return 512;
+    return cus * (per > 0 ? per : 1);
+  }();
+  return n;
 }
 
-static int attend_plan(const char *fn, int T, int q_heads, int heads, int D, int B, int most_rows, int longest, int *row_tiles,
-                       int *chunk, int *chunks) {
+static int attend_plan(const char *fn, int T, int q_heads, int heads, int D, int B, int most_rows, int longest, AttendPlan *plan) {
   LMOE_REQUIRE(D == 64 || D == 128 || D == 256, LMOE_ESHAPE, "%s: heads of %d channels (64, 128 and 256 are served)", fn, D);
   LMOE_REQUIRE(heads > 0 && q_heads > 0 && q_heads % heads == 0, LMOE_ESHAPE, "%s: %d query heads over %d key heads", fn, q_heads,
                heads);
-  LMOE_REQUIRE(T >= 0 && B >= 0 && B <= 65535 && most_rows > 0 && longest > 0, LMOE_ESHAPE,
-               "%s: %d rows, %d sequences (65535 at most) of %d rows and %d tokens", fn, T, B, most_rows, longest);
+  LMOE_REQUIRE(T >= 0 && B >= 0 && most_rows > 0 && longest > 0, LMOE_ESHAPE, "%s: %d rows, %d sequences of %d rows and %d tokens",
+               fn, T, B, most_rows, longest);
   const long long flat = (long long)(most_rows < T ? most_rows : (T > 0 ? T : 1)) * (q_heads / heads);
-  const long long tiles = (flat + 15) / 16, room = 65535 / heads;
-  LMOE_REQUIRE(room > 0, LMOE_ESHAPE, "%s: %d key heads", fn, heads);
-  *row_tiles = int(tiles < room ? tiles : room);
-  *chunk = attend_chunk(B, heads, *row_tiles, longest);
-  *chunks = (longest + *chunk - 1) / *chunk;
+  const long long items = (flat + 15) / 16 * heads * (B > 0 ? B : 1);
+  plan->split = longest > kShort;
+  long long n = items;
+  if (plan->split) {
+    const long long units = items * ((longest + kUnit - 1) / kUnit);
+    n = D == 64 ? attend_resident<64>() : D == 128 ? attend_resident<128>() : attend_resident<256>();
+    n = n < units ? n : units;
+  }
+  plan->groups = int(n < (1 << 20) ? n : (1 << 20));  // (a workgroup takes several items where there are more)
+  plan->bytes = plan->split ? size_t(plan->groups) * 2 * 16 * (D + 2) * sizeof(float) : 0;
   return 0;
 }
 
@@ -402,10 +514,8 @@ static int attend_plan(const char *fn, int T, int q_heads, int heads, int D, int
 using namespace lmoe;
 
 extern "C" size_t lmoe_kv_attend_workspace_bytes(int T, int q_heads, int heads, int D, int B, int most_rows, int longest) {
-  int row_tiles, chunk, chunks;
-  if (attend_plan("lmoe_kv_attend_workspace_bytes", T, q_heads, heads, D, B, most_rows, longest, &row_tiles, &chunk, &chunks))
-    return 0;
-  return chunks > 1 ? size_t(T) * q_heads * chunks * (D + 2) * sizeof(float) : 0;
+  AttendPlan plan;
+  return attend_plan("lmoe_kv_attend_workspace_bytes", T, q_heads, heads, D, B, most_rows, longest, &plan) ? 0 : plan.bytes;
 }
 
 extern "C" int lmoe_kv_attend(const void *q, int dtype, long long q_row, long long q_head, int T, int q_heads, int heads, int D,
@@ -415,32 +525,33 @@ extern "C" int lmoe_kv_attend(const void *q, int dtype, long long q_row, long lo
                               void *stream) {
   const char *fn = "lmoe_kv_attend";
   LMOE_REQUIRE(dtype == LMOE_F16 || dtype == LMOE_BF16, LMOE_EINVAL, "%s: dtype %d (float16 and bfloat16 are served)", fn, dtype);
-  int row_tiles, chunk, chunks;
-  if (const int rc = attend_plan(fn, T, q_heads, heads, D, B, most_rows, longest, &row_tiles, &chunk, &chunks)) return rc;
+  AttendPlan plan;
+  if (const int rc = attend_plan(fn, T, q_heads, heads, D, B, most_rows, longest, &plan)) return rc;
   LMOE_REQUIRE(page == 32 || page == 64 || page == 128, LMOE_ESHAPE, "%s: pages of %d tokens (32, 64 and 128 are served)", fn,
                page);
-  LMOE_REQUIRE(pages > 0 && width > 0, LMOE_ESHAPE, "%s: %d pages, a table of %d", fn, pages, width);
+  const int page_shift = page == 32 ? 5 : page == 64 ? 6 : 7;
+  LMOE_REQUIRE(pages > 0 && width > 0 && width <= (1 << 30) >> page_shift, LMOE_ESHAPE, "%s: %d pages, a table of %d", fn, pages,
+               width);
   if (T == 0) return 0;
   LMOE_REQUIRE(B > 0 && (cu || T == B), LMOE_ESHAPE, "%s: %d rows of %d sequences need their offsets", fn, T, B);
   LMOE_REQUIRE(scale > 0.0f && scale < INFINITY, LMOE_EINVAL, "%s: scale %g", fn, double(scale));
   LMOE_REQUIRE(q && lens && table && k_codes && k_scale && v_codes && v_scale && out, LMOE_EINVAL, "%s: null pointer", fn);
   LMOE_REQUIRE(aligned16(q) && q_row % 8 == 0 && q_head % 8 == 0 && aligned16(k_codes) && aligned16(v_codes) && aligned16(out),
                LMOE_EALIGN, "%s: rows and codes must be 16-byte aligned", fn);
-  const size_t need = chunks > 1 ? size_t(T) * q_heads * chunks * (D + 2) * sizeof(float) : 0;
-  LMOE_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need), LMOE_EWORKSPACE,
-               "%s: a 16-byte aligned workspace of %zu bytes is needed", fn, need);
-  LMOE_REQUIRE((long long)T * q_heads < (1ll << 31), LMOE_ESHAPE, "%s: %d rows of %d heads", fn, T, q_heads);
+  LMOE_REQUIRE(!plan.split || (workspace && aligned16(workspace) && workspace_bytes >= plan.bytes), LMOE_EWORKSPACE,
+               "%s: a 16-byte aligned workspace of %zu bytes is needed", fn, plan.bytes);
+  LMOE_REQUIRE((long long)T * q_heads < (1ll << 27), LMOE_ESHAPE, "%s: %d rows of %d heads", fn, T, q_heads);
   AttendArgs a = {q, q_row, q_head, k_codes, v_codes, k_scale, v_scale, table, lens, cu, out,
-                  need ? static_cast<float *>(workspace) : nullptr, scale * kLog2e, T, B, q_heads, heads,
-                  page == 32 ? 5 : page == 64 ? 6 : 7, pages, width, q_heads / heads, row_tiles, chunk, chunks};
+                  plan.split ? static_cast<float *>(workspace) : nullptr, scale * kLog2e, T, B, q_heads, heads, page_shift, pages,
+                  width, q_heads / heads, plan.groups};
   hipStream_t st = (hipStream_t)stream;
   auto go = [&](auto kernel, auto join) -> int {
     const size_t lds = size_t(kAttendWaves) * 16 * (D + 2) * sizeof(float);
     if (const int rc = allow_lds(kernel, lds, fn)) return rc;
-    launch(kernel, dim3(unsigned(chunks), unsigned(heads * row_tiles), unsigned(B)), dim3(64 * kAttendWaves), lds, st, a);
+    launch(kernel, dim3(unsigned(plan.groups)), dim3(64 * kAttendWaves), lds, st, a);
     LMOE_LAUNCHED(fn);
-    if (need) {
-      launch(join, dim3(unsigned(T) * unsigned(q_heads)), dim3(256), 0, st, a);
+    if (plan.split) {
+      launch(join, dim3(unsigned(T) * unsigned(q_heads)), dim3(512), 0, st, a);
       LMOE_LAUNCHED(fn);
     }
     return 0;
