@@ -17,8 +17,8 @@
 // multiply float32 sums.
 //
 // All of a call's work lies on one line of units of 128 tokens (one 32-token tile for each of a workgroup's four wavefronts):
-// sequence by sequence, in it each tile of 16 rows and key head, in that the sequence's units in order. As many workgroups as
-// the GPU holds at once take equal stretches of the line, whatever the sequences' lengths. A workgroup finishes the items
+// sequence by sequence, in it each tile of 16 rows and key head, in that the sequence's units in order. Two workgroups a CU
+// take equal stretches of the line, whatever the sequences' lengths. A workgroup finishes the items
 // that lie in its stretch whole; the two that may reach over its ends go to its two places in the workspace, and a second
 // kernel joins those. Where sequences are short, each is one unit and there is nothing to join.
 #include "rows.h"
@@ -28,7 +28,6 @@ namespace lmoe {
 constexpr int kAttendWaves = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
-constexpr int kUnit = 32 * kAttendWaves;  // tokens
 // A weight is 2^(score - maximum in use + kLift), the maximum lagging at most kLag behind
 constexpr float kLift = 11.0f, kLag = 4.0f;
 
@@ -40,71 +39,57 @@ struct AttendArgs {
   const int *table, *lens, *cu;
   void *out;    // [T][q_heads][D]
   float *part;  // [workgroups][2] of [16 rows][D] sums and [16 rows] of {maximum, weight}; null: an item is one unit
+  int2 *joins;  // [T][q_heads]: the first place of a row's item (-1: one workgroup had it all), 16 times its last workgroup
+                // and the row of the tile
   float scale;  // times log2 e
-  int T, B, q_heads, heads, page_shift, pages, width, group, groups;  // groups: workgroups of k_attend
+  int T, B, q_heads, heads, page_shift, unit_shift, pages, width, group, groups;  // groups: workgroups of k_attend
 };
 
 // A sequence's share of the line
 struct Share {
   int row0, n, len, tiles, units;  // rows, tokens, tiles of 16 (row, query head of the group) pairs, units an item
-  __device__ __forceinline__ long long total(int heads) const { return (long long)tiles * heads * units; }
+  __device__ __forceinline__ int total(int heads) const { return tiles * heads * units; }
 };
-__device__ __forceinline__ Share share_of(const AttendArgs &a, int b) {
-  Share s;
-  seq_rows(a.cu, b, a.T, &s.row0, &s.n);
-  s.len = a.lens[b];
-  s.tiles = (s.n * a.group + 15) >> 4;
-  s.units = a.part ? (min(max(s.len, 1), a.width << a.page_shift) + kUnit - 1) / kUnit : 1;
-  return s;
+__device__ __forceinline__ Share share(const AttendArgs &a, int row0, int n, int len) {
+  return {row0, n, len, (n * a.group + 15) >> 4,
+          a.part ? ((min(max(len, 1), a.width << a.page_shift) - 1) >> a.unit_shift) + 1 : 1};
 }
 
-// The line's length and, by one wavefront, where sequence `until` (or that of unit `unit`) begins on it
-__device__ __forceinline__ long long wave_scan(long long v) {
+// Inclusive sums over a wavefront's lanes
+__device__ __forceinline__ int wave_scan(int v) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const long long u = __shfl_up(v, d);
-    if ((threadIdx.x & 63) >= d) v += u;
+    const int u = __shfl_up(v, d);
+    if (int(threadIdx.x & 63) >= d) v += u;
   }
   return v;
 }
-__device__ __forceinline__ long long lane_i64(long long v, int l) {
-  const uint32_t lo = __builtin_amdgcn_readlane(uint32_t(v), l), hi = __builtin_amdgcn_readlane(uint32_t(v >> 32), l);
-  return (long long)(uint64_t(hi) << 32 | lo);
-}
-__device__ __forceinline__ long long line_length(const AttendArgs &a) {
-  long long sum = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int b = b0 + (threadIdx.x & 63);
-    sum += lane_i64(wave_scan(b < a.B ? share_of(a, b).total(a.heads) : 0), 63);
-  }
-  return sum;
-}
-// the sequence that has unit `unit` (of a line longer than that), and where it begins
-__device__ __forceinline__ int sequence_of(const AttendArgs &a, long long unit, long long *begins) {
-  long long base = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int b = b0 + (threadIdx.x & 63);
-    const long long own = b < a.B ? share_of(a, b).total(a.heads) : 0, sum = wave_scan(own);
-    const unsigned long long past = __ballot(base + sum > unit);
-    if (past) {
-      const int l = __ffsll(past) - 1;
-      *begins = base + lane_i64(sum - own, l);
-      return __builtin_amdgcn_readfirstlane(b0 + l);
+
+// Workgroup w of n has the units [stretch(w), stretch(w + 1)) of a line
+__device__ __forceinline__ int stretch(int line, int w, int n) { return int((long long)line * w / n); }
+
+// 64 sequences of the line, in LDS for each wavefront (in registers they would be there through the whole loop)
+struct Seqs {
+  int3 *seq;  // [64] first row, rows, tokens
+  int *ends;  // [64] where a sequence ends on the line
+  int b0;     // the first of them
+  int base;   // where that begins
+
+  __device__ __forceinline__ void load(const AttendArgs &a, int from, int begins) {
+    const int lane = threadIdx.x & 63, b = from + lane;
+    int3 s = {0, 0, 0};
+    if (b < a.B) {
+      seq_rows(a.cu, b, a.T, &s.x, &s.y);
+      s.z = a.lens[b];
     }
-    base += lane_i64(sum, 63);
+    seq[lane] = s;
+    ends[lane] = begins + wave_scan(share(a, s.x, s.y, s.z).total(a.heads));
+    b0 = from;
+    base = begins;
   }
-  *begins = base;
-  return a.B;
-}
-// where sequence `which` begins
-__device__ __forceinline__ long long begin_of(const AttendArgs &a, int which) {
-  long long base = 0;
-  for (int b0 = 0; b0 < which; b0 += 64) {
-    const int b = b0 + (threadIdx.x & 63);
-    base += lane_i64(wave_scan(b < which ? share_of(a, b).total(a.heads) : 0), 63);
-  }
-  return base;
-}
+  __device__ __forceinline__ int end() const { return __builtin_amdgcn_readfirstlane(ends[63]); }
+};
+constexpr size_t kSeqsLds = kAttendWaves * 64 * (sizeof(int3) + sizeof(int));
 
 template <bool BF>
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
@@ -175,6 +160,9 @@ __device__ __forceinline__ void zero_rows(const AttendArgs &a, int from, int to)
   const long long per = (long long)a.q_heads * D / 8;
   u32x4 *out = reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(a.out) + size_t(from) * a.q_heads * D);
   for (long long i = threadIdx.x; i < (to - from) * per; i += 64 * kAttendWaves) out[i] = u32x4{};
+  if (a.part)
+    for (long long i = threadIdx.x; i < (long long)(to - from) * a.q_heads; i += 64 * kAttendWaves)
+      a.joins[(long long)from * a.q_heads + i] = int2{-1, 0};
 }
 
 template <bool BF>
@@ -190,41 +178,55 @@ __device__ __forceinline__ void store4(void *out, size_t at, f32x4 v, float weig
 
 template <int D>
 constexpr int kPlace = 16 * (D + 2);  // floats of a place in the workspace
+template <int D>
+constexpr int kRow = D + 4;  // floats of a row of sums in LDS: 16 rows' same channels lie in different banks
+template <int D>
+constexpr size_t kSumsLds = size_t(kAttendWaves) * 16 * (kRow<D> + 2) * sizeof(float);
+template <int D>
+constexpr size_t kAttendLds = kSumsLds<D> + kSeqsLds;
 
 template <int D, bool BF>
 __global__ void __launch_bounds__(64 * kAttendWaves, D == 256 ? 2 : 3) k_attend(AttendArgs a) {
   constexpr int NC = D / 64, NT = D / 16;  // 64-channel groups, 16-channel tiles
-  extern __shared__ float lds[];           // [wave][16 rows][D] sums, then [wave][16] maxima, [wave][16] weights
+  extern __shared__ float lds[];           // [wave][16 rows][kRow] sums, then [wave][16] maxima, [wave][16] weights; then Seqs
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   if (blockIdx.x == 0 && a.cu) {  // rows before the first sequence or behind the last one come back zero
     zero_rows<D>(a, 0, min(max(a.cu[0], 0), a.T));
     zero_rows<D>(a, min(max(a.cu[a.B], 0), a.T), a.T);
   }
-  const long long line = line_length(a);
-  long long at_unit = line * blockIdx.x / a.groups;
-  const long long stop_unit = line * (blockIdx.x + 1) / a.groups;
+  char *seqs_at = reinterpret_cast<char *>(lds) + kSumsLds<D>;
+  Seqs seqs = {reinterpret_cast<int3 *>(seqs_at + kAttendWaves * 64 * sizeof(int)) + wave * 64,
+               reinterpret_cast<int *>(seqs_at) + wave * 64, 0, 0};
+  int line = 0;
+  for (int b0 = (a.B - 1) & ~63; b0 > 0; b0 -= 64) {  // the first ones last: they stay
+    seqs.load(a, b0, 0);
+    line += seqs.end();
+  }
+  seqs.load(a, 0, 0);
+  line += seqs.end();
+  int at_unit = stretch(line, blockIdx.x, a.groups);
+  const int stop_unit = stretch(line, blockIdx.x + 1, a.groups);
   if (at_unit >= stop_unit) return;
-  const long long first_unit = at_unit;
-  long long base;
-  int b = sequence_of(a, at_unit, &base);
-  Share s = share_of(a, b);
+  const int first_unit = at_unit;
   const int page_tokens = 1 << a.page_shift;
   const size_t head_bytes = size_t(page_tokens) * D, page_bytes = head_bytes * a.heads;
 
   while (at_unit < stop_unit) {
-    while (at_unit >= base + s.total(a.heads)) {  // on to the next sequence that has rows
-      base += s.total(a.heads);
-      s = share_of(a, ++b);
-    }
-    const int item = int((at_unit - base) / s.units), unit0 = int((at_unit - base) - (long long)item * s.units);
-    const int units = int(min((long long)(s.units - unit0), stop_unit - at_unit));
+    while (at_unit >= seqs.end()) seqs.load(a, seqs.b0 + 64, seqs.end());
+    const int in64 = __ffsll(__ballot(seqs.ends[opaque(lane)] > at_unit)) - 1, b = seqs.b0 + in64;
+    const int3 found = seqs.seq[in64];
+    const Share s = share(a, __builtin_amdgcn_readfirstlane(found.x), __builtin_amdgcn_readfirstlane(found.y),
+                          __builtin_amdgcn_readfirstlane(found.z));
+    const int base = in64 ? __builtin_amdgcn_readfirstlane(seqs.ends[in64 - 1]) : seqs.base;
+    const int item = (at_unit - base) / s.units, unit0 = (at_unit - base) - item * s.units;
+    const int units = min(s.units - unit0, stop_unit - at_unit);
     const int rt = item / a.heads, head = item - rt * a.heads, rows = s.n * a.group;
     const bool whole = units == s.units;
     const int last = min(16 * rt + 15, rows - 1) / a.group;
     // this stretch's tokens [begin, end): an item's last unit ends with what its last row sees
-    const int begin = unit0 * kUnit;
+    const int begin = unit0 << a.unit_shift;
     int end = s.len - s.n + last + 1;
-    if (unit0 + units < s.units) end = min(end, begin + units * kUnit);
+    if (unit0 + units < s.units) end = min(end, begin + (units << a.unit_shift));
     // the lane's row: query row `mine` of the sequence, seeing the first `sees` places; every row sees those below `all`
     const int flat = min(16 * rt + r, rows - 1), mine = flat / a.group, sub = flat - mine * a.group;
     const int sees = s.len - s.n + mine + 1, all = s.len - s.n + (16 * rt) / a.group + 1;
@@ -241,7 +243,7 @@ __global__ void __launch_bounds__(64 * kAttendWaves, D == 256 ? 2 : 3) k_attend(
     }
     f32x4 o[NT] = {};
     float m = -INFINITY, l = 0.0f;
-    uint8_t *marks = reinterpret_cast<uint8_t *>(lds + wave * 16 * D);
+    uint8_t *marks = reinterpret_cast<uint8_t *>(lds + wave * 16 * kRow<D>);
     const int first = begin / 32 + wave, tiles = max(0, ((max(end, begin) + 31) / 32 - first + 3) / 4);
 
     for (int t0 = 0; t0 < tiles; t0 += 64) {
@@ -379,18 +381,25 @@ __global__ void __launch_bounds__(64 * kAttendWaves, D == 256 ? 2 : 3) k_attend(
     // the four wavefronts' sums: a lane's o[4 w + j][e] is channel (4 g + e) D / 16 + 4 w + j of row r
     l += lane_xor16(l);
     l += lane_xor32(l);
-    float *sums = lds, *tops = lds + kAttendWaves * 16 * D, *weights = tops + kAttendWaves * 16;
+    const int tid = opaque(int(threadIdx.x)), er = tid & 15, eg = tid >> 4 & 3;  // opaque: no address of this lives through the loop
+    float *sums = lds, *tops = lds + kAttendWaves * 16 * kRow<D>, *weights = tops + kAttendWaves * 16;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
       for (int w = 0; w < NC; ++w) {
         const f32x4 v = {o[4 * w][e], o[4 * w + 1][e], o[4 * w + 2][e], o[4 * w + 3][e]};
-        *reinterpret_cast<f32x4 *>(sums + (wave * 16 + r) * D + (4 * g + e) * NT + 4 * w) = v;
+        *reinterpret_cast<f32x4 *>(sums + (wave * 16 + er) * kRow<D> + (4 * eg + e) * NT + 4 * w) = v;
       }
-    if (g == 0) tops[wave * 16 + r] = m, weights[wave * 16 + r] = l;
+    if (eg == 0) tops[wave * 16 + er] = m, weights[wave * 16 + er] = l;
     __syncthreads();
+    if (a.part && unit0 == 0) {  // what the joining kernel has to do for the item's rows
+      const int2 join = {whole ? -1 : int(blockIdx.x) * 2 + (at_unit == first_unit ? 0 : 1),
+                         int(((long long)(at_unit + s.units) * a.groups - 1) / line) * 16 + tid};
+      const int fl = 16 * rt + tid, qr = fl / a.group;
+      if (tid < 16 && fl < rows) a.joins[size_t(s.row0 + qr) * a.q_heads + head * a.group + (fl - qr * a.group)] = join;
+    }
     float *place = whole ? nullptr : a.part + (size_t(blockIdx.x) * 2 + (at_unit == first_unit ? 0 : 1)) * kPlace<D>;
-    for (int i = threadIdx.x; i < 16 * (D / 4); i += 64 * kAttendWaves) {
+    for (int i = tid; i < 16 * (D / 4); i += 64 * kAttendWaves) {
       const int row = i / (D / 4), d = (i - row * (D / 4)) * 4, fl = 16 * rt + row;
       if (fl >= rows) break;
       float top = tops[row];
@@ -401,7 +410,7 @@ __global__ void __launch_bounds__(64 * kAttendWaves, D == 256 ? 2 : 3) k_attend(
 #pragma unroll
       for (int w = 0; w < kAttendWaves; ++w) {
         const float mw = tops[w * 16 + row], f = mw == -INFINITY && top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - top);
-        const f32x4 y = *reinterpret_cast<const f32x4 *>(sums + (w * 16 + row) * D + d);
+        const f32x4 y = *reinterpret_cast<const f32x4 *>(sums + (w * 16 + row) * kRow<D> + d);
         weight = fmaf(weights[w * 16 + row], f, weight);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = fmaf(y[e], f, v[e]);
@@ -421,73 +430,62 @@ __global__ void __launch_bounds__(64 * kAttendWaves, D == 256 ? 2 : 3) k_attend(
 
 // One workgroup a query row and head: where more than one workgroup of k_attend had its item, their places joined in order
 template <int D, bool BF>
-__global__ void __launch_bounds__(512) k_attend_join(AttendArgs a) {
-  constexpr int LANES = D / 4, PARTS = 512 / LANES;  // threads over the channels, and over the places
+__global__ void __launch_bounds__(256) k_attend_join(AttendArgs a) {
+  constexpr int LANES = D / 4, PARTS = 256 / LANES;  // threads over the channels, and over the places
   __shared__ float sums[PARTS][D];
-  __shared__ float weights[PARTS];
-  const int row = blockIdx.x / a.q_heads, qh = blockIdx.x - row * a.q_heads, head = qh / a.group;
-  const int b = a.cu ? last_at(a.cu, a.B, row, [](int c, int) { return (long long)c; }) : row;
-  if (b < 0 || b >= a.B) return;
-  const Share s = share_of(a, b);
-  if (row >= s.row0 + s.n) return;
-  const int flat = (row - s.row0) * a.group + (qh - head * a.group), rt = flat >> 4;
-  const long long line = line_length(a), from = begin_of(a, b) + (long long)(rt * a.heads + head) * s.units, to = from + s.units;
-  // the workgroups that have its first and its last unit
-  const int w0 = int(((from + 1) * a.groups - 1) / line), w1 = int((to * a.groups - 1) / line);
-  if (w0 == w1) return;
-  const int skip = line * w0 / a.groups < from ? 1 : 0;  // it was not the first thing that workgroup w0 did
-  auto place = [&](int w) { return a.part + (size_t(w) * 2 + (w == w0 ? skip : 0)) * kPlace<D>; };
-  const int in = flat & 15;
-  float top = -INFINITY;
-  for (int w = w0 + (threadIdx.x & 63); w <= w1; w += 64) top = fmaxf(top, place(w)[16 * D + 2 * in]);
-  top = wave_max(top);
+  __shared__ float tops[PARTS], weights[PARTS];
+  const int2 join = a.joins[blockIdx.x];
+  if (join.x < 0) return;
+  const int in = join.y & 15, w0 = min(join.x >> 1, a.groups - 1), w1 = min(join.y >> 4, a.groups - 1);
   const int part = threadIdx.x / LANES, d = (threadIdx.x - part * LANES) * 4;
   f32x4 v = {};
-  float weight = 0.0f;
-#pragma unroll 4
-  for (int w = w0 + part; w <= w1; w += PARTS) {
-    const float2 c = *reinterpret_cast<const float2 *>(place(w) + 16 * D + 2 * in);
-    const f32x4 y = *reinterpret_cast<const f32x4 *>(place(w) + in * D + d);
-    // a place that the row sees nothing of weighs 0 (what is seen weighs 2^kLift at most, 2^(kLift - kLag) at least; NaN goes on)
-    const float f = c.y == 0.0f ? 0.0f : c.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(c.x - top);
-    weight = fmaf(c.y, f, weight);
+  float top = -INFINITY, weight = 0.0f;
+  // a place that the row sees nothing of weighs 0 (one that it sees weighs 2^(kLift - kLag) at least; NaN goes on)
+  auto add = [&](float m, float l, f32x4 y) {
+    const float to = fmaxf(top, l == 0.0f ? top : m);
+    const float keep = weight == 0.0f ? 0.0f : to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - to);
+    const float f = l == 0.0f ? 0.0f : to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+    top = to;
+    weight = fmaf(l, f, weight * keep);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = fmaf(y[e], f, v[e]);
+    for (int e = 0; e < 4; ++e) v[e] = fmaf(y[e], f, v[e] * keep);
+  };
+  for (int first = w0 + part; first <= w1; first += 4 * PARTS) {  // four places' loads at a time
+    float2 c[4];
+    f32x4 y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int w = min(first + j * PARTS, w1);
+      const float *place = a.part + (size_t(w) * 2 + (w == w0 ? join.x & 1 : 0)) * kPlace<D>;
+      c[j] = *reinterpret_cast<const float2 *>(place + 16 * D + 2 * in);
+      y[j] = *reinterpret_cast<const f32x4 *>(place + in * D + d);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (first + j * PARTS <= w1) add(c[j].x, c[j].y, y[j]);
   }
   *reinterpret_cast<f32x4 *>(&sums[part][d]) = v;
-  if (d == 0) weights[part] = weight;
+  if (d == 0) tops[part] = top, weights[part] = weight;
   __syncthreads();
   if (threadIdx.x >= LANES) return;
-#pragma unroll
-  for (int j = 1; j < PARTS; ++j) {
-    weight += weights[j];
-    v += *reinterpret_cast<const f32x4 *>(&sums[j][d]);
-  }
+#pragma unroll 1
+  for (int j = 1; j < PARTS; ++j) add(tops[j], weights[j], *reinterpret_cast<const f32x4 *>(&sums[j][d]));
   store4<BF>(a.out, size_t(blockIdx.x) * D + d, v, weight);
 }
 
 // Sequences of up to 512 tokens (four tiles a wavefront) are one unit each: joining would cost what splitting gains
 constexpr int kShort = 512;
 
-struct AttendPlan {
-  int groups;    // workgroups
-  bool split;    // items of more than one unit
-  size_t bytes;  // workspace
-};
+// Two workgroups a CU. The GPU holds three (width 128) or four (64), but three gain 1 % on 64 sequences of 16,384 tokens
+// (75.7 -> 74.9 us), and every workgroup more is another place to join (131,072 tokens of one sequence: 7.5 -> 8.8 us)
+constexpr int kAttendGroups = 512;
 
-// The workgroups that the GPU holds at once, but no more than there can be units of work
-template <int D>
-static int attend_resident() {
-  static const int n = [] {
-    int dev = 0, cus = 0, per = 0;
-    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
-        hipOccupancyMaxActiveBlocksPerMultiprocessor(&per, k_attend<D, true>, 64 * kAttendWaves,
-                                                     size_t(kAttendWaves) * 16 * (D + 2) * sizeof(float)) != hipSuccess)
-      return 512;
-    return cus * (per > 0 ? per : 1);
-  }();
-  return n;
-}
+struct AttendPlan {
+  int groups;      // workgroups
+  int unit_shift;  // a unit's tokens
+  bool split;    // items of more than one unit
+  size_t places, bytes;  // the workspace's places, and all of it
+};
 
 static int attend_plan(const char *fn, int T, int q_heads, int heads, int D, int B, int most_rows, int longest, AttendPlan *plan) {
   LMOE_REQUIRE(D == 64 || D == 128 || D == 256, LMOE_ESHAPE, "%s: heads of %d channels (64, 128 and 256 are served)", fn, D);
@@ -498,14 +496,15 @@ static int attend_plan(const char *fn, int T, int q_heads, int heads, int D, int
   const long long flat = (long long)(most_rows < T ? most_rows : (T > 0 ? T : 1)) * (q_heads / heads);
   const long long items = (flat + 15) / 16 * heads * (B > 0 ? B : 1);
   plan->split = longest > kShort;
+  plan->unit_shift = 7;
   long long n = items;
   if (plan->split) {
-    const long long units = items * ((longest + kUnit - 1) / kUnit);
-    n = D == 64 ? attend_resident<64>() : D == 128 ? attend_resident<128>() : attend_resident<256>();
-    n = n < units ? n : units;
+    const long long units = items * ((longest + 127) / 128);
+    n = kAttendGroups < units ? kAttendGroups : units;
   }
   plan->groups = int(n < (1 << 20) ? n : (1 << 20));  // (a workgroup takes several items where there are more)
-  plan->bytes = plan->split ? size_t(plan->groups) * 2 * 16 * (D + 2) * sizeof(float) : 0;
+  plan->places = size_t(plan->groups) * 2 * 16 * (D + 2) * sizeof(float);
+  plan->bytes = plan->split ? plan->places + size_t(T) * q_heads * sizeof(int2) : 0;
   return 0;
 }
 
@@ -541,24 +540,33 @@ extern "C" int lmoe_kv_attend(const void *q, int dtype, long long q_row, long lo
   LMOE_REQUIRE(!plan.split || (workspace && aligned16(workspace) && workspace_bytes >= plan.bytes), LMOE_EWORKSPACE,
                "%s: a 16-byte aligned workspace of %zu bytes is needed", fn, plan.bytes);
   LMOE_REQUIRE((long long)T * q_heads < (1ll << 27), LMOE_ESHAPE, "%s: %d rows of %d heads", fn, T, q_heads);
+  // units are counted in 32 bits: longer ones where a table's room could hold more than that
+  const long long most = ((long long)T * (q_heads / heads) / 16 + B) * heads;
+  while ((most * ((((long long)width << page_shift) >> plan.unit_shift) + 1)) >> 31 && plan.unit_shift < 30) ++plan.unit_shift;
+  LMOE_REQUIRE(most * ((((long long)width << page_shift) >> plan.unit_shift) + 1) < (1ll << 31), LMOE_ESHAPE,
+               "%s: %d rows of %d sequences and %d key heads", fn, T, B, heads);
   AttendArgs a = {q, q_row, q_head, k_codes, v_codes, k_scale, v_scale, table, lens, cu, out,
-                  plan.split ? static_cast<float *>(workspace) : nullptr, scale * kLog2e, T, B, q_heads, heads, page_shift, pages,
+                  plan.split ? static_cast<float *>(workspace) : nullptr,
+                  plan.split ? reinterpret_cast<int2 *>(static_cast<char *>(workspace) + plan.places) : nullptr, scale * kLog2e, T, B, q_heads, heads, page_shift, plan.unit_shift, pages,
                   width, q_heads / heads, plan.groups};
   hipStream_t st = (hipStream_t)stream;
-  auto go = [&](auto kernel, auto join) -> int {
-    const size_t lds = size_t(kAttendWaves) * 16 * (D + 2) * sizeof(float);
+  auto go = [&](auto kernel, auto join, size_t lds) -> int {
     if (const int rc = allow_lds(kernel, lds, fn)) return rc;
     launch(kernel, dim3(unsigned(plan.groups)), dim3(64 * kAttendWaves), lds, st, a);
     LMOE_LAUNCHED(fn);
     if (plan.split) {
-      launch(join, dim3(unsigned(T) * unsigned(q_heads)), dim3(512), 0, st, a);
+      launch(join, dim3(unsigned(T) * unsigned(q_heads)), dim3(256), 0, st, a);
       LMOE_LAUNCHED(fn);
     }
     return 0;
   };
   const bool bf = dtype == LMOE_BF16;
-  if (D == 64) return bf ? go(k_attend<64, true>, k_attend_join<64, true>) : go(k_attend<64, false>, k_attend_join<64, false>);
+  if (D == 64)
+    return bf ? go(k_attend<64, true>, k_attend_join<64, true>, kAttendLds<64>)
+              : go(k_attend<64, false>, k_attend_join<64, false>, kAttendLds<64>);
   if (D == 128)
-    return bf ? go(k_attend<128, true>, k_attend_join<128, true>) : go(k_attend<128, false>, k_attend_join<128, false>);
-  return bf ? go(k_attend<256, true>, k_attend_join<256, true>) : go(k_attend<256, false>, k_attend_join<256, false>);
+    return bf ? go(k_attend<128, true>, k_attend_join<128, true>, kAttendLds<128>)
+              : go(k_attend<128, false>, k_attend_join<128, false>, kAttendLds<128>);
+  return bf ? go(k_attend<256, true>, k_attend_join<256, true>, kAttendLds<256>)
+            : go(k_attend<256, false>, k_attend_join<256, false>, kAttendLds<256>);
 }
