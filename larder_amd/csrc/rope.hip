@@ -81,30 +81,43 @@ struct RopeArgs {
   const double *freq;
   const int *cu, *lens;
   float gain;
-  int pos64, T, B, heads, k_heads, D, F, inter, dt, tokens;
+  int pos64, T, B, heads, k_heads, D, F, inter, dt, tokens, turn_shift, copy_shift;
 };
 
-// One workgroup, `tokens` rows: their cos / sin into LDS, then every head of them. A thread takes both sides of its pairs, so
-// xo may be x. W 8: eight channels a load (interleaved: four pairs; else one load of either side); W 1: any widths, strides
-// and alignments.
-template <int W>
-__global__ void __launch_bounds__(kRopeThreads) k_rope(RopeArgs a) {
-  extern __shared__ float2 cs[];
-  const int t0 = blockIdx.x * a.tokens, nt = min(a.tokens, a.T - t0);
-  __shared__ int place[64];  // a row's position; a row of no sequence: kNoRow
-  constexpr int kNoRow = -0x7fffffff - 1;
-  if (!a.positions) {
-    for (int i = threadIdx.x >> 6; i < nt; i += kRopeThreads / 64) {
-      const int row = t0 + i;
-      const int b = a.cu ? last_at(a.cu, a.B, row, [](int c, int) { return (long long)c; }) : row;
-      int pos = kNoRow;
-      if (b >= 0 && b < a.B) {
-        int r0, n;
-        seq_rows(a.cu, b, a.T, &r0, &n);
-        if (row < r0 + n) pos = a.lens[b] - n + (row - r0);
-      }
-      if ((threadIdx.x & 63) == 0) place[i] = pos;
+constexpr int kNoRow = -0x7fffffff - 1;  // the position of a row of no sequence
+
+// The positions of rows t0 .. t0 + nt - 1 (nt <= 8) from their sequences, by one wavefront, into place: the first row's
+// sequence, then the 64 that follow it in one load
+__device__ __forceinline__ void places_of(const RopeArgs &a, int t0, int nt, int *place) {
+  const int lane = threadIdx.x & 63;
+  if (!a.cu) {
+    if (lane < nt) place[lane] = t0 + lane < a.B ? a.lens[t0 + lane] - 1 : kNoRow;
+    return;
+  }
+  auto begins = [](int c, int) { return (long long)c; };
+  const int b0 = last_at(a.cu, a.B, t0, begins);
+  const int c = a.cu[min(b0 + 1 + lane, a.B)];
+  for (int i = 0; i < nt; ++i) {
+    const int row = t0 + i, past = __popcll(__ballot(b0 + 1 + lane <= a.B && c <= row));
+    const int b = past < 64 ? b0 + past : last_at(a.cu, a.B, row, begins);
+    int pos = kNoRow;
+    if (b >= 0 && b < a.B) {
+      int r0, n;
+      seq_rows(a.cu, b, a.T, &r0, &n);
+      if (row < r0 + n) pos = a.lens[b] - n + (row - r0);
     }
+    if (lane == 0) place[i] = pos;
+  }
+}
+
+// One workgroup, `tokens` rows from t0 on: their cos / sin into LDS, then every head of them. A thread takes both sides of its
+// pairs, so xo may be x. W 8: eight channels a load; W 1: any widths, strides and alignments.
+template <int W>
+__device__ __forceinline__ void rope_block(const RopeArgs &a, int t0, float2 *cs) {
+  __shared__ int place[8];
+  const int nt = min(a.tokens, a.T - t0);
+  if (!a.positions) {
+    if (threadIdx.x < 64) places_of(a, t0, nt, place);
     __syncthreads();
   }
   for (int i = threadIdx.x; i < nt * a.F; i += kRopeThreads) {
@@ -117,62 +130,109 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope(RopeArgs a) {
     cs[i] = v;
   }
   __syncthreads();
-  const bool quads = W == 8 && a.inter;  // pairs inside a load
-  const int sides = quads ? 0 : a.F / W;  // units that take a load of either side
-  const int per = quads ? a.D / W : sides + (a.D - 2 * a.F) / W, per_t = per * (a.heads + a.k_heads);
-  for (int i = threadIdx.x; i < nt * per_t; i += kRopeThreads) {
-    const int t = i / per_t, j = i - t * per_t, h = j / per, u = j - h * per;
-    const bool key = h >= a.heads, none = !a.positions && place[t] == kNoRow;
-    const void *x = key ? a.k.p : a.x.p;
-    void *y = key ? a.ko : a.xo;
-    const int hk = key ? h - a.heads : h;
-    const size_t at = size_t(t0 + t) * (key ? a.k.st : a.x.st) + size_t(hk) * (key ? a.k.sh : a.x.sh);
-    const size_t to = key ? (size_t(t0 + t) * a.k_heads + hk) * a.D : size_t(t0 + t) * a.xo_st + size_t(hk) * a.xo_sh;
-    const float2 *c = cs + t * a.F;
-    if constexpr (W == 8) {
-      if (u < sides) {
-        float v[8], w[8], p[8], q[8];
-        load8(x, at + u * 8, a.dt, v);
-        load8(x, at + u * 8 + a.F, a.dt, w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float2 r = c[u * 8 + e];
-          p[e] = none ? 0.0f : v[e] * r.x - w[e] * r.y;
-          q[e] = none ? 0.0f : w[e] * r.x + v[e] * r.y;
-        }
-        store8(y, to + u * 8, a.dt, p);
-        store8(y, to + u * 8 + a.F, a.dt, q);
-      } else {
-        const int d = quads ? u * 8 : 2 * a.F + (u - sides) * 8;
-        float v[8], o[8];
-        load8(x, at + d, a.dt, v);
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const float2 r = d + e < 2 * a.F ? c[(d + e) >> 1] : float2{1.0f, 0.0f};
-          const bool turns = d + e < 2 * a.F;
-          o[e] = none ? 0.0f : turns ? v[e] * r.x - v[e + 1] * r.y : v[e];
-          o[e + 1] = none ? 0.0f : turns ? v[e + 1] * r.x + v[e] * r.y : v[e + 1];
-        }
-        store8(y, to + d, a.dt, o);
-      }
-    } else {
-      if (u < sides) {
-        const int d = a.inter ? 2 * u : u, e = a.inter ? d + 1 : d + a.F;
-        const float v = load_elt(x, at + d, a.dt), w = load_elt(x, at + e, a.dt);
-        store_elt(y, to + d, v * c[u].x - w * c[u].y, a.dt);
-        store_elt(y, to + e, w * c[u].x + v * c[u].y, a.dt);
-      } else {
-        const int d = 2 * a.F + u - sides;
-        store_elt(y, to + d, load_elt(x, at + d, a.dt), a.dt);
-      }
+  // f(head's input row offset, output row offset, input, output, their row strides, unit, first row, row step) for every unit
+  // of `per` a head: threads over a row's units, and over rows where a row has fewer units than there are threads
+  auto units = [&](int per, int shift, auto &&f) {
+    const int per_t = per * (a.heads + a.k_heads);
+    for (int j = threadIdx.x & ((1 << shift) - 1); j < per_t; j += 1 << shift) {
+      const int h = j / per, u = j - h * per;
+      const bool key = h >= a.heads;
+      const int hk = key ? h - a.heads : h;
+      const size_t x_row = key ? a.k.st : a.x.st, y_row = key ? size_t(a.k_heads) * a.D : size_t(a.xo_st);
+      f(size_t(t0) * x_row + size_t(hk) * (key ? a.k.sh : a.x.sh), size_t(t0) * y_row + size_t(hk) * (key ? (long long)a.D : a.xo_sh),
+        key ? a.k.p : a.x.p, key ? a.ko : a.xo, x_row, y_row, u, int(threadIdx.x) >> shift, kRopeThreads >> shift);
     }
+  };
+  if constexpr (W == 8) {
+    if (a.inter)  // four pairs inside a load
+      units(a.F / 4, a.turn_shift, [&](size_t from, size_t to, const void *x, void *y, size_t xs, size_t ys, int u, int t, int step) {
+        for (; t < nt; t += step) {
+          const bool none = !a.positions && place[t] == kNoRow;
+          float v[8], o[8];
+          load8(x, from + t * xs + u * 8, a.dt, v);
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const float2 r = cs[t * a.F + u * 4 + (e >> 1)];
+            o[e] = none ? 0.0f : v[e] * r.x - v[e + 1] * r.y;
+            o[e + 1] = none ? 0.0f : v[e + 1] * r.x + v[e] * r.y;
+          }
+          store8(y, to + t * ys + u * 8, a.dt, o);
+        }
+      });
+    else  // a load of either side
+      units(a.F / 8, a.turn_shift, [&](size_t from, size_t to, const void *x, void *y, size_t xs, size_t ys, int u, int t, int step) {
+        for (; t < nt; t += step) {
+          const bool none = !a.positions && place[t] == kNoRow;
+          float v[8], w[8], p[8], q[8];
+          load8(x, from + t * xs + u * 8, a.dt, v);
+          load8(x, from + t * xs + u * 8 + a.F, a.dt, w);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float2 r = cs[t * a.F + u * 8 + e];
+            p[e] = none ? 0.0f : v[e] * r.x - w[e] * r.y;
+            q[e] = none ? 0.0f : w[e] * r.x + v[e] * r.y;
+          }
+          store8(y, to + t * ys + u * 8, a.dt, p);
+          store8(y, to + t * ys + u * 8 + a.F, a.dt, q);
+        }
+      });
+    const int wide = a.dt == LMOE_F32 ? 4 : 8;  // channels in 16 bytes
+    if (a.D > 2 * a.F)                          // the other channels, four rows' loads at a time
+      units((a.D - 2 * a.F) / wide, a.copy_shift, [&](size_t from, size_t to, const void *x, void *y, size_t xs, size_t ys, int u,
+                                                      int t, int step) {
+        if (x == y && from == to && xs == ys) return;
+        const int d = (2 * a.F + u * wide) / wide;
+        for (; t < nt; t += 4 * step) {
+          u32x4 v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = static_cast<const u32x4 *>(x)[(from + min(t + i * step, nt - 1) * xs) / wide + d];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (t + i * step < nt) {
+              const bool none = !a.positions && place[t + i * step] == kNoRow;
+              static_cast<u32x4 *>(y)[(to + (t + i * step) * ys) / wide + d] = none ? u32x4{} : v[i];
+            }
+        }
+      });
+  } else {
+    units(a.D - a.F, a.turn_shift, [&](size_t from, size_t to, const void *x, void *y, size_t xs, size_t ys, int u, int t, int step) {
+      for (; t < nt; t += step) {
+        if (u < a.F) {
+          const int d = a.inter ? 2 * u : u, e = a.inter ? d + 1 : d + a.F;
+          const float2 c = cs[t * a.F + u];
+          const float v = load_elt(x, from + t * xs + d, a.dt), w = load_elt(x, from + t * xs + e, a.dt);
+          store_elt(y, to + t * ys + d, v * c.x - w * c.y, a.dt);
+          store_elt(y, to + t * ys + e, w * c.x + v * c.y, a.dt);
+        } else {
+          const int d = u + a.F;
+          store_elt(y, to + t * ys + d, load_elt(x, from + t * xs + d, a.dt), a.dt);
+        }
+      }
+    });
   }
 }
 
+template <int W>
+__global__ void __launch_bounds__(kRopeThreads) k_rope(RopeArgs a) {
+  extern __shared__ float2 cs[];
+  rope_block<W>(a, blockIdx.x * a.tokens, cs);
+}
+
+// Rows a workgroup, and the threads over a row's units. One row while that gives no more than 1,024 workgroups, then up to
+// eight, so that a prompt's cos / sin and sequence search serve more heads.
+static void plan_rope(RopeArgs *a, bool wide) {
+  a->tokens = a->T <= 1024 ? 1 : a->T >= 8192 ? 8 : (a->T + 1023) / 1024;
+  auto shift = [&](int per) {
+    int s = 0;
+    while (s < 8 && (1 << s) < per * (a->heads + a->k_heads)) ++s;
+    return s;
+  };
+  a->turn_shift = shift(!wide ? a->D - a->F : a->inter ? a->F / 4 : a->F / 8);
+  a->copy_shift = shift((a->D - 2 * a->F) / (a->dt == LMOE_F32 ? 4 : 8));
+}
+
 static int launch_rope(const char *fn, RopeArgs a, bool wide, hipStream_t st) {
-  // rows a workgroup: one while that gives no more than 1,024 workgroups, then up to eight, so that a prompt's cos / sin
-  // and sequence search serve more heads
-  a.tokens = a.T <= 1024 ? 1 : a.T >= 8192 ? 8 : (a.T + 1023) / 1024;
+  plan_rope(&a, wide);
   const size_t lds = size_t(a.tokens) * a.F * sizeof(float2);
   const dim3 grid(unsigned((a.T + a.tokens - 1) / a.tokens));
   if (wide)
@@ -199,6 +259,7 @@ struct AppendArgs {
   const double *freq;
   float gain;
   int T, B, heads, D, page, pages, width, F, inter, dt;
+  int tasks;  // workgroups that write pages; those after them rotate rows
 };
 
 // the least s >= -100 with m <= 448 2^s
@@ -224,15 +285,20 @@ __device__ __forceinline__ float finite_or_nan(float v) {
   return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fc00000u) : v;
 }
 
-// One workgroup: the new tokens of one page's head, of keys (blockIdx.z 0, rotated) or of values. Page task x of the call:
-// sequence b's tasks begin at cu[b] / page + 2 b, which leaves it room for every page that its rows can touch, so no task
-// list is made. NV: groups of 8 channels a thread (page * D / 2048).
+// One workgroup: the new tokens of one page's head, of keys (rotated) or of values. Page task t of the call: sequence b's
+// tasks begin at cu[b] / page + 2 b, which leaves it room for every page that its rows can touch, so no task list is made.
+// NV: groups of 8 channels a thread (page * D / 2048). A call of few rows has the workgroups that rotate its queries behind
+// these, in the same launch.
 template <int NV>
-__global__ void __launch_bounds__(256) k_append(AppendArgs a) {
+__global__ void __launch_bounds__(256) k_append(AppendArgs a, RopeArgs rope_rows) {
   extern __shared__ float2 cs[];
   __shared__ float top[4];
-  const int task = blockIdx.x, head = blockIdx.y;
-  const bool key = blockIdx.z == 0;
+  if (int(blockIdx.x) >= a.tasks) {
+    rope_block<8>(rope_rows, (blockIdx.x - a.tasks) * rope_rows.tokens, cs);
+    return;
+  }
+  const int task = blockIdx.x / (2 * a.heads), head = (blockIdx.x >> 1) % a.heads;
+  const bool key = !(blockIdx.x & 1);
   const int page = a.page;
   int b;
   if (a.cu)
@@ -407,15 +473,27 @@ extern "C" int lmoe_kv_append(const void *q, long long q_row, long long q_head, 
                    wide_rows(v, v_row, v_head, D, dtype) && aligned16(k_codes) && aligned16(v_codes),
                LMOE_EALIGN, "%s: rows and codes must be 16-byte aligned", fn);
   hipStream_t st = (hipStream_t)stream;
-  const long long tasks = cu ? T / page + 2ll * B : B;
-  LMOE_REQUIRE(tasks < (1ll << 31), LMOE_ESHAPE, "%s: %d rows of %d sequences", fn, T, B);
+  const long long tasks = (cu ? T / page + 2ll * B : B) * heads * 2;
+  LMOE_REQUIRE(tasks < (1ll << 30), LMOE_ESHAPE, "%s: %d rows of %d sequences and %d heads", fn, T, B, heads);
   AppendArgs a = {{k, k_row, k_head}, {v, v_row, v_head}, k_codes, v_codes, k_scale, v_scale, table, lens, cu, freq, gain,
-                  T, B, heads, D, page, pages, width, n_freq, interleaved, dtype};
+                  T, B, heads, D, page, pages, width, n_freq, interleaved, dtype, int(tasks)};
+  RopeArgs r = {};
+  r.x = {q, q_row, q_head};
+  r.k = {k, k_row, k_head};
+  r.xo = q_out, r.xo_st = (long long)q_heads * D, r.xo_sh = D, r.ko = k_out;
+  r.freq = freq, r.cu = cu, r.lens = lens, r.gain = gain;
+  r.T = T, r.B = B, r.heads = q ? q_heads : 0, r.k_heads = k_out ? heads : 0, r.D = D, r.F = n_freq, r.inter = interleaved;
+  r.dt = dtype;
+  const bool rows = q || k_out;
+  plan_rope(&r, true);
+  // One launch where there are few rows (a launch and its gap cost more than what runs in it); apart for prompts, where the
+  // rotation wants the wavefronts that a page's registers would cost it
+  const bool together = rows && T <= 1024;
   const size_t lds = size_t(cu ? page : 1) * n_freq * sizeof(float2);
-  const dim3 grid = dim3(unsigned(tasks), unsigned(heads), 2);
+  const unsigned grid = unsigned(tasks) + (together ? unsigned(T) : 0u);
   auto go = [&](auto kernel) -> int {
     if (const int rc = allow_lds(kernel, lds, fn)) return rc;
-    launch(kernel, grid, dim3(256), lds, st, a);
+    launch(kernel, dim3(grid), dim3(256), lds, st, a, r);
     LMOE_LAUNCHED(fn);
     return 0;
   };
@@ -427,15 +505,7 @@ extern "C" int lmoe_kv_append(const void *q, long long q_row, long long q_head, 
     case 8: rc = go(k_append<8>); break;
     default: rc = go(k_append<16>); break;
   }
-  if (rc || (!q && !k_out)) return rc;
-  RopeArgs r = {};
-  r.x = {q, q_row, q_head};
-  r.k = {k, k_row, k_head};
-  r.xo = q_out, r.xo_st = (long long)q_heads * D, r.xo_sh = D, r.ko = k_out;
-  r.freq = freq, r.cu = cu, r.lens = lens, r.gain = gain;
-  r.T = T, r.B = B, r.heads = q ? q_heads : 0, r.k_heads = k_out ? heads : 0, r.D = D, r.F = n_freq, r.inter = interleaved;
-  r.dt = dtype;
-  return launch_rope(fn, r, true, st);
+  return rc || !rows || together ? rc : launch_rope(fn, r, true, st);
 }
 
 extern "C" int lmoe_kv_read(const uint8_t *k_codes, const float *k_scale, const uint8_t *v_codes, const float *v_scale, int pages,
