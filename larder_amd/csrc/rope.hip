@@ -132,7 +132,7 @@ __device__ __forceinline__ void rope_block(const RopeArgs &a, int t0, float2 *cs
   __syncthreads();
   // f(head's input row offset, output row offset, input, output, their row strides, unit, first row, row step) for every unit
   // of `per` a head: threads over a row's units, and over rows where a row has fewer units than there are threads
-  auto units = [&](int per, int shift, auto &&f) {
+  auto units = [&](int per, int shift, auto &&f) __attribute__((always_inline)) {
     const int per_t = per * (a.heads + a.k_heads);
     for (int j = threadIdx.x & ((1 << shift) - 1); j < per_t; j += 1 << shift) {
       const int h = j / per, u = j - h * per;
@@ -259,7 +259,7 @@ struct AppendArgs {
   const double *freq;
   float gain;
   int T, B, heads, D, page, pages, width, F, inter, dt;
-  int tasks;  // workgroups that write pages; those after them rotate rows
+  int rotating;  // workgroups that rotate rows; those after them write pages
 };
 
 // the least s >= -100 with m <= 448 2^s
@@ -287,18 +287,19 @@ __device__ __forceinline__ float finite_or_nan(float v) {
 
 // One workgroup: the new tokens of one page's head, of keys (rotated) or of values. Page task t of the call: sequence b's
 // tasks begin at cu[b] / page + 2 b, which leaves it room for every page that its rows can touch, so no task list is made.
-// NV: groups of 8 channels a thread (page * D / 2048). A call of few rows has the workgroups that rotate its queries behind
-// these, in the same launch.
+// NV: groups of 8 channels a thread (page * D / 2048). A call of few rows has the workgroups that rotate its queries
+// before these, in the same launch.
 template <int NV>
 __global__ void __launch_bounds__(256) k_append(AppendArgs a, RopeArgs rope_rows) {
   extern __shared__ float2 cs[];
   __shared__ float top[4];
-  if (int(blockIdx.x) >= a.tasks) {
-    rope_block<8>(rope_rows, (blockIdx.x - a.tasks) * rope_rows.tokens, cs);
+  const int block = int(blockIdx.x) - a.rotating;
+  if (block < 0) {
+    rope_block<8>(rope_rows, blockIdx.x * rope_rows.tokens, cs);
     return;
   }
-  const int task = blockIdx.x / (2 * a.heads), head = (blockIdx.x >> 1) % a.heads;
-  const bool key = !(blockIdx.x & 1);
+  const int task = block / (2 * a.heads), head = (block >> 1) % a.heads;
+  const bool key = !(block & 1);
   const int page = a.page;
   int b;
   if (a.cu)
@@ -476,7 +477,7 @@ extern "C" int lmoe_kv_append(const void *q, long long q_row, long long q_head, 
   const long long tasks = (cu ? T / page + 2ll * B : B) * heads * 2;
   LMOE_REQUIRE(tasks < (1ll << 30), LMOE_ESHAPE, "%s: %d rows of %d sequences and %d heads", fn, T, B, heads);
   AppendArgs a = {{k, k_row, k_head}, {v, v_row, v_head}, k_codes, v_codes, k_scale, v_scale, table, lens, cu, freq, gain,
-                  T, B, heads, D, page, pages, width, n_freq, interleaved, dtype, int(tasks)};
+                  T, B, heads, D, page, pages, width, n_freq, interleaved, dtype, 0};
   RopeArgs r = {};
   r.x = {q, q_row, q_head};
   r.k = {k, k_row, k_head};
@@ -490,7 +491,8 @@ extern "C" int lmoe_kv_append(const void *q, long long q_row, long long q_head, 
   // rotation wants the wavefronts that a page's registers would cost it
   const bool together = rows && T <= 1024;
   const size_t lds = size_t(cu ? page : 1) * n_freq * sizeof(float2);
-  const unsigned grid = unsigned(tasks) + (together ? unsigned(T) : 0u);
+  a.rotating = together ? T : 0;
+  const unsigned grid = unsigned(tasks + a.rotating);
   auto go = [&](auto kernel) -> int {
     if (const int rc = allow_lds(kernel, lds, fn)) return rc;
     launch(kernel, dim3(grid), dim3(256), lds, st, a, r);
