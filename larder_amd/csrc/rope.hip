@@ -259,7 +259,7 @@ struct AppendArgs {
   const double *freq;
   float gain;
   int T, B, heads, D, page, pages, width, F, inter, dt;
-  int rotating;  // workgroups that rotate rows; those after them write pages
+  int pages_at, tasks;  // the workgroups that write pages: tasks of them from pages_at on; the others rotate rows
 };
 
 // the least s >= -100 with m <= 448 2^s
@@ -287,15 +287,14 @@ __device__ __forceinline__ float finite_or_nan(float v) {
 
 // One workgroup: the new tokens of one page's head, of keys (rotated) or of values. Page task t of the call: sequence b's
 // tasks begin at cu[b] / page + 2 b, which leaves it room for every page that its rows can touch, so no task list is made.
-// NV: groups of 8 channels a thread (page * D / 2048). A call of few rows has the workgroups that rotate its queries
-// before these, in the same launch.
+// NV: groups of 8 channels a thread (page * D / 2048). The workgroups that rotate queries share the launch.
 template <int NV>
 __global__ void __launch_bounds__(256) k_append(AppendArgs a, RopeArgs rope_rows) {
   extern __shared__ float2 cs[];
   __shared__ float top[4];
-  const int block = int(blockIdx.x) - a.rotating;
-  if (block < 0) {
-    rope_block<8>(rope_rows, blockIdx.x * rope_rows.tokens, cs);
+  const int block = int(blockIdx.x) - a.pages_at;
+  if (block < 0 || block >= a.tasks) {
+    rope_block<8>(rope_rows, (block < 0 ? int(blockIdx.x) : block - a.tasks) * rope_rows.tokens, cs);
     return;
   }
   const int task = block / (2 * a.heads), head = (block >> 1) % a.heads;
@@ -477,7 +476,7 @@ extern "C" int lmoe_kv_append(const void *q, long long q_row, long long q_head, 
   const long long tasks = (cu ? T / page + 2ll * B : B) * heads * 2;
   LMOE_REQUIRE(tasks < (1ll << 30), LMOE_ESHAPE, "%s: %d rows of %d sequences and %d heads", fn, T, B, heads);
   AppendArgs a = {{k, k_row, k_head}, {v, v_row, v_head}, k_codes, v_codes, k_scale, v_scale, table, lens, cu, freq, gain,
-                  T, B, heads, D, page, pages, width, n_freq, interleaved, dtype, 0};
+                  T, B, heads, D, page, pages, width, n_freq, interleaved, dtype, 0, int(tasks)};
   RopeArgs r = {};
   r.x = {q, q_row, q_head};
   r.k = {k, k_row, k_head};
@@ -487,12 +486,14 @@ extern "C" int lmoe_kv_append(const void *q, long long q_row, long long q_head, 
   r.dt = dtype;
   const bool rows = q || k_out;
   plan_rope(&r, true);
-  // One launch where there are few rows (a launch and its gap cost more than what runs in it); apart for prompts, where the
-  // rotation wants the wavefronts that a page's registers would cost it
-  const bool together = rows && T <= 1024;
-  const size_t lds = size_t(cu ? page : 1) * n_freq * sizeof(float2);
-  a.rotating = together ? T : 0;
-  const unsigned grid = unsigned(tasks + a.rotating);
+  // One launch: the rotation hides the latency of the pages' few workgroups (prompts at width 256: 18 + 33 us apart, 46
+  // together), and a token's call saves a launch. Pages go first where there are many rows, so that their chain of loads is
+  // not what the launch ends with. Apart only where a page's registers would leave the rotation two wavefronts a SIMD.
+  const bool together = rows && (T <= 1024 || page * D <= 16384);
+  const int rotating = together ? (T + r.tokens - 1) / r.tokens : 0;
+  a.pages_at = T <= 1024 ? rotating : 0;
+  const size_t lds = size_t(max(cu ? page : 1, r.tokens)) * n_freq * sizeof(float2);
+  const unsigned grid = unsigned(tasks + rotating);
   auto go = [&](auto kernel) -> int {
     if (const int rc = allow_lds(kernel, lds, fn)) return rc;
     launch(kernel, dim3(grid), dim3(256), lds, st, a, r);
