@@ -514,7 +514,7 @@ int lmoe_rope_rows(const void *x, int dtype, long long x_row, long long x_head, 
  * lmoe_kv_read: rows cu[b] .. cu[b + 1] of k_out / v_out [total][heads][D] get sequence b's first tokens, code times scale.
  * lmoe_kv_attend: out [T][q_heads][D] = softmax(scale q k^T) v in float16 / bfloat16, row r of a sequence's n over its first
  * lens - n + r + 1 tokens (none: zero). most_rows / longest: about the most rows / tokens of a sequence (any value is sound;
- * they size the launch). workspace: lmoe_kv_attend_workspace_bytes of the same numbers, 16-byte aligned. B <= 65535. */
+ * they size the launch). workspace: lmoe_kv_attend_workspace_bytes of the same numbers, 16-byte aligned. */
 int lmoe_kv_append(const void *q, long long q_row, long long q_head, int q_heads, const void *k, long long k_row,
                    long long k_head, const void *v, long long v_row, long long v_head, int dtype, int T, int heads, int D,
                    const int *cu, const int *lens, int B, const int *table, int width, uint8_t *k_codes, float *k_scale,
@@ -532,10 +532,13 @@ int lmoe_kv_attend(const void *q, int dtype, long long q_row, long long q_head, 
 /* Attention over whole prompts, causal: q [T][q_heads][D], k and v [U][heads][D] (float16 or bfloat16; q_heads a multiple of
  * heads; D 64, 128 or 256), sequence b's rows cu[b] .. cu[b + 1] of q over keys cu_k[b] .. cu_k[b + 1]: the last row sees all of
  * them, each one before it one fewer (none: zero). out [T][q_heads][D] dense, in dtype. Rows of k and v are less than 2^23
- * elements apart. The reference runs its trunk's prompt attention on MLX (cpu_ext/cpu_kern.cpp:493-659 is its CPU form). */
+ * elements apart. workspace: lmoe_prompt_attend_workspace_bytes of the same numbers (0: none), 16-byte aligned. The
+ * reference runs its trunk's prompt attention on MLX (cpu_ext/cpu_kern.cpp:493-659 is its CPU form). */
 int lmoe_prompt_attend(const void *q, long long q_row, long long q_head, const void *k, long long k_row, long long k_head,
                        const void *v, long long v_row, long long v_head, int dtype, int T, int U, int q_heads, int heads, int D,
-                       const int *cu, const int *cu_k, int B, float scale, void *out, void *stream);
+                       const int *cu, const int *cu_k, int B, float scale, void *workspace, size_t workspace_bytes, void *out,
+                       void *stream);
+size_t lmoe_prompt_attend_workspace_bytes(int T, int U, int q_heads, int heads, int D, int B);
 
 #ifdef __cplusplus
 }

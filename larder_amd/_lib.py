@@ -112,7 +112,9 @@ SIGNATURES = {
     "lmoe_kv_attend_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I]),
     "lmoe_kv_attend": (_I, [_P, _I, _LL, _LL, _I, _I, _I, _I, _P, _P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _F, _P, _SZ,
                             _P, _P]),
-    "lmoe_prompt_attend": (_I, [_P, _LL, _LL, _P, _LL, _LL, _P, _LL, _LL, _I, _I, _I, _I, _I, _I, _P, _P, _I, _F, _P, _P]),
+    "lmoe_prompt_attend": (_I, [_P, _LL, _LL, _P, _LL, _LL, _P, _LL, _LL, _I, _I, _I, _I, _I, _I, _P, _P, _I, _F, _P, _SZ, _P,
+                                _P]),
+    "lmoe_prompt_attend_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I]),
 }
 
 _LIB = None

@@ -189,6 +189,11 @@ def _attend_workspace(*sizes):
     return _lib.lib().lmoe_kv_attend_workspace_bytes(*sizes)
 
 
+@functools.lru_cache(maxsize=1024)
+def _prompt_workspace(*sizes):
+    return _lib.lib().lmoe_prompt_attend_workspace_bytes(*sizes)
+
+
 # ---- the calls -------------------------------------------------------------------------------------------------
 
 def rope_rows(x, positions, freq, interleaved=False, gain=1.0, out=None):
@@ -339,7 +344,9 @@ def prompt_rows(q, k, v, cu, cu_k=None, scale=None):
     out = torch.empty((t, q_heads, width), dtype=dtype, device=q.device)
     if not t or not n:
         return out.zero_()
+    need = _prompt_workspace(t, u, q_heads, heads, width, n)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     _launch(dev, "lmoe_prompt_attend", q.data_ptr(), q_row, q_head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
             dcode(dtype), t, u, q_heads, heads, width, cu.data_ptr(), (cu if cu_k is None else cu_k).data_ptr(), n,
-            width ** -0.5 if scale is None else scale, out.data_ptr())
+            width ** -0.5 if scale is None else scale, None if ws is None else ws.data_ptr(), need, out.data_ptr())
     return out

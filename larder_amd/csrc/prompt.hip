@@ -29,8 +29,10 @@ struct PromptArgs {
   long long q_row, q_head, k_row, k_head, v_row, v_head;  // elements
   const int *cu, *cu_k;
   uint16_t *out;
+  float *part;  // [chunks][T][q_heads] of [D] sums and {maximum, weight}: rows whose keys are worked in more than one chunk
+  int *joins;   // [T][q_heads]: how many chunks (0: one, the row is done)
   float scale;  // times log2 e
-  int T, U, B, q_heads, heads, tiles;
+  int T, U, B, q_heads, heads, tiles, chunk, chunks;  // chunk: keys, the last of `chunks` goes on to the end
 };
 
 // A weight is 2^(score - maximum in use + kLift), the maximum lagging at most kLag: float16 weights reach 2^15 at most, and
@@ -142,7 +144,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_prompt(PromptArgs a) 
   __shared__ uint32_t marks[2 * BN * DT];   // of take_bad: [pos, neg][key][32 channels]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, h = lane >> 5;
   // heads of one XCD are neighbours (they share key heads in its L2); later tiles, which see more keys, go first
-  const int slot = blockIdx.x % a.q_heads, task = a.tiles - 1 - int(blockIdx.x) / a.q_heads;
+  const int slot = blockIdx.x % a.q_heads, chunk = int(blockIdx.x) / a.q_heads % a.chunks;
+  const int task = a.tiles - 1 - int(blockIdx.x) / (a.q_heads * a.chunks);
   const int head = a.q_heads % 8 == 0 ? (slot & 7) * (a.q_heads / 8) + (slot >> 3) : slot;
   const int b = last_at(a.cu, a.B, task, [](int c, int i) { return (long long)(c / kPromptRows) + i; });
   if (b < 0) return;
@@ -150,18 +153,23 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_prompt(PromptArgs a) 
   seq_rows(a.cu, b, a.T, &row0, &nq);
   seq_rows(a.cu_k, b, a.U, &key0, &nk);
   const int tile = task - (a.cu[b] / kPromptRows + b);
-  if (tile == 0 && (b == 0 || b == a.B - 1)) {
+  if (tile == 0 && chunk == 0 && (b == 0 || b == a.B - 1)) {
     // rows before the first sequence or behind the last one come back zero
     const int lo = b == 0 ? min(max(a.cu[0], 0), a.T) : 0, hi = b == a.B - 1 ? min(max(a.cu[a.B], 0), a.T) : a.T;
     for (int row = int(threadIdx.x) / (D / 8); row < lo + (a.T - hi); row += 256 / (D / 8)) {
       const size_t line = size_t(row < lo ? row : hi + row - lo) * a.q_heads + head;
       *reinterpret_cast<u32x4 *>(a.out + line * D + (threadIdx.x % (D / 8)) * 8) = u32x4{};
+      if (a.joins) a.joins[line] = 0;
     }
   }
   const int first = tile * kPromptRows;
   if (first >= nq) return;
   const int off = nk - nq;                                  // row i sees keys 0 .. i + off
-  const int keys = off + min(first + kPromptRows, nq);      // what the workgroup's last row sees
+  const int most_keys = off + min(first + kPromptRows, nq);  // what the workgroup's last row sees
+  const int begin = chunk * a.chunk;                         // this workgroup's keys: [begin, keys)
+  if (chunk > 0 && begin >= most_keys) return;
+  const int keys = chunk + 1 < a.chunks ? min(most_keys, begin + a.chunk) : most_keys;
+  const int parts = a.part ? min(a.chunks, (most_keys - 1) / a.chunk + 1) : 1;  // chunks that the tile's keys take
   const int mine = min(first + 32 * wave + r, nq - 1), sees = mine + off + 1;
   const int all = first + 32 * wave + off + 1;  // what every row of the wavefront sees
   const int kv = head / (a.q_heads / a.heads);
@@ -194,10 +202,10 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_prompt(PromptArgs a) 
 #pragma unroll
     for (int i = 0; i < COPIES; ++i) dma_rows(rows, v_off[i], to + (2 + stage) * kTileBytes + i * 1024);
   };
-  if (keys > 0) {
-    fetch_k(0, 0);
-    fetch_v(0, 0);
-    fetch_k(BN, 1);
+  if (keys > begin) {
+    fetch_k(begin, 0);
+    fetch_v(begin, 0);
+    fetch_k(begin + BN, 1);
   }
   u32x4 qf[KS];
   {
@@ -235,7 +243,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_prompt(PromptArgs a) 
   f32x16 s[MT] = {};  // the scores of the tile at hand
   // The compiler's own wait for q, here: it does not see the copies, and one left to the loop would wait for them too
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-  if (keys > 0) {
+  if (keys > begin) {
     wait_vm<0>();
     barrier_lds();
 #pragma unroll
@@ -351,7 +359,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_prompt(PromptArgs a) 
     }
   };
   f32x16 other[MT];
-  for (int at = 0; at < keys; at += 2 * BN) {
+  for (int at = begin; at < keys; at += 2 * BN) {
     step(at, IC<0>{}, s, other);
     if (at + BN >= keys) break;
     step(at + BN, IC<1>{}, other, s);
@@ -359,8 +367,22 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_prompt(PromptArgs a) 
   wait_vm<0>();  // the last tiles' copies (of nothing) land before the LDS is another workgroup's
   l += lane_xor32(l);
   if (first + 32 * wave + r >= nq) return;
+  const size_t line = size_t(row0 + mine) * a.q_heads + head;
+  if (a.part) {
+    if (chunk == 0 && h == 0) a.joins[line] = parts > 1 ? parts : 0;
+    if (parts > 1) {
+      float *part = a.part + (size_t(chunk) * a.T * a.q_heads + line) * (D + 4);
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<f32x4 *>(part + 32 * d + 8 * e + 4 * h) = f32x4{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
+      if (h == 0) *reinterpret_cast<float2 *>(part + D) = float2{m, l};
+      return;
+    }
+  }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint16_t *out = a.out + (size_t(row0 + mine) * a.q_heads + head) * D;
+  uint16_t *out = a.out + line * D;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -369,14 +391,75 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_prompt(PromptArgs a) 
           u32x2{pack2<BF>(o[d][4 * e] * inv, o[d][4 * e + 1] * inv), pack2<BF>(o[d][4 * e + 2] * inv, o[d][4 * e + 3] * inv)};
 }
 
+// Rows whose keys were worked in more than one chunk: D / 4 threads a row and head, the chunks joined in order
+template <int D, bool BF>
+__global__ void __launch_bounds__(256) k_prompt_join(PromptArgs a) {
+  constexpr int LANES = D / 4;
+  const size_t line = size_t(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES, lines = size_t(a.T) * a.q_heads;
+  if (line >= lines) return;
+  const int parts = min(a.joins[line], a.chunks), d = (threadIdx.x % LANES) * 4;
+  if (parts < 2) return;
+  f32x4 v = {};
+  float top = -INFINITY, weight = 0.0f;
+  for (int c0 = 0; c0 < parts; c0 += 4) {
+    float2 ml[4];
+    f32x4 y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float *part = a.part + (size_t(min(c0 + j, parts - 1)) * lines + line) * (D + 4);
+      ml[j] = *reinterpret_cast<const float2 *>(part + D);
+      y[j] = *reinterpret_cast<const f32x4 *>(part + d);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (c0 + j >= parts || ml[j].y == 0.0f) continue;  // (a chunk that the row sees nothing of weighs 0; NaN goes on)
+      const float to = fmaxf(top, ml[j].x), f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml[j].x - to);
+      const float keep = weight == 0.0f ? 0.0f : to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - to);
+      top = to;
+      weight = fmaf(ml[j].y, f, weight * keep);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = fmaf(y[j][e], f, v[e] * keep);
+    }
+  }
+  const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
+  *reinterpret_cast<u32x2 *>(a.out + line * D + d) = u32x2{pack2<BF>(v[0] * inv, v[1] * inv), pack2<BF>(v[2] * inv, v[3] * inv)};
+}
+
+// Chunks of keys, where the rows alone would leave CUs idle: as many as bring the workgroups to two a CU (one at width 256),
+// of 512 keys (eight tiles) at least
+struct PromptPlan {
+  int chunk, chunks;
+  size_t rows, bytes;  // the workspace's sums, and all of it
+};
+static PromptPlan prompt_plan(int T, int U, int q_heads, int D, int B) {
+  PromptPlan p = {1 << 30, 1, 0, 0};
+  const long long work = (long long)((T + kPromptRows - 1) / kPromptRows) * q_heads, full = D == 256 ? 256 : 512;
+  if (work <= 0 || 2 * work > full) return p;
+  const int splits = int(full / work);
+  long long chunk = ((long long)U / (B > 0 ? B : 1) + splits - 1) / splits;
+  chunk = (chunk < 512 ? 512 : chunk) + kPromptKeys - 1;
+  chunk -= chunk % kPromptKeys;
+  const long long chunks = (U + chunk - 1) / chunk, most = 4ll * splits;
+  if (chunks <= 1) return p;
+  p.chunk = int(chunk);
+  p.chunks = int(chunks < most ? chunks : most);
+  p.rows = size_t(p.chunks) * T * q_heads * (D + 4) * sizeof(float);
+  p.bytes = p.rows + size_t(T) * q_heads * sizeof(int);
+  return p;
+}
+
 }  // namespace lmoe
 
 using namespace lmoe;
 
+extern "C" size_t lmoe_prompt_attend_workspace_bytes(int T, int U, int q_heads, int heads, int D, int B) {
+  return T > 0 && U > 0 && q_heads > 0 ? prompt_plan(T, U, q_heads, D, B).bytes : 0;
+}
+
 extern "C" int lmoe_prompt_attend(const void *q, long long q_row, long long q_head, const void *k, long long k_row,
                                   long long k_head, const void *v, long long v_row, long long v_head, int dtype, int T, int U,
-                                  int q_heads, int heads, int D, const int *cu, const int *cu_k, int B, float scale, void *out,
-                                  void *stream) {
+                                  int q_heads, int heads, int D, const int *cu, const int *cu_k, int B, float scale, void *workspace,
+                                  size_t workspace_bytes, void *out, void *stream) {
   const char *fn = "lmoe_prompt_attend";
   LMOE_REQUIRE(dtype == LMOE_F16 || dtype == LMOE_BF16, LMOE_EINVAL, "%s: dtype %d (float16 and bfloat16 are served)", fn, dtype);
   LMOE_REQUIRE(D == 64 || D == 128 || D == 256, LMOE_ESHAPE, "%s: heads of %d channels (64, 128 and 256 are served)", fn, D);
@@ -393,19 +476,28 @@ extern "C" int lmoe_prompt_attend(const void *q, long long q_row, long long q_he
   LMOE_REQUIRE(k_row >= 0 && v_row >= 0 && k_row < (1 << 23) && v_row < (1 << 23), LMOE_ESHAPE,
                "%s: rows of keys %lld and of values %lld elements apart", fn, k_row, v_row);
   const long long tiles = T / kPromptRows + (long long)B;
-  LMOE_REQUIRE(tiles * q_heads < (1ll << 31), LMOE_ESHAPE, "%s: %d rows of %d heads", fn, T, q_heads);
+  const PromptPlan plan = prompt_plan(T, U, q_heads, D, B);
+  LMOE_REQUIRE(tiles * q_heads * plan.chunks < (1ll << 31), LMOE_ESHAPE, "%s: %d rows of %d heads", fn, T, q_heads);
+  LMOE_REQUIRE(plan.bytes == 0 || (workspace && aligned16(workspace) && workspace_bytes >= plan.bytes), LMOE_EWORKSPACE,
+               "%s: a 16-byte aligned workspace of %zu bytes is needed", fn, plan.bytes);
+  float *part = plan.bytes ? static_cast<float *>(workspace) : nullptr;
+  int *joins = plan.bytes ? reinterpret_cast<int *>(static_cast<char *>(workspace) + plan.rows) : nullptr;
   PromptArgs a = {static_cast<const uint16_t *>(q), static_cast<const uint16_t *>(k), static_cast<const uint16_t *>(v), q_row,
-                  q_head, k_row, k_head, v_row, v_head, cu, cu_k, static_cast<uint16_t *>(out), scale * 1.4426950408889634f, T, U,
-                  B, q_heads, heads, int(tiles)};
-  auto go = [&](auto kernel) -> int {
+                  q_head, k_row, k_head, v_row, v_head, cu, cu_k, static_cast<uint16_t *>(out), part, joins,
+                  scale * 1.4426950408889634f, T, U, B, q_heads, heads, int(tiles), plan.chunk, plan.chunks};
+  auto go = [&](auto kernel, auto join) -> int {
     const size_t lds = size_t(kPromptKeys) * D * 2 * 4;
     if (const int rc = allow_lds(kernel, lds, fn)) return rc;
-    launch(kernel, dim3(unsigned(tiles * q_heads)), dim3(256), lds, (hipStream_t)stream, a);
+    launch(kernel, dim3(unsigned(tiles * q_heads * plan.chunks)), dim3(256), lds, (hipStream_t)stream, a);
     LMOE_LAUNCHED(fn);
+    if (part) {
+      launch(join, dim3(unsigned(((long long)T * q_heads * (D / 4) + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a);
+      LMOE_LAUNCHED(fn);
+    }
     return 0;
   };
   const bool bf = dtype == LMOE_BF16;
-  if (D == 64) return bf ? go(k_prompt<64, true>) : go(k_prompt<64, false>);
-  if (D == 128) return bf ? go(k_prompt<128, true>) : go(k_prompt<128, false>);
-  return bf ? go(k_prompt<256, true>) : go(k_prompt<256, false>);
+  if (D == 64) return bf ? go(k_prompt<64, true>, k_prompt_join<64, true>) : go(k_prompt<64, false>, k_prompt_join<64, false>);
+  if (D == 128) return bf ? go(k_prompt<128, true>, k_prompt_join<128, true>) : go(k_prompt<128, false>, k_prompt_join<128, false>);
+  return bf ? go(k_prompt<256, true>, k_prompt_join<256, true>) : go(k_prompt<256, false>, k_prompt_join<256, false>);
 }

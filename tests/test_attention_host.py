@@ -105,7 +105,6 @@ def test_entry_points_refuse(built_lib):
     refused(L, _lib.ESHAPE, b"query heads", "lmoe_kv_attend", *attend(qh=3, h=2))
     refused(L, _lib.ESHAPE, b"channels", "lmoe_kv_attend", *attend(D=192))
     refused(L, _lib.ESHAPE, b"tokens", "lmoe_kv_attend", *attend(page=256))
-    refused(L, _lib.ESHAPE, b"sequences", "lmoe_kv_attend", *attend(B=65536))
     refused(L, _lib.ESHAPE, b"sequences", "lmoe_kv_attend", *attend(longest=0))
     refused(L, _lib.ESHAPE, b"offsets", "lmoe_kv_attend", *attend(cu=None))
     refused(L, _lib.EINVAL, b"null", "lmoe_kv_attend", *attend(q=None))
@@ -113,8 +112,8 @@ def test_entry_points_refuse(built_lib):
     refused(L, _lib.EWORKSPACE, b"workspace", "lmoe_kv_attend", *attend(wsb=16))
     refused(L, _lib.EWORKSPACE, b"workspace", "lmoe_kv_attend", *attend(ws=None))
 
-    def prompt(q=P, k=P, st=64, kst=64, dt=1, T=2, U=2, qh=1, h=1, D=64, cu=P, B=1):
-        return q, st, 64, k, kst, 64, P, 64, 64, dt, T, U, qh, h, D, cu, P, B, 0.125, P
+    def prompt(q=P, k=P, st=64, kst=64, dt=1, T=2, U=2, qh=1, h=1, D=64, cu=P, B=1, ws=P, wsb=1 << 30):
+        return q, st, 64, k, kst, 64, P, 64, 64, dt, T, U, qh, h, D, cu, P, B, 0.125, ws, wsb, P
 
     refused(L, _lib.EINVAL, b"dtype", "lmoe_prompt_attend", *prompt(dt=0))
     refused(L, _lib.ESHAPE, b"channels", "lmoe_prompt_attend", *prompt(D=80))
@@ -123,14 +122,20 @@ def test_entry_points_refuse(built_lib):
     refused(L, _lib.EINVAL, b"null", "lmoe_prompt_attend", *prompt(cu=None))
     refused(L, _lib.EALIGN, b"aligned", "lmoe_prompt_attend", *prompt(q=ODD))
     refused(L, _lib.ESHAPE, b"apart", "lmoe_prompt_attend", *prompt(kst=1 << 23))
+    refused(L, _lib.EWORKSPACE, b"workspace", "lmoe_prompt_attend", *prompt(U=8192, wsb=16))
+    refused(L, _lib.EWORKSPACE, b"workspace", "lmoe_prompt_attend", *prompt(U=8192, ws=None))
     assert L.lmoe_prompt_attend(*prompt(T=0), None) == 0
 
 
 def test_attend_workspace(built_lib):
     need = built_lib.lmoe_kv_attend_workspace_bytes
-    assert need(1, 16, 16, 128, 1, 1, 100) == 0                      # one chunk: nothing to join
-    assert need(1, 32, 4, 128, 1, 1, 8192) % (32 * 130 * 4) == 0 and need(1, 32, 4, 128, 1, 1, 8192) > 0
-    assert need(1, 3, 2, 128, 1, 1, 8192) == 0                       # refused shapes ask for nothing
+    assert need(1, 16, 16, 128, 1, 1, 100) == 0                       # each sequence whole: nothing to join
+    assert need(1, 32, 4, 128, 1, 1, 8192) == 256 * 2 * 16 * 130 * 4 + 32 * 8   # 64 units of 4 heads: two places each
+    assert need(64, 32, 4, 128, 64, 1, 8192) == 512 * 2 * 16 * 130 * 4 + 64 * 32 * 8  # at most two workgroups a CU
+    assert need(1, 3, 2, 128, 1, 1, 8192) == 0                        # refused shapes ask for nothing
+    need = built_lib.lmoe_prompt_attend_workspace_bytes
+    assert need(8192, 8192, 32, 4, 128, 1) == 0 and need(300, 300, 4, 4, 128, 1) == 0
+    assert need(100, 8100, 28, 4, 128, 1) == 16 * 100 * 28 * 132 * 4 + 100 * 28 * 4  # 28 workgroups: 18 chunks, 512 keys at least
 
 
 @pytest.mark.parametrize("unit,spare", [(32, 2), (64, 2), (128, 2), (128, 1)])
