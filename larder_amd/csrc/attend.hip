@@ -197,16 +197,23 @@ __global__ void __launch_bounds__(64 * kAttendWaves, D == 256 ? 2 : 3) k_attend(
   char *seqs_at = reinterpret_cast<char *>(lds) + kSumsLds<D>;
   Seqs seqs = {reinterpret_cast<int3 *>(seqs_at + kAttendWaves * 64 * sizeof(int)) + wave * 64,
                reinterpret_cast<int *>(seqs_at) + wave * 64, 0, 0};
-  int line = 0;
-  for (int b0 = (a.B - 1) & ~63; b0 > 0; b0 -= 64) {  // the first ones last: they stay
-    seqs.load(a, b0, 0);
-    line += seqs.end();
-  }
   seqs.load(a, 0, 0);
-  line += seqs.end();
-  int at_unit = stretch(line, blockIdx.x, a.groups);
-  const int stop_unit = stretch(line, blockIdx.x + 1, a.groups);
-  if (at_unit >= stop_unit) return;
+  int line = seqs.end();
+  if (a.B > 64) {  // the rest of the line: a lane adds up every 64th sequence
+    int more = 0;
+#pragma unroll 4
+    for (int b = 64 + lane; b < a.B; b += 64) {
+      int row0, n;
+      seq_rows(a.cu, b, a.T, &row0, &n);
+      more += share(a, row0, n, a.lens[b]).total(a.heads);
+    }
+    line += __builtin_amdgcn_readlane(wave_scan(more), 63);
+  }
+  // no more workgroups than units: each has one at least, so that every one between an item's first and last writes its place
+  const int groups = min(a.groups, line);
+  if (int(blockIdx.x) >= groups) return;
+  int at_unit = stretch(line, blockIdx.x, groups);
+  const int stop_unit = stretch(line, blockIdx.x + 1, groups);
   const int first_unit = at_unit;
   const int page_tokens = 1 << a.page_shift;
   const size_t head_bytes = size_t(page_tokens) * D, page_bytes = head_bytes * a.heads;
@@ -225,7 +232,7 @@ __global__ void __launch_bounds__(64 * kAttendWaves, D == 256 ? 2 : 3) k_attend(
     const int last = min(16 * rt + 15, rows - 1) / a.group;
     // this stretch's tokens [begin, end): an item's last unit ends with what its last row sees
     const int begin = unit0 << a.unit_shift;
-    int end = s.len - s.n + last + 1;
+    int end = min(s.len - s.n + last + 1, a.width << a.page_shift);  // (the table has no places past that)
     if (unit0 + units < s.units) end = min(end, begin + (units << a.unit_shift));
     // the lane's row: query row `mine` of the sequence, seeing the first `sees` places; every row sees those below `all`
     const int flat = min(16 * rt + r, rows - 1), mine = flat / a.group, sub = flat - mine * a.group;
@@ -394,7 +401,7 @@ __global__ void __launch_bounds__(64 * kAttendWaves, D == 256 ? 2 : 3) k_attend(
     __syncthreads();
     if (a.part && unit0 == 0) {  // what the joining kernel has to do for the item's rows
       const int2 join = {whole ? -1 : int(blockIdx.x) * 2 + (at_unit == first_unit ? 0 : 1),
-                         int(((long long)(at_unit + s.units) * a.groups - 1) / line) * 16 + tid};
+                         int(((long long)(at_unit + s.units) * groups - 1) / line) * 16 + tid};
       const int fl = 16 * rt + tid, qr = fl / a.group;
       if (tid < 16 && fl < rows) a.joins[size_t(s.row0 + qr) * a.q_heads + head * a.group + (fl - qr * a.group)] = join;
     }

@@ -15,6 +15,13 @@ pytestmark = pytest.mark.gpu
 F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
 
 
+@pytest.fixture(autouse=True)
+def poisoned_memory():
+    """What outputs and workspaces are allocated from holds NaN."""
+    for n in (1 << 16, 1 << 18, 1 << 22, 1 << 25):
+        torch.full((n,), float("nan"), device="cuda")
+
+
 def host(t):
     return t.detach().double().cpu().numpy()
 
@@ -220,6 +227,29 @@ def test_append_edges():
     assert q.shape == (0, 1, 64) and kk is None
 
 
+@pytest.mark.parametrize("page,heads,width,rows", [(128, 1, 256, [1500, 3]), (64, 2, 128, [1100, 0, 64]), (32, 1, 64, [8200])])
+def test_append_prompts(page, heads, width, rows):
+    """Calls of more than 1,024 rows (several rows a rotating workgroup; widest pages: a launch of their own)."""
+    from larder_amd import attention
+    rng = np.random.default_rng(19)
+    cu, t = cu_of(rows), sum(rows)
+    table, n = page_table(rng, [-(-x // page) for x in rows])
+    cache = poisoned(n, heads, width, page)
+    want = cache_host(cache)
+    freq = frequencies(width // 4)
+    x = normal(rng, t + 1, 4 * heads, width)
+    q, k, v = x.split([2 * heads, heads, heads], 1)
+    got = attention.append_rows(cache, q, k, v, ints(table), ints(rows), cu=ints(cu), freq=freq, keys=True)
+    pos = np.concatenate([np.arange(m) for m in rows] + [[0]])
+    for a, b in zip((q, k), got):
+        w = ref.rope(host(a), pos, host(freq))
+        assert (np.abs(host(b) - w) <= rope_bound(host(a), w, freq, 1.0, BF16))[:t].all() and (b[t:] == 0).all()
+    ref.append(*want[0], ref.rope(host(k), pos, host(freq)), cu, rows, table)
+    ref.append(*want[1], host(v), cu, rows, table)
+    for (codes, scales), (gc, gs) in zip(want, cache_host(cache)):
+        assert np.array_equal(scales, gs, equal_nan=True) and close_codes(gc, codes, 1e-4)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("page,heads,width", [(32, 3, 64), (64, 4, 128), (128, 2, 256)])
 def test_read(dtype, page, heads, width):
@@ -346,6 +376,26 @@ def test_attend_holes_and_nan(longest):
     assert (gone == 0).all()
 
 
+def test_attend_many_sequences():
+    """More sequences than a wavefront has lanes, empty ones and ones longer than their table among them."""
+    from larder_amd import attention
+    rng = np.random.default_rng(20)
+    lens = [int(x) for x in rng.choice([0, 1, 5, 40, 64, 130, 700], 150)]
+    lens[7], lens[100] = 2 ** 31 - 1, 900
+    rows = [int(x) for x in rng.choice([0, 1, 2], 150)]
+    rows[7] = rows[100] = 1
+    cu = cu_of(rows)
+    table, n = page_table(rng, [min(-(-x // 32), 22) for x in lens], width=22)
+    cache = random_cache(rng, n, 1, 64, 32)
+    q = normal(rng, cu[-1], 3, 64, dtype=F16)
+    got = attention.attend_rows(q, cache, ints(table), ints(lens), cu=ints(cu), longest=704)
+    for b in range(150):
+        if rows[b]:
+            at = slice(cu[b], cu[b + 1])
+            check_attend(got[at], q[at], cache, table[b:b + 1], [min(lens[b], 704)], [0, rows[b]], 0.125, F16)
+    assert torch.equal(got, attention.attend_rows(q, cache, ints(table), ints(lens), cu=ints(cu), longest=704))
+
+
 def test_attend_keeps_small_weights():
     """A token that stands out over 8,191 that weigh 2^-20 of it each: together 2^-7, which a float16 weight of 2^-20 would
     lose or move by up to 2^-5 of itself."""
@@ -434,6 +484,22 @@ def test_prompt_over_more_and_fewer_keys(dtype, width):
     got = attention.prompt_rows(q, k, v, ints(cu), cu_k=ints(cu_k), scale=0.2)
     check_prompt(got, q, k, v, cu, cu_k, 0.2, dtype)
     assert (got[cu[2]:cu[2] + 130] == 0).all() and (got[cu[3]:cu[4]] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("width", [64, 128, 256])
+@pytest.mark.parametrize("rows,keys", [([100], [3000]), ([130, 1, 200], [1300, 2200, 200]), ([5, 5], [0, 0])])
+def test_prompt_keys_in_chunks(dtype, width, rows, keys):
+    """Few rows over many keys: the keys go to several workgroups; no keys at all."""
+    from larder_amd import _lib, attention
+    rng = np.random.default_rng(sum(keys) + width)
+    cu, cu_k = cu_of(rows), cu_of(keys)
+    q, k, v = normal(rng, cu[-1] + 2, 4, width, dtype=dtype), *(normal(rng, cu_k[-1], 2, width, dtype=dtype) for _ in range(2))
+    split = _lib.lib().lmoe_prompt_attend_workspace_bytes(q.shape[0], k.shape[0], 4, 2, width, len(rows))
+    assert (split > 0) == (sum(keys) > 0)
+    got = attention.prompt_rows(q, k, v, ints(cu), cu_k=ints(cu_k))
+    check_prompt(got, q, k, v, cu, cu_k, width ** -0.5, dtype)
+    assert (got[cu[-1]:] == 0).all() and torch.equal(got, attention.prompt_rows(q, k, v, ints(cu), cu_k=ints(cu_k)))
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
@@ -542,6 +608,40 @@ def test_decode_step_in_a_graph():
         assert torch.equal(out, want), i
         for a, b in zip(eager, caught):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("width", [128, 256])
+def test_prompt_in_a_graph_and_on_streams(width):
+    """A prompt chunk (keys in chunks, their workspace in the graph's memory) replayed between eager calls, and two calls on two
+    streams at once."""
+    from larder_amd import attention
+    rng = np.random.default_rng(21)
+    q, k, v = normal(rng, 70, 4, width), normal(rng, 2000, 2, width), normal(rng, 2000, 2, width)
+    cu, cu_k = ints([0, 70]), ints([0, 2000])
+    cache = attention.KVCache.empty(40, 2, width)
+    table, lens = torch.arange(40, dtype=torch.int32, device="cuda")[None], ints([2000])
+    attention.append_rows(cache, None, k, v, table, lens, cu=cu_k)
+
+    def both():
+        return attention.prompt_rows(q, k, v, cu, cu_k=cu_k), attention.attend_rows(q[:3], cache, table, lens, cu=ints3)
+    ints3 = ints([0, 3])
+    both()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        caught = both()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for i in range(4):
+        q.copy_(normal(rng, 70, 4, width))
+        want = both()
+        g.replay()
+        torch.cuda.synchronize()
+        outs = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(both())
+        torch.cuda.synchronize()
+        for got in [caught] + outs:
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), i
 
 
 def test_trunk_attention_rows():
