@@ -177,11 +177,11 @@ def qcode(t):
 _CHECKED = {}
 
 
-def stream():
-    """The current torch stream as a hipStream_t, for a call that launches work. The first such call on a device
-    first runs the library's known-answer self-check there (and raises if it fails), unless LMOE_SELF_CHECK=0 or a
-    graph is being captured (then the next eager call checks)."""
-    dev = torch.cuda.current_device()
+def stream(dev=None):
+    """The current torch stream as a hipStream_t, for a call that launches work (dev: the current device, where the caller
+    knows it). The first such call on a device first runs the library's known-answer self-check there (and raises if it
+    fails), unless LMOE_SELF_CHECK=0 or a graph is being captured (then the next eager call checks)."""
+    dev = torch.cuda.current_device() if dev is None else dev
     if dev not in _CHECKED:
         _self_check(dev)
     return torch._C._cuda_getCurrentRawStream(dev)  # torch.cuda.current_stream() would build an object a call, 1.4 us

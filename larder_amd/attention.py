@@ -178,9 +178,9 @@ def _freq(fn, freq, width):
 def _launch(dev, name, *args):
     """call(name, *args, stream) with dev as the current device."""
     if dev == torch.cuda.current_device():
-        return call(name, *args, stream())
+        return call(name, *args, stream(dev))
     with torch.cuda.device(dev):
-        return call(name, *args, stream())
+        return call(name, *args, stream(dev))
 
 
 # the workspace of a call is a function of its sizes alone
@@ -210,7 +210,7 @@ def rope_rows(x, positions, freq, interleaved=False, gain=1.0, out=None):
         _refuse(fn, "positions is int32 or int64 [rows]")
     freq = _freq(fn, freq, width)
     if out is None:
-        out = torch.empty((t, heads, width), dtype=x.dtype, device=x.device)
+        out = x.new_empty((t, heads, width))
     elif out.shape != x.shape or out.dtype is not x.dtype or (width > 1 and out.stride(2) != 1):
         _refuse(fn, "out has x's shape and type and a dense last axis")
     dev = _device(fn, x, positions, freq, out)
@@ -252,9 +252,9 @@ def append_rows(cache, q, k, v, table, lens, cu=None, freq=None, interleaved=Fal
         q_out = q
         if pairs:
             q_heads, q_in = q.shape[1], q.data_ptr()
-            q_out = torch.empty((t, q_heads, width), dtype=dtype, device=q.device)
+            q_out = q.new_empty((t, q_heads, width))
     if keys:
-        k_out = torch.empty((t, heads, width), dtype=dtype, device=k.device)
+        k_out = k.new_empty((t, heads, width))
     if t and n:
         _launch(dev, "lmoe_kv_append", q_in, q_row, q_head, q_heads, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, dt,
                 t, heads, width, None if cu is None else cu.data_ptr(), lens.data_ptr(), n, table.data_ptr(), room, *codes, pages,
@@ -301,13 +301,13 @@ def attend_rows(q, cache, table, lens, cu=None, most_rows=None, longest=None, sc
         _refuse(fn, f"{q_heads} query heads over {heads} key heads")
     cu, lens, table, n, room = _sequences(fn, cu, lens, table, t)
     dev = _device(fn, q, table, lens, cu, *cache)
-    out = torch.empty((t, q_heads, width), dtype=dtype, device=q.device)
+    out = q.new_empty((t, q_heads, width))
     if not t or not n:
         return out.zero_()
     most = max(1, int(most_rows)) if most_rows is not None else 1 if cu is None else -(-t // n)
     long = room * page if longest is None else max(1, min(int(longest), room * page))
     need = _attend_workspace(t, q_heads, heads, width, n, most, long)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
     _launch(dev, "lmoe_kv_attend", q.data_ptr(), dcode(dtype), q_row, q_head, t, q_heads, heads, width,
             None if cu is None else cu.data_ptr(), lens.data_ptr(), n, table.data_ptr(), room, *codes, pages, page, most, long,
             width ** -0.5 if scale is None else scale, None if ws is None else ws.data_ptr(), need, out.data_ptr())
@@ -341,11 +341,11 @@ def prompt_rows(q, k, v, cu, cu_k=None, scale=None):
     elif u != t:
         _refuse(fn, f"{t} rows over {u} keys need their offsets cu_k")
     dev = _device(fn, q, k, v, cu, cu_k)
-    out = torch.empty((t, q_heads, width), dtype=dtype, device=q.device)
+    out = q.new_empty((t, q_heads, width))
     if not t or not n:
         return out.zero_()
     need = _prompt_workspace(t, u, q_heads, heads, width, n)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
     _launch(dev, "lmoe_prompt_attend", q.data_ptr(), q_row, q_head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
             dcode(dtype), t, u, q_heads, heads, width, cu.data_ptr(), (cu if cu_k is None else cu_k).data_ptr(), n,
             width ** -0.5 if scale is None else scale, None if ws is None else ws.data_ptr(), need, out.data_ptr())
