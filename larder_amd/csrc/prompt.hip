@@ -15,6 +15,12 @@
 // Weights are rounded to the inputs' type for the matrix cores (float16: times 2^11, so that those down to 2^-25 of a row's
 // largest keep all their bits), and what a row is divided by is the float32 sum of the rounded weights.
 //
+// The next tile's score products, this tile's exponentials and its output products are issued in one stream of slots, a
+// product and about eight vector instructions each: 32 cycles of either. Measured (32 heads over 4 of 128, bf16, 8,192 rows):
+// masks in every tile 714 us, full tiles without them 557, fragments read ahead and copies spread over the slots (a burst of
+// them stalls a wavefront for 900 cycles) 521-530, 1.05 PFLOP/s. What is left is LDS traffic: without half of the key reads
+// 457, without the copies 453, without exponentials 488.
+//
 // Values that a row must not see are multiplied by a weight of zero; where one is not finite in a tile that some row does
 // not see whole, it is taken out and given to the rows that do see it alone.
 #include "rows.h"

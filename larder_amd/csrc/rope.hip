@@ -8,11 +8,18 @@
 // 1e6. Sine and cosine of what is left are their Taylor series in float32 (remainders below 2e-9 at pi / 4), once a token and
 // pair for all heads, in LDS. Everything else is one float32 multiply or add after the other, and one rounding at the end.
 //
+// Bound by HBM: 8,192 rows of 32 heads of 128 in float16, neighbouring pairs: 23.5 us, 5.7 TB/s. Threads run over a row's
+// units, pairs and the channels that stay apart; with divisions for every unit and both kinds in one wavefront it took 29.3,
+// and 54 for what takes 32 where a quarter of 256 channels turns.
+//
 // The cache: e4m3 codes [page][head][token of the page][width] and one float32 scale for each page and head, of keys and of
 // values. The scale is the least power of two (2^-100 at least) that brings the largest finite magnitude of the page's head
 // to 448 or less. With a power of two, restating a page when a later token is larger moves exponents and rounds nothing but
 // codes that become subnormal, so a page filled token by token holds what one written at once would, up to those. e4m3 has
 // no infinity: infinities and NaN become NaN, and stay out of the scale.
+//
+// Measured: 64 sequences' tokens (32 + 8 heads of 128) 8.8 us, five dependent loads; 9,344 rows of prompts (16 + 4 heads of
+// 256) with their rotation 40 us, 4.3 TB/s; reading those pages back in 16 bits 11 us.
 #include "rows.h"
 
 namespace lmoe {
