@@ -481,7 +481,7 @@ struct PromptPlan {
 };
 static PromptPlan prompt_plan(int T, int U, int q_heads, int D, int B) {
   PromptPlan p = {1 << 30, 1, 0, 0};
-  const long long work = (long long)((T + kPromptRows - 1) / kPromptRows) * q_heads, full = D == 256 ? 256 : 512;
+  const long long work = (T / 128 + (long long)B) * q_heads, full = D == 256 ? 256 : 512;
   if (work <= 0 || 2 * work > full) return p;
   const int splits = int(full / work);
   long long chunk = ((long long)U / (B > 0 ? B : 1) + splits - 1) / splits;
@@ -535,7 +535,7 @@ extern "C" int lmoe_prompt_attend(const void *q, long long q_row, long long q_he
                   scale * 1.4426950408889634f, T, U, B, q_heads, heads, int(tiles), plan.chunk, plan.chunks};
   auto go = [&](auto kernel, auto join) -> int {
     const size_t lds = size_t(kPromptKeys) * D * 2 * 4;
-    if (const int rc = allow_lds(kernel, lds, fn)) return rc;
+    if (const int rc = allow_lds(kernel, lds + 4096, fn)) return rc;  // with what the kernel declares itself
     launch(kernel, dim3(unsigned(tiles * q_heads * plan.chunks)), dim3(256), lds, (hipStream_t)stream, a);
     LMOE_LAUNCHED(fn);
     if (part) {

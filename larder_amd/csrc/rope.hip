@@ -502,7 +502,7 @@ extern "C" int lmoe_kv_append(const void *q, long long q_row, long long q_head, 
   const size_t lds = size_t(max(cu ? page : 1, r.tokens)) * n_freq * sizeof(float2);
   const unsigned grid = unsigned(tasks + rotating);
   auto go = [&](auto kernel) -> int {
-    if (const int rc = allow_lds(kernel, lds, fn)) return rc;
+    if (const int rc = allow_lds(kernel, lds + 256, fn)) return rc;  // with what the kernel declares itself
     launch(kernel, dim3(grid), dim3(256), lds, st, a, r);
     LMOE_LAUNCHED(fn);
     return 0;

@@ -9,18 +9,21 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // The largest b < B with first(cu[b], b) <= t, by one wavefront (-1 if there is none); first never falls with b where cu
-// does not. 64 sequences a step. Whatever cu holds, the result is in [-1, B).
+// does not. A load for every factor of 64 in B. Whatever cu holds, the result is in [-1, B).
 template <typename F>
 __device__ __forceinline__ int last_at(const int *cu, int B, int t, F &&first) {
   const int lane = threadIdx.x & 63;
-  int n = 0;
-  for (int b0 = 0; b0 < B; b0 += 64) {
-    const int b = b0 + lane;
-    const unsigned long long le = __ballot(b < B && first(cu[b < B ? b : B - 1], b) <= (long long)t);
-    n += __popcll(le);
-    if (le != ~0ull) break;
+  int lo = 0, hi = B;  // how many b there are is in [lo, hi]
+  while (hi - lo > 64) {
+    const int step = (hi - lo + 63) >> 6, i = lo + (lane + 1) * step - 1;
+    lo += step * __popcll(__ballot(i < hi && first(cu[min(i, hi - 1)], i) <= (long long)t));
+    hi = min(lo + step, hi);
   }
-  return __builtin_amdgcn_readfirstlane(n - 1);
+  if (lo < hi) {
+    const int b = min(lo + lane, hi - 1);
+    lo += __popcll(__ballot(lo + lane < hi && first(cu[b], b) <= (long long)t));
+  }
+  return __builtin_amdgcn_readfirstlane(lo - 1);
 }
 
 // A sequence's rows [row0, row0 + n) of T packed ones: cu[b] .. cu[b + 1], or row b alone where cu is null. Offsets past

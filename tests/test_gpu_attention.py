@@ -174,6 +174,31 @@ def test_append(dtype, page, heads, width, pairs, interleaved):
             assert (tens.view(torch.uint8)[torch.from_numpy(rest).cuda()] == 0x7f).all()
 
 
+@pytest.mark.parametrize("n", [65, 130, 5000])
+def test_append_many_sequences(n):
+    """More sequences than a wavefront has lanes, and than its square; empty ones among them, one of many rows."""
+    from larder_amd import attention
+    rng = np.random.default_rng(23)
+    rows = [int(x) for x in rng.choice([0, 1, 1, 2], n)]
+    rows[n // 2] = 100
+    cu = cu_of(rows)
+    table, pages = page_table(rng, [-(-x // 32) for x in rows])
+    cache = poisoned(pages, 1, 64, 32)
+    want = cache_host(cache)
+    k, v = (normal(rng, cu[-1], 1, 64) for _ in range(2))
+    freq = frequencies(16)
+    q, _ = attention.append_rows(cache, k, k, v, ints(table), ints(rows), cu=ints(cu), freq=freq)
+    turned = ref.rope(host(k), np.concatenate([np.arange(m) for m in rows]), host(freq))
+    assert (np.abs(host(q) - turned) <= rope_bound(host(k), turned, freq, 1.0, BF16)).all()
+    ref.append(*want[0], turned, cu, rows, table)
+    ref.append(*want[1], host(v), cu, rows, table)
+    for (codes, scales), (gc, gs) in zip(want, cache_host(cache)):
+        assert np.array_equal(scales, gs, equal_nan=True) and close_codes(gc, codes, 1e-4)
+    back, held = attention.read_rows(cache, ints(table), ints(cu), cu[-1], dtype=F32)[0], cache_host(cache)[0]
+    want = np.concatenate([ref.read(*held, table[b], rows[b])[0] for b in range(n)])
+    assert np.array_equal(host(back), want)
+
+
 def test_append_token_by_token_and_idempotent():
     """A page filled by single tokens holds what one call writes (values within 2^8 of each other: no code becomes subnormal);
     the same call twice changes nothing."""
@@ -470,6 +495,21 @@ def test_prompt(dtype, q_heads, heads, width, lengths):
     check_prompt(got, q, k, v, cu, cu, width ** -0.5, dtype)
     assert (got[cu[-1]:] == 0).all()
     assert torch.equal(got, attention.prompt_rows(q.contiguous(), k.contiguous(), v.contiguous(), ints(cu)))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("width", [64, 128, 256])
+def test_prompt_many_sequences(dtype, width):
+    """More sequences than a wavefront has lanes, most of them a row or none."""
+    from larder_amd import attention
+    rng = np.random.default_rng(22)
+    lengths = [int(x) for x in rng.choice([0, 0, 1, 2, 9], 300)]
+    lengths[17], lengths[299] = 140, 0
+    cu = cu_of(lengths)
+    q, k, v = normal(rng, cu[-1] + 1, 2, width, dtype=dtype), *(normal(rng, cu[-1] + 1, 1, width, dtype=dtype) for _ in range(2))
+    got = attention.prompt_rows(q, k, v, ints(cu))
+    check_prompt(got, q, k, v, cu, cu, width ** -0.5, dtype)
+    assert (got[cu[-1]:] == 0).all()
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
