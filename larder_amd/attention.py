@@ -18,7 +18,8 @@ and v side by side; one whose layout no kernel reads is copied first.
 lens int32 [sequences] counts a sequence's tokens with the rows of the call among them: row r of n stands at place lens -
 n + r. table int32 [sequences, width] lists each sequence's pages in order; entries behind its last page are not read. A
 page outside the cache (or the table) holds nothing: no token is written there and none is seen. Sequences may share pages
-they only read; a page that a call writes to stands in one place of one table.
+they only read; a page that a call writes to stands in one place of one table. A row that sees no token, or only tokens that
+score -infinity, attends to nothing: it is zero.
 """
 import functools
 import math

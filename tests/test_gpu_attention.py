@@ -564,6 +564,39 @@ def test_prompt_values_not_finite(dtype, width):
     check_prompt(got[:100], q[:100], k[:100], v[:100], [0, 100], [0, 100], width ** -0.5, dtype)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("width,rows,keys", [(64, 130, 130), (128, 40, 2100), (256, 70, 70)])
+def test_prompt_scores_of_minus_infinity(dtype, width, rows, keys):
+    """Keys whose scores are -inf weigh nothing, in whole tiles and chunks and among others; a row with only such is zero."""
+    from larder_amd import attention
+    rng = np.random.default_rng(16)
+    q, k, v = (normal(rng, n, 1, width, dtype=dtype) for n in (rows, keys, keys))
+    q[:, 0, 0] = q[:, 0, 0].abs() + 1
+    k[:keys - rows + 20, 0, 0] = float("-inf")
+    k[keys - 10, 0, 0] = float("-inf")
+    got = attention.prompt_rows(q, k, v, ints([0, rows]), cu_k=ints([0, keys]))
+    assert (got[:20] == 0).all() and (got[20:] != 0).any(-1).all()
+    check_prompt(got, q, k, v, [0, rows], [0, keys], width ** -0.5, dtype)
+
+
+def test_attend_scores_of_minus_infinity():
+    """A query that scores -inf against every token (or all but those of one page) among others that do not."""
+    from larder_amd import attention
+    rng = np.random.default_rng(17)
+    cache = random_cache(rng, 30, 1, 64, 64)
+    codes = cache.k.view(torch.uint8)
+    codes[:, :, :, 0] = 0x38   # 1.0
+    codes[29, :, :, 0] = 0xb8  # -1.0: +inf against the second query, which is NaN
+    table, lens = np.arange(30, dtype=np.int32)[None].repeat(3, 0), np.array([29 * 64, 30 * 64, 29 * 64 - 5], np.int32)
+    q = normal(rng, 3, 2, 64, dtype=F16)
+    q[:2, 0, 0] = float("-inf")
+    for longest in (None, 1):
+        got = attention.attend_rows(q, cache, ints(table), ints(lens), longest=longest)
+        assert (got[0, 0] == 0).all() and torch.isnan(got[1, 0]).all() and torch.isfinite(got[2]).all()
+        check_attend(got[2:], q[2:], cache, table[2:], lens[2:], [0, 1], 64 ** -0.5, F16)
+        check_attend(got[:1, 1:], q[:1, 1:], cache, table, lens[:1], [0, 1], 64 ** -0.5, F16)
+
+
 def test_large_scores():
     """Scores in the thousands, one key far above the rest, and equal scores: no overflow, the weights of a softmax."""
     from larder_amd import attention
