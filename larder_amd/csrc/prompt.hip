@@ -151,14 +151,18 @@ constexpr bool weights_in_time(int NM, int NV, int NP, int DT, int NS) {
 // which see the most keys, so that what is left for the end is short (16 prompts of up to 4,000 rows at width 64: 160 -> 134
 // us, of up to 900 at 128: 37 -> 30; long prompts lose up to 5 % by sharing less of L2: 12 of up to 3,500 rows 332 -> 345).
 // More: the sequences from the last on, each from its end; sequence b's tiles begin at cu[b] / rows + b, which leaves it room
-// for all of them. b < 0: there is none. The first and the last sequence have a tile even without rows.
+// for all of them, and for one that is empty where its rows fill their tiles. Eight tiles in turn are shifted against the next
+// eight: workgroups go to the four quarters of an XCD in turn, and 72 sequences of 128 rows, every second workgroup empty, left
+// half of the CUs idle (16 heads of 256: 118 -> 81 us). b < 0: there is none. The first and the last sequence have a tile even
+// without rows.
 struct PromptTile {
   int b, tile, row0, nq, key0, nk;
 };
 __device__ __forceinline__ PromptTile nth_tile(const PromptArgs &a, int nth) {
   PromptTile w = {-1, 0, 0, 0, 0, 0};
   if (a.B > 64) {
-    const int task = a.tiles - 1 - nth;
+    const int turned = nth < (a.tiles & ~7) ? (nth & ~7) | ((nth + (nth >> 3)) & 7) : nth;
+    const int task = a.tiles - 1 - turned;
     w.b = last_at(a.cu, a.B, task, [](int c, int i) { return (long long)(c / kPromptRows) + i; });
     if (w.b < 0) return w;
     seq_rows(a.cu, w.b, a.T, &w.row0, &w.nq);
