@@ -437,14 +437,22 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_prompt(PromptArgs a) 
   if (a.part) {
     if (there && chunk == 0 && h == 0) a.joins[line] = parts > 1 ? parts : 0;
     if (parts > 1) {
-      if (!there) return;
-      float *part = a.part + (size_t(chunk) * a.T * a.q_heads + line) * (D + 4);
+      float *rows = reinterpret_cast<float *>(lds) + wave * 32 * D;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          *reinterpret_cast<f32x4 *>(part + 32 * d + 8 * e + 4 * h) = f32x4{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
-      if (h == 0) *reinterpret_cast<float2 *>(part + D) = float2{m, l};
+          *reinterpret_cast<f32x4 *>(rows + r * D + ((8 * d + 2 * e + h) ^ (r & 15)) * 4) =
+              f32x4{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      float *part = a.part + (size_t(chunk) * a.T + row0 + first + 32 * wave) * a.q_heads * (D + 4) + size_t(head) * (D + 4);
+#pragma unroll
+      for (int i = 0; i < 32 * D / 256; ++i) {
+        const int j = i * 64 + lane, row = j / (D / 4), c = j % (D / 4);
+        const f32x4 w = *reinterpret_cast<const f32x4 *>(rows + row * D + (c ^ (row & 15)) * 4);
+        if (first + 32 * wave + row < nq) *reinterpret_cast<f32x4 *>(part + size_t(row) * a.q_heads * (D + 4) + c * 4) = w;
+      }
+      if (there && h == 0) *reinterpret_cast<float2 *>(part + size_t(r) * a.q_heads * (D + 4) + D) = float2{m, l};
       return;
     }
   }
