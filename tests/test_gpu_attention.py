@@ -512,6 +512,30 @@ def test_prompt_many_sequences(dtype, width):
     assert (got[cu[-1]:] == 0).all()
 
 
+@pytest.mark.parametrize("lengths", [[128] * 70, [127, 129] * 33, [1] * 64 + [300, 256, 384]])
+def test_prompt_many_full_tiles(lengths):
+    """More sequences than a wavefront has lanes, whose rows fill their tiles or just do not: every tile is worked once."""
+    from larder_amd import attention
+    rng = np.random.default_rng(len(lengths))
+    cu = cu_of(lengths)
+    q, k, v = normal(rng, cu[-1], 2, 64, dtype=F16), *(normal(rng, cu[-1], 1, 64, dtype=F16) for _ in range(2))
+    check_prompt(attention.prompt_rows(q, k, v, ints(cu)), q, k, v, cu, cu, 64 ** -0.5, F16)
+
+
+@pytest.mark.parametrize("width", [64, 128, 256])
+def test_prompt_rows_far_apart(width):
+    """Query rows whose strides pass 2^31 bytes together, and a page-long gap between keys."""
+    from larder_amd import attention
+    rng = np.random.default_rng(width + 1)
+    wide = torch.zeros(40, 2 ** 24 + 8, dtype=F16, device="cuda")
+    q = wide[:, :2 * width].view(40, 2, width)
+    q.copy_(normal(rng, 40, 2, width, dtype=F16))
+    k, v = (normal(rng, 40, 40, width, dtype=F16)[:, 7:8] for _ in range(2))
+    got = attention.prompt_rows(q, k, v, ints([0, 40]))
+    assert torch.equal(got, attention.prompt_rows(q.contiguous(), k.contiguous(), v.contiguous(), ints([0, 40])))
+    check_prompt(got, q, k, v, [0, 40], [0, 40], width ** -0.5, F16)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("width", [64, 128, 256])
 def test_prompt_over_more_and_fewer_keys(dtype, width):
