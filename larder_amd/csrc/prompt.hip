@@ -18,8 +18,8 @@
 // The next tile's score products, this tile's exponentials and its output products are issued in one stream of slots, a
 // product and about eight vector instructions each: 32 cycles of either. Measured (32 heads over 4 of 128, bf16, 8,192 rows):
 // masks in every tile 714 us, full tiles without them 557, fragments read ahead and copies spread over the slots (a burst of
-// them stalls a wavefront for 900 cycles) 521-530, 1.05 PFLOP/s. What is left is LDS traffic: without half of the key reads
-// 457, without the copies 453, without exponentials 488.
+// them stalls a wavefront for 900 cycles) 521-530, q and output in whole rows 503-532, 1.03-1.09 PFLOP/s. What is left is LDS
+// traffic: of 521, without half of the key reads 457, without the copies 453, without exponentials 488.
 //
 // Values that a row must not see are multiplied by a weight of zero; where one is not finite in a tile that some row does
 // not see whole, it is taken out and given to the rows that do see it alone.
