@@ -126,12 +126,13 @@ def _rows(fn, name, x, heads=None, width=None, rows=None):
     if (heads is not None and h != heads) or (width is not None and w != width) or (rows is not None and r != rows):
         _refuse(fn, f"{name} is [{r}, {h}, {w}]")
     s0, s1, s2 = x.stride()
+    s0, s1 = s0 if r > 1 else h * w, s1 if h > 1 else w  # one row's or one head's own stride leads nowhere, and may be anything
     mask = 3 if x.element_size() == 4 else 7
     if s2 != 1 or s0 & mask or s1 & mask or x.data_ptr() & 15:
         x = x.contiguous()
         if x.data_ptr() & 15:
             x = x.clone()
-        s0, s1, s2 = x.stride()
+        s0, s1 = h * w, w
     return x, s0, s1
 
 

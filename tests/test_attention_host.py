@@ -46,6 +46,22 @@ def test_tensors_off_the_gpu_are_refused():
             call()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_rows_of_any_layout_have_strides_the_kernels_read(dtype):
+    """Aligned strides, and the same values through them: also where an axis of size one has a stride of its own, which torch
+    calls contiguous whatever it is."""
+    step = 16 // torch.zeros((), dtype=dtype).element_size()
+    wide = torch.arange(9 * 1027, dtype=torch.float32).remainder(97).to(dtype).view(9, 1027)
+    cols = torch.arange(9 * 3 * 129, dtype=torch.float32).remainder(89).to(dtype).view(9, 3, 129)
+    rows = wide[:, :512].view(9, 4, 128)
+    for x in (rows, rows[0:1], rows[3:4], rows[2:2], cols[:, 1:2, :128], cols[4:5, 2:3, 1:], cols[:, :, :128], rows[:, :, 1:65],
+              rows[3:4, :1, ::2], wide[:, :1024].view(9, 8, 128), wide[:, :1024].view(9, 8, 128).transpose(0, 1), rows[:1].expand(5, 4, 128)):
+        y, s0, s1 = attention._rows("f", "x", x)
+        assert y.shape == x.shape and s0 % step == 0 and s1 % step == 0 and y.data_ptr() % 16 == 0
+        if x.numel():
+            assert torch.equal(torch.as_strided(y, y.shape, (s0, s1, 1), y.storage_offset()), x)
+
+
 P = ctypes.c_void_p(16)  # never dereferenced: every call below is refused while its arguments are checked
 ODD = ctypes.c_void_p(24)
 

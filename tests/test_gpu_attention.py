@@ -814,3 +814,27 @@ def test_refusals():
         attention.append_rows(cache, q, k, k, table, lens, freq=frequencies(10))
     odd = torch.zeros(2 * 512 + 1, dtype=F16, device="cuda")[1:].view(2, 4, 128)  # rows at odd addresses are copied, not refused
     assert torch.equal(attention.attend_rows(odd, cache, table, lens), attention.attend_rows(q, cache, table, lens))
+
+
+@pytest.mark.parametrize("width,page", [(64, 32), (128, 64), (256, 64)])
+def test_one_row_or_head_with_a_stride_of_its_own(width, page):
+    """A single row out of a padded product, and a single head with an odd head stride: appended, attended and run as a prompt as
+    their dense copies are."""
+    from larder_amd import attention
+    rng = np.random.default_rng(width)
+    padded = normal(rng, 9, 4 * width + 3)
+    row = padded[3:4, :4 * width].view(1, 4, width)                    # row stride 4 width + 3
+    head = normal(rng, 5, 3, width + 1)[2:3, 1:2, 1:]                  # head stride width + 1, an odd address
+    q, k, v = row[:, :2], row[:, 2:3], head
+    assert q.stride(0) % 8 and k.stride(0) % 8 and v.stride(1) % 8
+    table, lens, freq = ints([[1]]), ints([1]), frequencies(16)
+    outs = []
+    for a, b, c in ((q, k, v), (q.clone(memory_format=torch.contiguous_format).reshape(-1).view(1, 2, width),
+                                k.reshape(-1).view(1, 1, width).clone(), v.reshape(-1).view(1, 1, width).clone())):
+        cache = poisoned(2, 1, width, page)
+        turned, keys = attention.append_rows(cache, a, b, c, table, lens, freq=freq, keys=True)
+        outs.append([turned, keys, *(t.view(torch.uint8) for t in cache), attention.attend_rows(a, cache, table, lens),
+                     attention.prompt_rows(a, b, c, ints([0, 1]))])
+    for x, y in zip(*outs):
+        assert torch.equal(x, y)
+    check_prompt(outs[0][-1], q, k, v, [0, 1], [0, 1], width ** -0.5, BF16)
