@@ -117,9 +117,12 @@ def _device(fn, first, *others):
     return dev
 
 
-def _rows(fn, name, x, heads=None, width=None, rows=None):
+_KEYS_APART = 1 << 23  # elements: lmoe_prompt_attend's rows of keys and values are less than that apart
+
+
+def _rows(fn, name, x, heads=None, width=None, rows=None, apart=1 << 62):
     """(x, row stride, head stride): a [rows, heads, width] tensor the kernels can read (its last axis dense, 16-byte aligned
-    rows and heads), copied if it is not."""
+    rows and heads, rows less than `apart` elements apart), copied if it is not."""
     if x.dim() != 3:
         _refuse(fn, f"{name} is [rows, heads, width], not {tuple(x.shape)}")
     r, h, w = x.shape
@@ -128,7 +131,7 @@ def _rows(fn, name, x, heads=None, width=None, rows=None):
     s0, s1, s2 = x.stride()
     s0, s1 = s0 if r > 1 else h * w, s1 if h > 1 else w  # one row's or one head's own stride leads nowhere, and may be anything
     mask = 3 if x.element_size() == 4 else 7
-    if s2 != 1 or s0 & mask or s1 & mask or x.data_ptr() & 15:
+    if s2 != 1 or s0 >= apart or s0 & mask or s1 & mask or x.data_ptr() & 15:
         x = x.contiguous()
         if x.data_ptr() & 15:
             x = x.clone()
@@ -324,9 +327,9 @@ def prompt_rows(q, k, v, cu, cu_k=None, scale=None):
     fn = "prompt_rows"
     q, q_row, q_head = _rows(fn, "q", q)
     t, q_heads, width = q.shape
-    k, k_row, k_head = _rows(fn, "k", k, None, width)
+    k, k_row, k_head = _rows(fn, "k", k, None, width, apart=_KEYS_APART)
     u, heads, _ = k.shape
-    v, v_row, v_head = _rows(fn, "v", v, heads, width, u)
+    v, v_row, v_head = _rows(fn, "v", v, heads, width, u, _KEYS_APART)
     dtype = q.dtype
     if dtype not in _HALVES or k.dtype is not dtype or v.dtype is not dtype:
         _refuse(fn, "q, k and v are all float16 or all bfloat16")

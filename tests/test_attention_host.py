@@ -62,6 +62,17 @@ def test_rows_of_any_layout_have_strides_the_kernels_read(dtype):
             assert torch.equal(torch.as_strided(y, y.shape, (s0, s1, 1), y.storage_offset()), x)
 
 
+def test_keys_too_far_apart_for_the_prompt_kernel_are_copied():
+    apart = attention._KEYS_APART
+    wide = torch.zeros(3, apart, dtype=torch.float16)
+    for n, copied in ((apart, True), (apart - 8, False)):
+        x = wide.view(-1)[:3 * n].view(3, n)[:, 64:192].view(3, 2, 64)
+        x.copy_(torch.arange(3 * 128).view(3, 2, 64))
+        y, s0, s1 = attention._rows("f", "k", x, apart=apart)
+        assert (s0, s1) == ((128, 64) if copied else (n, 64)) and torch.equal(y, x)
+        assert attention._rows("f", "k", x[1:2], apart=apart)[1:] == (128, 64)
+
+
 P = ctypes.c_void_p(16)  # never dereferenced: every call below is refused while its arguments are checked
 ODD = ctypes.c_void_p(24)
 

@@ -838,3 +838,15 @@ def test_one_row_or_head_with_a_stride_of_its_own(width, page):
     for x, y in zip(*outs):
         assert torch.equal(x, y)
     check_prompt(outs[0][-1], q, k, v, [0, 1], [0, 1], width ** -0.5, BF16)
+
+
+def test_prompt_keys_far_apart():
+    """Keys and values of rows 2^23 elements and more apart, and one key of such rows."""
+    from larder_amd import attention
+    rng = np.random.default_rng(31)
+    wide = torch.zeros(5, (1 << 23) + 8, dtype=F16, device="cuda")
+    wide[:, :512] = normal(rng, 5, 512, dtype=F16)
+    q, k, v = normal(rng, 5, 4, 128, dtype=F16), wide[:, :256].view(5, 2, 128), wide[:, 256:512].view(5, 2, 128)
+    for n in (5, 1):
+        got = attention.prompt_rows(q[:n], k[:n], v[:n], ints([0, n]))
+        check_prompt(got, q[:n], k[:n], v[:n], [0, n], [0, n], 128 ** -0.5, F16)
