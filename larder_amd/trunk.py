@@ -75,22 +75,29 @@ def attention_rows(x, qkv, out, cache, table, lens, cu=None, freq=None, interlea
                                [sequences + 1] where each begins (read_rows, prompt_rows)
     """
     heads, width = cache.k.shape[1], cache.k.shape[3]
+    # what a later call would refuse is refused here, before the cache is written
+    if prompt is not None and cu is None:
+        raise ValueError("attention_rows: a prompt's rows need their offsets cu")
+    whole = prompt is True
+    cu_k = total = None
+    if prompt is not None and not whole:
+        cu_k, total = prompt
+        cu_k = attention._ints("attention_rows", "cu_k", cu_k, table.shape[0] + 1)
+        if cu_k.device != x.device or total < 0:
+            raise ValueError("attention_rows: cu_k lives where x does, and total is no less than zero")
     y = qmv_rows(x, *qkv)
     t, q_heads = y.shape[0], y.shape[1] // width - 2 * heads
-    if q_heads <= 0 or y.shape[1] % width:
+    if q_heads <= 0 or y.shape[1] % width or heads == 0 or q_heads % heads:
         raise ValueError(f"attention_rows: {y.shape[1]} outputs are not query heads and {heads} key and value heads of {width}")
+    w, scales, biases, group_size = out
+    if not qmv_fits(y[:, :q_heads * width], w, scales, group_size, 4, "affine", biases):
+        raise ValueError(f"attention_rows: out is a 4-bit affine weight of {q_heads} heads of {width}")
     q, k, v = y.view(t, -1, width).split([q_heads, heads, heads], 1)
-    whole = prompt is True
-    if whole and cu is None:
-        raise ValueError("attention_rows: a prompt's rows need their offsets cu")
     q, k = attention.append_rows(cache, q, k, v, table, lens, cu=cu, freq=freq, interleaved=interleaved, gain=gain, keys=whole)
     if prompt is None:
         o = attention.attend_rows(q, cache, table, lens, cu=cu, most_rows=most_rows, longest=longest)
     elif whole:
         o = attention.prompt_rows(q, k, v, cu)
     else:
-        if cu is None:
-            raise ValueError("attention_rows: a prompt's rows need their offsets cu")
-        cu_k, total = prompt
         o = attention.prompt_rows(q, *attention.read_rows(cache, table, cu_k, total, dtype=x.dtype), cu, cu_k=cu_k)
     return qmv_rows(o.reshape(t, q_heads * width), *out)

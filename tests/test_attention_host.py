@@ -73,6 +73,31 @@ def test_keys_too_far_apart_for_the_prompt_kernel_are_copied():
         assert attention._rows("f", "k", x[1:2], apart=apart)[1:] == (128, 64)
 
 
+def affine(n, k):
+    return torch.zeros(n, k // 8, dtype=torch.int32), *(torch.zeros(n, k // 64, dtype=torch.bfloat16) for _ in range(2)), 64
+
+
+CU = torch.tensor([0, 2], dtype=torch.int32)
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(prompt=True), "offsets"), (dict(prompt=(CU, 2)), "offsets"), (dict(prompt=(CU.long(), 2), cu=CU), "cu_k"),
+    (dict(prompt=(CU[:1], 2), cu=CU), "cu_k"), (dict(prompt=(CU, -1), cu=CU), "total"), (dict(qkv=affine(7 * 64, 128)), "heads"),
+    (dict(qkv=affine(4 * 64, 128)), "heads"), (dict(qkv=affine(8 * 64 + 8, 128)), "heads"), (dict(out=affine(128, 3 * 64)), "out"),
+    (dict(out=affine(128, 4 * 64)[:2] + (None, 64)), "out")])
+def test_the_trunks_attention_refuses_before_it_writes(monkeypatch, kw, why):
+    """attention_rows on two key heads of 64: what one of its steps would refuse is refused before the cache is written."""
+    from larder_amd import trunk
+    written = []
+    monkeypatch.setattr(trunk, "qmv_rows", lambda x, w, *_: torch.zeros(x.shape[0], w.shape[0], dtype=torch.bfloat16))
+    monkeypatch.setattr(attention, "append_rows", lambda *a, **_: written.append(a) or (a[1], a[2]))
+    args = dict(qkv=affine(8 * 64, 128), out=affine(128, 4 * 64), cache=attention.KVCache.empty(1, 2, 64, device="cpu"),
+                table=torch.zeros(1, 1, dtype=torch.int32), lens=torch.tensor([2], dtype=torch.int32))
+    with pytest.raises(ValueError, match=why):
+        trunk.attention_rows(torch.zeros(2, 128, dtype=torch.bfloat16), **{**args, **kw})
+    assert not written
+
+
 P = ctypes.c_void_p(16)  # never dereferenced: every call below is refused while its arguments are checked
 ODD = ctypes.c_void_p(24)
 

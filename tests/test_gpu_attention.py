@@ -850,3 +850,25 @@ def test_prompt_keys_far_apart():
     for n in (5, 1):
         got = attention.prompt_rows(q[:n], k[:n], v[:n], ints([0, n]))
         check_prompt(got, q[:n], k[:n], v[:n], [0, n], [0, n], 128 ** -0.5, F16)
+
+
+def affine4(rng, n, k, group=64):
+    """A 4-bit affine weight [n, k] for trunk.qmv_rows."""
+    from oracle import qmv
+    wq, s, b = qmv.quantize_affine4((rng.standard_normal((n, k)) * 0.05).astype(np.float32), group)
+    return torch.from_numpy(wq.view(np.int32)).cuda(), *(torch.from_numpy(np.ascontiguousarray(a)).cuda().bfloat16() for a in (s, b)), group
+
+
+def test_trunk_attention_refuses_before_it_writes():
+    """Refused calls of attention_rows leave the cache as it was."""
+    from larder_amd import trunk
+    rng = np.random.default_rng(32)
+    cache = random_cache(rng, 2, 2, 64, 32)
+    before = [t.clone() for t in cache]
+    x, qkv, out = normal(rng, 1, 128), affine4(rng, 8 * 64, 128), affine4(rng, 128, 4 * 64)
+    table, lens, cu = ints([[0]]), ints([1]), ints([0, 1])
+    for kw, why in ((dict(prompt=(cu, 1)), "offsets"), (dict(prompt=(cu.cpu(), 1), cu=cu), "lives"),
+                    (dict(qkv=affine4(rng, 7 * 64, 128)), "heads"), (dict(out=affine4(rng, 128, 3 * 64)), "out")):
+        with pytest.raises(ValueError, match=why):
+            trunk.attention_rows(x, **{**dict(qkv=qkv, out=out, cache=cache, table=table, lens=lens), **kw})
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache, before))
