@@ -92,7 +92,7 @@ def attention_rows(x, qkv, out, cache, table, lens, cu=None, freq=None, interlea
     w, scales, biases, group_size = out
     if not qmv_fits(y[:, :q_heads * width], w, scales, group_size, 4, "affine", biases):
         raise ValueError(f"attention_rows: out is a 4-bit affine weight of {q_heads} heads of {width}")
-    q, k, v = y.view(t, -1, width).split([q_heads, heads, heads], 1)
+    q, k, v = y.view(t, y.shape[1] // width, width).split([q_heads, heads, heads], 1)
     q, k = attention.append_rows(cache, q, k, v, table, lens, cu=cu, freq=freq, interleaved=interleaved, gain=gain, keys=whole)
     if prompt is None:
         o = attention.attend_rows(q, cache, table, lens, cu=cu, most_rows=most_rows, longest=longest)

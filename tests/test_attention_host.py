@@ -98,6 +98,21 @@ def test_the_trunks_attention_refuses_before_it_writes(monkeypatch, kw, why):
     assert not written
 
 
+@pytest.mark.parametrize("prompt", [None, True, "later"])
+def test_the_trunks_attention_of_no_rows(monkeypatch, prompt):
+    from larder_amd import trunk
+    monkeypatch.setattr(trunk, "qmv_rows", lambda x, w, *_: torch.zeros(x.shape[0], w.shape[0], dtype=torch.bfloat16))
+    monkeypatch.setattr(attention, "append_rows", lambda c, q, k, v, *a, **_: (q, k))
+    monkeypatch.setattr(attention, "read_rows", lambda c, t, cu, n, **_: [torch.zeros(n, 2, 64, dtype=torch.bfloat16)] * 2)
+    for f in ("attend_rows", "prompt_rows"):
+        monkeypatch.setattr(attention, f, lambda q, *a, **_: q)
+    cu = torch.zeros(2, dtype=torch.int32)
+    got = trunk.attention_rows(torch.zeros(0, 128, dtype=torch.bfloat16), affine(8 * 64, 128), affine(128, 4 * 64),
+                               attention.KVCache.empty(1, 2, 64, device="cpu"), cu[:1, None], cu[:1], cu=cu,
+                               prompt=(cu, 0) if prompt == "later" else prompt)
+    assert got.shape == (0, 128)
+
+
 P = ctypes.c_void_p(16)  # never dereferenced: every call below is refused while its arguments are checked
 ODD = ctypes.c_void_p(24)
 

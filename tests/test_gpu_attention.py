@@ -872,3 +872,16 @@ def test_trunk_attention_refuses_before_it_writes():
         with pytest.raises(ValueError, match=why):
             trunk.attention_rows(x, **{**dict(qkv=qkv, out=out, cache=cache, table=table, lens=lens), **kw})
         assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache, before))
+
+
+def test_trunk_attention_of_no_rows():
+    """A call without rows gives none back, and changes no page."""
+    from larder_amd import trunk
+    rng = np.random.default_rng(33)
+    cache = random_cache(rng, 2, 2, 64, 32)
+    before = [t.clone() for t in cache]
+    qkv, out, cu = affine4(rng, 8 * 64, 128), affine4(rng, 128, 4 * 64), ints([0, 0])
+    for prompt in (None, True, (ints([0, 5]), 5)):
+        got = trunk.attention_rows(normal(rng, 0, 128), qkv, out, cache, ints([[1]]), ints([5]), cu=cu, prompt=prompt)
+        assert got.shape == (0, 128) and got.dtype == BF16
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache, before))
