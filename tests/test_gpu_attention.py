@@ -823,7 +823,7 @@ def test_one_row_or_head_with_a_stride_of_its_own(width, page):
     from larder_amd import attention
     rng = np.random.default_rng(width)
     padded = normal(rng, 9, 4 * width + 3)
-    row = padded[3:4, :4 * width].view(1, 4, width)                    # row stride 4 width + 3
+    row = padded[:, :4 * width].view(9, 4, width)[3:4]                 # row stride 4 width + 3
     head = normal(rng, 5, 3, width + 1)[2:3, 1:2, 1:]                  # head stride width + 1, an odd address
     q, k, v = row[:, :2], row[:, 2:3], head
     assert q.stride(0) % 8 and k.stride(0) % 8 and v.stride(1) % 8
