@@ -232,9 +232,9 @@ def rope_rows(x, positions, freq, interleaved=False, gain=1.0, out=None):
 
 def append_rows(cache, q, k, v, table, lens, cu=None, freq=None, interleaved=False, gain=1.0, keys=False):
     """Writes the rows k, v [T, heads, width] of each sequence into its pages, k rotated by the rows' places as rope_rows does
-    (freq None: as it is), and returns (q, k): q [T, query heads, width] rotated likewise (None for None), and with keys=True
-    the rotated k in its own type, as prompt_rows reads it (else None). float16, bfloat16 or float32. len(freq) is a multiple
-    of 8 (of 4 where interleaved). The cache's tensors are written in place."""
+    (freq None: as it is), and returns (q, k), tensors of their own: q [T, query heads, width] rotated likewise (None for None),
+    and with keys=True the rotated k in its own type, as prompt_rows reads it (else None). float16, bfloat16 or float32. len(freq)
+    is a multiple of 8 (of 4 where interleaved). The cache's tensors are written in place."""
     fn = "append_rows"
     pages, heads, page, width, *codes = _cache(fn, cache)
     k, k_row, k_head = _rows(fn, "k", k, heads, width)
@@ -254,10 +254,8 @@ def append_rows(cache, q, k, v, table, lens, cu=None, freq=None, interleaved=Fal
     q_heads = q_row = q_head = 0
     if q is not None:
         q, q_row, q_head = _rows(fn, "q", q, None, width, t)
-        q_out = q
-        if pairs:
-            q_heads, q_in = q.shape[1], q.data_ptr()
-            q_out = q.new_empty((t, q_heads, width))
+        q_heads, q_in = q.shape[1], q.data_ptr()
+        q_out = q.new_empty((t, q_heads, width))
     if keys:
         k_out = k.new_empty((t, heads, width))
     if t and n:
@@ -266,7 +264,7 @@ def append_rows(cache, q, k, v, table, lens, cu=None, freq=None, interleaved=Fal
                 page, None if freq is None else freq.data_ptr(), pairs, bool(interleaved), gain,
                 None if q_in is None else q_out.data_ptr(), None if k_out is None else k_out.data_ptr())
     elif t:
-        q_out = q_out if q_in is None else q_out.zero_()
+        q_out = q_out if q is None else q_out.zero_()
         k_out = k_out if k_out is None else k_out.zero_()
     return q_out, k_out
 

@@ -885,3 +885,37 @@ def test_trunk_attention_of_no_rows():
         got = trunk.attention_rows(normal(rng, 0, 128), qkv, out, cache, ints([[1]]), ints([5]), cu=cu, prompt=prompt)
         assert got.shape == (0, 128) and got.dtype == BF16
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache, before))
+
+
+@pytest.mark.parametrize("rotated", [False, True])
+@pytest.mark.parametrize("rows", [[3, 0, 2], [1200, 40, 1], [0, 0, 0]])
+def test_append_rows_of_no_sequence_come_back_zero(rows, rotated):
+    """Rows before the first sequence and behind the last one, with a rotation and without, and a call of no sequences."""
+    from larder_amd import attention
+    rng = np.random.default_rng(34)
+    cu = [2 + int(x) for x in cu_of(rows)]
+    t = cu[-1] + 3
+    x = normal(rng, t, 4, 64)
+    q, k, v = x.split([2, 1, 1], 1)
+    table, n = page_table(rng, [-(-m // 32) for m in rows])
+    freq = frequencies(16) if rotated else None
+    got = attention.append_rows(poisoned(n, 1, 64, 32), q, k, v, ints(table), ints(rows), cu=ints(cu), freq=freq, keys=True)
+    pos = np.concatenate([np.zeros(2, int)] + [np.arange(m) for m in rows] + [np.zeros(3, int)])
+    for a, b in zip((q, k), got):
+        assert (b[:2] == 0).all() and (b[cu[-1]:] == 0).all()
+        w = ref.rope(host(a), pos, host(freq) if rotated else [])
+        assert (np.abs(host(b) - w) <= rope_bound(host(a), w, freq, 1.0, BF16))[2:cu[-1]].all()
+        assert rotated or torch.equal(b[2:cu[-1]], a[2:cu[-1]])
+    none = attention.append_rows(poisoned(n, 1, 64, 32), q, k, v, ints(table)[:0], ints(rows)[:0], cu=ints([2]), freq=freq, keys=True)
+    assert all((a == 0).all() for a in none) and (x != 0).any()
+
+
+def test_append_gives_tensors_of_its_own():
+    """Writing to what append_rows returned does not reach the caller's q and k, with a rotation or without."""
+    from larder_amd import attention
+    x = torch.ones(1, 4, 64, dtype=F16, device="cuda")
+    for freq in (None, frequencies(0), frequencies(8)):
+        cache = attention.KVCache.empty(1, 1, 64)
+        q, k = attention.append_rows(cache, x[:, :2], x[:, 2:3], x[:, 3:], ints([[0]]), ints([1]), freq=freq, keys=True)
+        q.zero_(), k.zero_()
+        assert (x == 1).all()
