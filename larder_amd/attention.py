@@ -85,7 +85,8 @@ def rotary_freq(width, base=10000.0, kind="default", factor=1.0, original=None, 
 
         def pair_of(turns):  # the pair (a real number) that turns so many times in `original` positions
             return width * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
-        low, high = max(math.floor(pair_of(beta[0])), 0), min(math.ceil(pair_of(beta[1])), width // 2 - 1)
+        # the ramp may end past the last pair, which is then interpolated in part, as the published one does
+        low, high = max(math.floor(pair_of(beta[0])), 0), min(math.ceil(pair_of(beta[1])), width - 1)
         keep = 1.0 - ((torch.arange(width // 2, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0, 1)
         freq = freq * keep + freq / factor * (1.0 - keep)
         gain = 0.1 * math.log(factor) + 1.0

@@ -27,6 +27,19 @@ def test_rotary_freq():
     assert torch.allclose(attention.rotary_freq(128, 10000.0, "yarn", 1.0, 4096, device="cpu")[0], f, rtol=2.0 ** -51, atol=0)
 
 
+@pytest.mark.parametrize("width,original,low,high", [(128, 131072, 45, 70), (128, 65536, 40, 65), (128, 4096, 20, 46),
+                                                     (64, 10 ** 7, 37, 50), (64, 10 ** 9, 53, 63), (32, 10 ** 9, 26, 31)])
+def test_yarn_ramps_end_where_the_published_ones_do(width, original, low, high):
+    """Base 10,000: the pair that turns n times in `original` positions is width ln(original / (2 pi n)) / (2 ln 10,000), 32
+    turns of it rounded down and one turn rounded up, within [0, width - 1]: also where that lies past the last pair."""
+    turns = [width * math.log(original / (2 * math.pi * n)) / (2 * math.log(10000)) for n in (32, 1)]
+    assert (max(math.floor(turns[0]), 0), min(math.ceil(turns[1]), width - 1)) == (low, high)
+    got, _ = attention.rotary_freq(width, 10000.0, "yarn", 8.0, original, device="cpu")
+    for i, f in enumerate(got.tolist()):
+        keep = 1 - min(max((i - low) / (high - low), 0), 1)
+        assert math.isclose(f, 10000 ** (-2 * i / width) * (keep + (1 - keep) / 8), rel_tol=1e-12)
+
+
 @pytest.mark.parametrize("kw", [dict(width=7), dict(width=0), dict(width=8, factor=0.5), dict(width=8, kind="yarn"),
                                 dict(width=8, kind="other")])
 def test_rotary_freq_refuses(kw):
