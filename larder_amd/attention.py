@@ -301,7 +301,7 @@ def attend_rows(q, cache, table, lens, cu=None, most_rows=None, longest=None, sc
     dtype = q.dtype
     if dtype not in _HALVES:
         _refuse(fn, f"q is float16 or bfloat16, not {dtype}")
-    if q_heads == 0 or q_heads % heads:
+    if q_heads == 0 or heads == 0 or q_heads % heads:
         _refuse(fn, f"{q_heads} query heads over {heads} key heads")
     cu, lens, table, n, room = _sequences(fn, cu, lens, table, t)
     dev = _device(fn, q, table, lens, cu, *cache)

@@ -126,6 +126,14 @@ def test_the_trunks_attention_of_no_rows(monkeypatch, prompt):
     assert got.shape == (0, 128)
 
 
+def test_a_cache_of_no_heads_is_refused():
+    cache, i = attention.KVCache.empty(1, 0, 64, device="cpu"), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="0 key heads"):
+        attention.attend_rows(torch.zeros(1, 2, 64, dtype=torch.float16), cache, i[None], i)
+    with pytest.raises(ValueError, match="0 key heads"):
+        attention.prompt_rows(torch.zeros(1, 2, 64, dtype=torch.float16), *[torch.zeros(1, 0, 64, dtype=torch.float16)] * 2, i)
+
+
 P = ctypes.c_void_p(16)  # never dereferenced: every call below is refused while its arguments are checked
 ODD = ctypes.c_void_p(24)
 
