@@ -308,7 +308,7 @@ def attend_rows(q, cache, table, lens, cu=None, most_rows=None, longest=None, sc
     out = q.new_empty((t, q_heads, width))
     if not t or not n:
         return out.zero_()
-    most = max(1, int(most_rows)) if most_rows is not None else 1 if cu is None else -(-t // n)
+    most = max(1, min(int(most_rows), t)) if most_rows is not None else 1 if cu is None else -(-t // n)
     long = room * page if longest is None else max(1, min(int(longest), room * page))
     need = _attend_workspace(t, q_heads, heads, width, n, most, long)
     ws = q.new_empty(need, dtype=torch.uint8) if need else None

@@ -134,6 +134,21 @@ def test_a_cache_of_no_heads_is_refused():
         attention.prompt_rows(torch.zeros(1, 2, 64, dtype=torch.float16), *[torch.zeros(1, 0, 64, dtype=torch.float16)] * 2, i)
 
 
+@pytest.mark.parametrize("most", [-1, 0, 1, 3, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 1, 10 ** 30])
+@pytest.mark.parametrize("longest", [-1, 5, 2 ** 31, 2 ** 32, 10 ** 30])
+def test_any_most_rows_and_longest_size_a_launch(monkeypatch, built_lib, most, longest):
+    """What they are worth to a launch is bounded by the rows and the table, so that no value passes an int."""
+    sizes = []
+    monkeypatch.setattr(attention, "_device", lambda *a: 0)
+    monkeypatch.setattr(attention, "_launch", lambda dev, name, *args: sizes.append(args))
+    cache = attention.KVCache.empty(1, 1, 64, device="cpu")
+    attention.attend_rows(torch.zeros(3, 2, 64, dtype=torch.float16), cache, torch.zeros(1, 20, dtype=torch.int32), CU[1:],
+                          cu=CU, most_rows=most, longest=longest)
+    rows, tokens = sizes[0][19:21]
+    assert rows == min(max(most, 1), 3) and tokens == min(max(longest, 1), 20 * 64)
+    assert sizes[0][23] == built_lib.lmoe_kv_attend_workspace_bytes(3, 2, 1, 64, 1, rows, tokens)
+
+
 P = ctypes.c_void_p(16)  # never dereferenced: every call below is refused while its arguments are checked
 ODD = ctypes.c_void_p(24)
 
