@@ -511,7 +511,7 @@ static int attend_plan(const char *fn, int T, int q_heads, int heads, int D, int
   plan->unit_shift = 7;
   long long n = items;
   if (plan->split) {
-    const long long units = items * ((longest + 127) / 128);
+    const long long units = items * ((longest + 127ll) / 128);
     n = kAttendGroups < units ? kAttendGroups : units;
   }
   plan->groups = int(n < (1 << 20) ? n : (1 << 20));  // (a workgroup takes several items where there are more)

@@ -241,6 +241,14 @@ def test_attend_workspace(built_lib):
     assert need(100, 8100, 28, 4, 128, 1) == 16 * 100 * 28 * 132 * 4 + 100 * 28 * 4  # 28 workgroups: 18 chunks, 512 keys at least
 
 
+def test_workspace_of_the_largest_sizes(built_lib):
+    """longest and most_rows of an int's end size a launch like any other: at most two workgroups a CU, two places each."""
+    need = built_lib.lmoe_kv_attend_workspace_bytes
+    for longest in (1 << 30, 2 ** 31 - 127, 2 ** 31 - 1):
+        for most in (1, 2 ** 31 - 1):
+            assert need(1, 32, 4, 128, 1, most, longest) == 512 * 2 * 16 * 130 * 4 + 32 * 8
+
+
 @pytest.mark.parametrize("unit,spare", [(32, 2), (64, 2), (128, 2), (128, 1)])
 def test_every_page_and_tile_has_a_workgroup(unit, spare):
     """Sequence b's workgroups begin at cu[b] // unit + spare b. With spare 2 that is room for every page that its rows can
