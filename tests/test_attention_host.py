@@ -249,6 +249,17 @@ def test_workspace_of_the_largest_sizes(built_lib):
             assert need(1, 32, 4, 128, 1, most, longest) == 512 * 2 * 16 * 130 * 4 + 32 * 8
 
 
+@pytest.mark.parametrize("page", [32, 64, 128])
+def test_tables_of_places_past_an_int_are_refused(built_lib, page):
+    """A table whose last page ends past 2^31 - 1: that page's tokens would not be written."""
+    wide = (1 << 31) // page
+    for name, *args in (("lmoe_kv_append", None, 64, 64, 0, P, 64, 64, P, 64, 64, 1, 1, 1, 64, P, P, 1, P, wide, P, P, P, P, 1, page, P,
+                         0, 0, 1.0, None, None),
+                        ("lmoe_kv_read", P, P, P, P, 1, page, 1, 64, P, wide, P, 1, 1, P, P, 1),
+                        ("lmoe_kv_attend", P, 1, 64, 64, 1, 1, 1, 64, P, P, 1, P, wide, P, P, P, P, 1, page, 1, 100, 0.1, P, 0, P)):
+        refused(built_lib, _lib.ESHAPE, b"a table of", name, *args)
+
+
 @pytest.mark.parametrize("unit,spare", [(32, 2), (64, 2), (128, 2), (128, 1)])
 def test_every_page_and_tile_has_a_workgroup(unit, spare):
     """Sequence b's workgroups begin at cu[b] // unit + spare b. With spare 2 that is room for every page that its rows can
