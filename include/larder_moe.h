@@ -511,7 +511,8 @@ int lmoe_rope_rows(const void *x, int dtype, long long x_row, long long x_head, 
  * its old one, and the held codes are restated. Infinities and NaN are written as NaN. q (optional) [T][q_heads][D] rotated
  * into q_out [T][q_heads][D] dense; k_out (optional) [T][heads][D] dense gets the rotated keys in dtype. n_freq % 8 == 0
  * (% 4 where interleaved), 0: no rotation. A page is written for one sequence of the call only.
- * lmoe_kv_read: rows cu[b] .. cu[b + 1] of k_out / v_out [total][heads][D] get sequence b's first tokens, code times scale.
+ * lmoe_kv_read: rows cu[b] .. cu[b + 1] of k_out / v_out [total][heads][D] get sequence b's first tokens, code times scale;
+ * zeros where the table has no page (lmoe_prompt_attend sees those as keys: leave them out of the table and cu).
  * lmoe_kv_attend: out [T][q_heads][D] = softmax(scale q k^T) v in float16 / bfloat16, row r of a sequence's n over its first
  * lens - n + r + 1 tokens (none: zero). most_rows / longest: about the most rows / tokens of a sequence (any value is sound;
  * they size the launch). workspace: lmoe_kv_attend_workspace_bytes of the same numbers, 16-byte aligned. */

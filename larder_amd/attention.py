@@ -17,9 +17,11 @@ and v side by side; one whose layout no kernel reads is copied first.
 
 lens int32 [sequences] counts a sequence's tokens with the rows of the call among them: row r of n stands at place lens -
 n + r. table int32 [sequences, width] lists each sequence's pages in order; entries behind its last page are not read. A
-page outside the cache (or the table) holds nothing: no token is written there and none is seen. Sequences may share pages
-they only read; a page that a call writes to stands in one place of one table. A row that sees no token, or only tokens that
-score -infinity, attends to nothing: it is zero.
+page outside the cache (or the table) holds nothing: no token is written there and attend_rows sees none. read_rows gives its
+tokens back as zeros, which prompt_rows would see as any others: a history with such holes is read through a table, and with
+offsets, that leave them out (the rows see the keys that are left, as attend_rows has them). Sequences may share pages they
+only read; a page that a call writes to stands in one place of one table. A row that sees no token, or only tokens that score
+-infinity, attends to nothing: it is zero.
 """
 import functools
 import math
@@ -272,7 +274,8 @@ def append_rows(cache, q, k, v, table, lens, cu=None, freq=None, interleaved=Fal
 
 def read_rows(cache, table, cu, total, dtype=torch.bfloat16):
     """(k, v) [total, heads, width] in dtype: the first cu[b + 1] - cu[b] tokens of every sequence, codes times scale, rounded
-    once (bfloat16 holds them exactly): the history that the rows of a later prompt chunk see, for prompt_rows."""
+    once (bfloat16 holds them exactly): the history that the rows of a later prompt chunk see, for prompt_rows. Tokens whose page
+    is not there are zero."""
     fn = "read_rows"
     pages, heads, page, width, *codes = _cache(fn, cache)
     dt = dcode(dtype)

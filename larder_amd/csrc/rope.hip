@@ -456,8 +456,8 @@ static int check_cache(const char *fn, int heads, int D, int page, int pages, in
   LMOE_REQUIRE(page == 32 || page == 64 || page == 128, LMOE_ESHAPE, "%s: pages of %d tokens (32, 64 and 128 are served)", fn,
                page);
   // a page's end is an int
-  LMOE_REQUIRE(heads > 0 && heads <= 65535 && pages > 0 && width > 0 && width <= 0x7fffffff / page, LMOE_ESHAPE, "%s: %d heads, %d pages, a table of %d", fn,
-               heads, pages, width);
+  LMOE_REQUIRE(heads > 0 && heads <= 65535 && pages > 0 && width > 0 && width <= 0x7fffffff / page, LMOE_ESHAPE,
+               "%s: %d heads, %d pages, a table of %d", fn, heads, pages, width);
   return 0;
 }
 

@@ -72,7 +72,8 @@ def attention_rows(x, qkv, out, cache, table, lens, cu=None, freq=None, interlea
       prompt None              the newest rows of each sequence over its cached tokens (attend_rows; most_rows, longest its)
       prompt True              sequences that begin with this call, over the call's own keys and values (prompt_rows)
       prompt (cu_k, total)     later chunks of prompts: over all the cached tokens, lens of each, total in all, cu_k int32
-                               [sequences + 1] where each begins (read_rows, prompt_rows)
+                               [sequences + 1] where each begins (read_rows, prompt_rows); none of them in a page that is
+                               not there
     """
     heads, width = cache.k.shape[1], cache.k.shape[3]
     # what a later call would refuse is refused here, before the cache is written

@@ -919,3 +919,33 @@ def test_append_gives_tensors_of_its_own():
         q, k = attention.append_rows(cache, x[:, :2], x[:, 2:3], x[:, 3:], ints([[0]]), ints([1]), freq=freq, keys=True)
         q.zero_(), k.zero_()
         assert (x == 1).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_history_with_holes_read_without_them(dtype):
+    """A prompt chunk over a history some of whose pages are gone: attend_rows through the table with the holes, and prompt_rows
+    over what a table without them reads, are the same attention."""
+    from larder_amd import attention
+    rng = np.random.default_rng(35)
+    heads, width, page = 2, 128, 32
+    rows, lens = [9, 20], [150, 70]
+    cu = cu_of(rows)
+    table, n = page_table(rng, [5, 3])
+    cache = random_cache(rng, n, heads, width, page)
+    held = [table[0][[0, 3, 4]], table[1][[1, 2]]]
+    gaps = table.copy()
+    gaps[0, 1], gaps[0, 2], gaps[1, 0] = -1, n, -5
+    compact = np.full((2, 3), -1, np.int32)
+    compact[0], compact[1, :2] = held
+    cu_k = cu_of([150 - 64, 70 - 32])
+    q = normal(rng, cu[-1], 4, width, dtype=dtype)
+    over_cache = attention.attend_rows(q, cache, ints(gaps), ints(lens), cu=ints(cu))
+    check_attend(over_cache, q, cache, gaps, lens, cu, width ** -0.5, dtype)
+    k, v = attention.read_rows(cache, ints(compact), ints(cu_k), cu_k[-1], dtype=dtype)
+    over_rows = attention.prompt_rows(q, k, v, ints(cu), cu_k=ints(cu_k))
+    for b in range(2):
+        codes = cache_host(cache)
+        (hk, there), (hv, _) = (ref.read(*c, gaps[b], lens[b]) for c in codes)
+        x, have = host(q[cu[b]:cu[b + 1]]), host(over_rows[cu[b]:cu[b + 1]])
+        want, spread = ref.attend(x, hk, hv, width ** -0.5, there)
+        assert (np.abs(have - want) <= attention_bound(x, hk, width ** -0.5, want, spread, dtype, dtype)).all()
