@@ -949,3 +949,103 @@ def test_history_with_holes_read_without_them(dtype):
         x, have = host(q[cu[b]:cu[b + 1]]), host(over_rows[cu[b]:cu[b + 1]])
         want, spread = ref.attend(x, hk, hv, width ** -0.5, there)
         assert (np.abs(have - want) <= attention_bound(x, hk, width ** -0.5, want, spread, dtype, dtype)).all()
+
+
+# ---- larger sizes, and a page's codes whatever begins it ---------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("q_heads,heads,width,rows,keys", [
+    (2, 1, 64, [1500], [1500]), (2, 1, 128, [1031, 640], [1031, 640]), (2, 2, 256, [900], [900]), (2, 1, 128, [700], [2900]),
+    (1, 1, 64, [513] * 2 + [1] * 70, [513] * 2 + [1] * 70)])
+def test_prompt_long(dtype, q_heads, heads, width, rows, keys):
+    """Prompts of many tiles, alone, beside others and over a history: the loop's full tiles, between its first and last."""
+    from larder_amd import attention
+    rng = np.random.default_rng(sum(rows) + width)
+    cu, cu_k = cu_of(rows), cu_of(keys)
+    q, k, v = normal(rng, cu[-1], q_heads, width, dtype=dtype), *(normal(rng, cu_k[-1], heads, width, dtype=dtype) for _ in range(2))
+    got = attention.prompt_rows(q, k, v, ints(cu), cu_k=ints(cu_k))
+    check_prompt(got, q, k, v, cu, cu_k, width ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("q_heads,heads,width,page,rows,lens", [
+    (7, 1, 128, 64, [1], [9001]), (4, 2, 64, 128, [1, 1, 1], [5000, 12, 7777]), (4, 1, 256, 32, [1, 3], [4100, 2500]),
+    (8, 1, 128, 64, [16], [6000]), (8, 2, 64, 32, [16, 5], [3500, 2101])])
+def test_attend_long(dtype, q_heads, heads, width, page, rows, lens):
+    """Long caches of varied values: many units an item, joined from several workgroups; single and draft rows."""
+    from larder_amd import attention
+    rng = np.random.default_rng(sum(lens))
+    cu = cu_of(rows)
+    table, n = page_table(rng, [-(-x // page) for x in lens])
+    cache = random_cache(rng, n, heads, width, page)
+    q = normal(rng, cu[-1], q_heads, width, dtype=dtype)
+    for longest in (None, max(lens), 600):
+        got = attention.attend_rows(q, cache, ints(table), ints(lens), cu=ints(cu), most_rows=max(rows), longest=longest)
+        check_attend(got, q, cache, table, lens, cu, width ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("rows,tokens", [(3, 2), (40, 33), (5, 1), (4, 0)])
+def test_append_more_rows_than_tokens(rows, tokens):
+    """Rows that stand before a sequence's first place are not written; the page's whole codes and its scale are those of the
+    tokens that have a place."""
+    from larder_amd import attention
+    rng = np.random.default_rng(rows)
+    k, v = (normal(rng, rows, 2, 64, dtype=F32, scale=s) for s in (1, 9))
+    k[0], v[0] = 1e6, 1e6  # before the first place: not in the scale
+    cache, table = poisoned(4, 2, 64, 32), np.array([[3, 1]])
+    want = cache_host(cache)
+    attention.append_rows(cache, None, k, v, ints(table), ints([tokens]), cu=ints([0, rows]))
+    for (codes, scales), x in zip(want, (k, v)):
+        ref.append(codes, scales, host(x)[rows - tokens:], [0, tokens], [tokens], table)
+    for (codes, scales), (gc, gs) in zip(want, cache_host(cache)):
+        assert np.array_equal(scales, gs, equal_nan=True)
+        assert np.array_equal(codes & 0x7f == 0x7f, gc & 0x7f == 0x7f) and np.array_equal(
+            np.nan_to_num(ref.E4M3[codes]), np.nan_to_num(ref.E4M3[gc]))  # no rotation: powers of two, one rounding, exactly
+
+
+def test_trunk_attention_against_float64():
+    """attention_rows against float64 from its 4-bit products on: a prompt, a later chunk, draft rows, a token, with a rotation of
+    half a head. The output weight is the identity (values 0 and 1, scale 1, no bias), which qmv gives back exactly, and the
+    products before it are the oracle's bits. q, and in the first chunk k, are rounded to bfloat16 once more than the oracle's:
+    each moves a score by 2^-8 of sum |q k| scale at most, and a weight by as much of itself, in a row's sums twice."""
+    from larder_amd import attention, trunk
+    from oracle import qmv
+    rng = np.random.default_rng(36)
+    H, q_heads, heads, width, G = 256, 4, 2, 64, 64
+    rows = (q_heads + 2 * heads) * width
+    wq, sc, bi = qmv.quantize_affine4((rng.standard_normal((rows, H)) * 0.05).astype(np.float32), G)
+    one = np.zeros((q_heads * width, q_heads * width // 8), np.uint32)
+    for i in range(q_heads * width):
+        one[i, i // 8] = 1 << 4 * (i % 8)
+    ones = np.ones((q_heads * width, q_heads * width // G), np.float32)
+    x0 = qmv.bf16(rng.standard_normal((2, q_heads * width)))
+    assert np.array_equal(qmv.qmv_rows(x0, one, ones, 0 * ones, G), x0)
+
+    def dev(w, s, b):
+        return torch.from_numpy(w.view(np.int32)).cuda(), *(torch.from_numpy(np.ascontiguousarray(a, np.float32)).cuda().bfloat16()
+                                                           for a in (s, b)), G
+    qkv, out = dev(wq, sc, bi), dev(one, ones, 0 * ones)
+    freq, gain = attention.rotary_freq(32, 1e4, "linear", 2.0)
+    table, n = page_table(rng, [5, 4])
+    cache, lens = poisoned(n, heads, width, 32), np.zeros(2, int)
+    for new, kind in (([70, 41], "first"), ([30, 50], "later"), ([3, 1], "drafts"), ([1, 1], "token")):
+        lens, cu = lens + new, cu_of(new)
+        x = normal(rng, cu[-1], H)
+        cu_k = cu_of(lens)
+        got = trunk.attention_rows(x, qkv, out, cache, ints(table), ints(lens), cu=None if kind == "token" else ints(cu), freq=freq,
+                                   gain=gain, prompt={"first": True, "later": (ints(cu_k), cu_k[-1])}.get(kind),
+                                   most_rows=3 if kind == "drafts" else None)
+        y = qmv.qmv_rows(host(x).astype(np.float32), wq, sc, bi, G).astype(np.float64).reshape(cu[-1], -1, width)
+        codes = cache_host(cache)
+        for b in range(2):
+            at, pos = slice(cu[b], cu[b + 1]), np.arange(lens[b] - new[b], lens[b])
+            q, k = (ref.rope(y[at, h], pos, host(freq), False, gain) for h in (slice(q_heads), slice(q_heads, q_heads + heads)))
+            v = y[at, q_heads + heads:]
+            if kind != "first":
+                k, v = (ref.read(*c, table[b], lens[b])[0] for c in codes)
+            want, spread = ref.attend(q, k, v, width ** -0.5)
+            top = np.einsum("ihd,jhd->ihj", np.abs(q), np.abs(k).repeat(2, 1)).max(-1)[..., None] * width ** -0.5
+            moved = 2 * (2 if kind == "first" else 1) * 2.0 ** -8 * top * 1.01
+            bound = attention_bound(q, k, width ** -0.5, want, spread, BF16, BF16 if kind in ("first", "later") else F16)
+            have = host(got[at]).reshape(want.shape)
+            assert (np.abs(have - want) <= bound + np.expm1(moved) * spread).all(), (kind, b)
