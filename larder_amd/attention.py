@@ -11,9 +11,10 @@ GPU.
     prompt_rows(q, k, v, cu, ...)                 packed sequences, causal, over their own keys and values
 
 Rows are packed: tensors [T, heads, width] hold the sequences one after the other, and cu int32 [sequences + 1] says where
-each begins (cu[0] = 0; one row a sequence where cu is None). Rows of no sequence come back zero. Heads are 64, 128 or 256
-channels wide, and any number of query heads shares a key head. Rows may be strided views, as of a product that gives q, k
-and v side by side; one whose layout no kernel reads is copied first.
+each begins (cu[0] = 0, none less than the one before; one row a sequence where cu is None). Rows of no sequence come back zero.
+Heads are 64, 128 or 256 channels wide, and any number of query heads shares a key head. Rows may be strided views, as of a
+product that gives q, k and v side by side; one whose layout no kernel reads is copied first. Offsets, lengths and tables live on
+the GPU, and the host does not see them: wrong ones give rows and pages of no meaning, and touch no other memory.
 
 lens int32 [sequences] counts a sequence's tokens with the rows of the call among them: row r of n stands at place lens -
 n + r. table int32 [sequences, width] lists each sequence's pages in order; entries behind its last page are not read. A

@@ -79,12 +79,13 @@ struct Seqs {
   int *ends;  // [64] where a sequence ends on the line
   int b0;     // the first of them
   int base;   // where that begins
+  bool rising = true;  // of the lane's sequences: offsets that do not fall
 
   __device__ __forceinline__ void load(const AttendArgs &a, int from, int begins) {
     const int lane = threadIdx.x & 63, b = from + lane;
     int3 s = {0, 0, 0};
     if (b < a.B) {
-      seq_rows(a.cu, b, a.T, &s.x, &s.y);
+      rising &= seq_rows(a.cu, b, a.T, &s.x, &s.y);
       s.z = a.lens[b];
     }
     seq[lane] = s;
@@ -209,11 +210,12 @@ __global__ void __launch_bounds__(64 * kAttendWaves, D == 256 ? 2 : 3) k_attend(
 #pragma unroll 4
     for (int b = 64 + lane; b < a.B; b += 64) {
       int row0, n;
-      seq_rows(a.cu, b, a.T, &row0, &n);
+      seqs.rising &= seq_rows(a.cu, b, a.T, &row0, &n);
       more += share(a, row0, n, a.lens[b]).total(a.heads);
     }
     line += __builtin_amdgcn_readlane(wave_scan(more), 63);
   }
+  if (!__all(seqs.rising)) return;  // sequences with the same rows could have more units than 32 bits count
   // no more workgroups than units: each has one at least, so that every one between an item's first and last writes its place
   const int groups = min(a.groups, line);
   if (int(blockIdx.x) >= groups) return;

@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_prompt(PromptArgs a) 
     }
   }
   const int first = tile * kPromptRows;
-  if (first >= nq) return;
+  if (uint32_t(first) >= uint32_t(nq)) return;  // (a tile before the sequence's first: where offsets fall)
   const int off = nk - nq;                                  // row i sees keys 0 .. i + off
   const int most_keys = off + min(first + kPromptRows, nq);  // what the workgroup's last row sees
   const int begin = chunk * a.chunk;                         // this workgroup's keys: [begin, keys)

@@ -111,7 +111,7 @@ __device__ __forceinline__ void places_of(const RopeArgs &a, int t0, int nt, int
     if (b >= 0 && b < a.B) {
       int r0, n;
       seq_rows(a.cu, b, a.T, &r0, &n);
-      if (row < r0 + n) pos = a.lens[b] - n + (row - r0);
+      if (row >= r0 && row < r0 + n) pos = a.lens[b] - n + (row - r0);
     }
     if (lane == 0) place[i] = pos;
   }
@@ -317,7 +317,9 @@ __global__ void __launch_bounds__(256) k_append(AppendArgs a, RopeArgs rope_rows
   seq_rows(a.cu, b, a.T, &row0, &n);
   if (n == 0) return;
   const int start = a.lens[b] - n;  // the first new token's place
-  const int p = max(start, 0) / page + (a.cu ? task - (row0 / page + 2 * b) : 0);
+  const int nth = a.cu ? task - (row0 / page + 2 * b) : 0;
+  if (nth < 0) return;  // (where offsets fall)
+  const int p = max(start, 0) / page + nth;
   const int lo = max(start, p * page), hi = min(start + n, (p + 1) * page);
   if (hi <= lo || p >= a.width) return;
   const int number = a.table[size_t(b) * a.width + p];
@@ -399,7 +401,7 @@ __global__ void __launch_bounds__(256) k_read(ReadArgs a) {
       int s0, n;
       seq_rows(a.cu, b, a.total, &s0, &n);
       at = row - s0;
-      if (at < n && at / a.page < a.width) number = a.table[size_t(b) * a.width + at / a.page];
+      if (at >= 0 && at < n && at / a.page < a.width) number = a.table[size_t(b) * a.width + at / a.page];
       if (number >= a.pages) number = -1;
     }
     if ((threadIdx.x & 63) == 0) page_of[i] = number, place[i] = at % a.page;

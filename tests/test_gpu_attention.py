@@ -1049,3 +1049,33 @@ def test_trunk_attention_against_float64():
             bound = attention_bound(q, k, width ** -0.5, want, spread, BF16, BF16 if kind in ("first", "later") else F16)
             have = host(got[at]).reshape(want.shape)
             assert (np.abs(have - want) <= bound + np.expm1(moved) * spread).all(), (kind, b)
+
+
+@pytest.mark.parametrize("n", [3, 70, 200])
+def test_offsets_that_fall_touch_nothing_else(n):
+    """Offsets in no order, negative ones and ones past the rows among them: calls end, pages of no table and memory around the
+    cache stay as they were, and the next sound call is right."""
+    from larder_amd import attention
+    rng = np.random.default_rng(n)
+    t, heads, width, page = 700, 2, 64, 32
+    wide = random_cache(rng, 60, heads, width, page)
+    before = [x.clone() for x in wide]
+    cache = attention.KVCache(*(x[20:40] for x in wide))
+    table = ints(rng.integers(0, 12, (n, 4)))          # pages 12 .. 19 of the cache are nobody's
+    lens = ints(rng.integers(-3, 140, n))
+    q, k, v = (normal(rng, t, h, width, dtype=F16) for h in (4, heads, heads))
+    for _ in range(6):
+        cu = rng.integers(-40, t + 100, n + 1)
+        cu[rng.integers(0, n + 1)] = rng.choice([-2 ** 31, 2 ** 31 - 1])
+        cu = ints(cu)
+        outs = [*attention.append_rows(cache, q, k, v, table, lens, cu=cu, freq=frequencies(16), keys=True),
+                *attention.read_rows(cache, table, cu, t, dtype=F16), attention.prompt_rows(q, k, v, cu),
+                attention.prompt_rows(q, k, v, cu, cu_k=ints(rng.integers(-40, t + 100, n + 1))),
+                attention.attend_rows(q, cache, table, lens, cu=cu), attention.attend_rows(q, cache, table, lens, cu=cu, longest=1)]
+        assert all(o.shape[0] == t for o in outs)
+        for a, b in zip(wide, before):
+            a, b = (x.view(torch.uint8) for x in (a, b))
+            assert torch.equal(a[:20], b[:20]) and torch.equal(a[32:], b[32:])
+    cu = [0, 300, 300, 333]
+    got = attention.prompt_rows(q[:333], k[:333], v[:333], ints(cu))
+    check_prompt(got, q[:333], k[:333], v[:333], cu, cu, width ** -0.5, F16)
