@@ -492,7 +492,8 @@ int lmoe_quantize_q4_k(const void *w, int wdtype, long long rows, int cols, uint
 
 /* ---- attention of the trunk's rows ----
  * Rows are packed: [T][heads][D] with strides in elements between rows and between heads, channels dense; sequence b's rows
- * are cu[b] .. cu[b + 1] (int32 [B + 1], cu NULL: row b alone, T == B). Rows of no sequence come back zero where a call
+ * are cu[b] .. cu[b + 1] (int32 [B + 1], none less than the one before; cu NULL: row b alone, T == B). Where offsets, lengths or
+ * tables are wrong, rows and pages have no meaning, and no other memory is touched. Rows of no sequence come back zero where a call
  * returns rows. Alignment of 16 bytes is asked of rows, heads and codes unless said otherwise.
  *
  * lmoe_rope_rows: rotary positions (route_cuda.py:549-591's rotation): the first 2 n_freq of a head's D channels (D <= 1024)

@@ -206,10 +206,11 @@ def _prompt_workspace(*sizes):
 # ---- the calls -------------------------------------------------------------------------------------------------
 
 def rope_rows(x, positions, freq, interleaved=False, gain=1.0, out=None):
-    """x [T, heads, width] (float16, bfloat16 or float32) with the first 2 len(freq) channels of every head rotated by the
+    """x [T, heads, width] (float16, bfloat16 or float32; width up to 1,024) with the first 2 len(freq) channels of every head rotated by the
     angles positions[t] * freq (positions int32 or int64 [T], any; freq float64, radians): pairs (i, i + len(freq)), or
     (2 i, 2 i + 1) where interleaved, multiplied by gain; the other channels as they are. float32 inside, one rounding.
-    out: a tensor of x's shape and type, which may be x; rows of any strides with a dense last axis."""
+    out: a tensor of x's shape and type, which may be x (and shares no memory with it otherwise); rows of any strides with a
+    dense last axis."""
     fn = "rope_rows"
     if x.dim() != 3:
         _refuse(fn, "x is [rows, heads, width]")
@@ -296,6 +297,10 @@ def attend_rows(q, cache, table, lens, cu=None, most_rows=None, longest=None, sc
     their sequences: row r of a sequence's n sees its first lens - n + r + 1 tokens (a row that sees none is zero); scale is
     width^-0.5 if None. Made for few rows a sequence: one token of each, or a speculative decoder's draft.
 
+    Sums are float32; weights are rounded to float16, times 2^11, so that one keeps all its bits down to 2^-25 of the row's
+    largest (below about 2^-35 it is zero), and the sum that a row is divided by is the rounded weights'. Values from about 2^90 on can
+    overflow the sums.
+
     most_rows and longest size the launch: about the most rows of a sequence (1 without cu, else T / sequences) and tokens of
     one (the table's room). Any values give the same sums in another order."""
     fn = "attend_rows"
@@ -326,7 +331,12 @@ def prompt_rows(q, k, v, cu, cu_k=None, scale=None):
     """softmax(scale q k^T) v of packed sequences, causal: q [T, query heads, width], k and v [U, heads, width] (float16 or
     bfloat16), sequence b's rows cu[b] .. cu[b + 1] of q and cu_k[b] .. cu_k[b + 1] of k and v (cu_k None: the same rows).
     The last row sees all of its sequence's keys, each row before it one fewer; a row that sees none is zero. scale is
-    width^-0.5 if None."""
+    width^-0.5 if None.
+
+    Sums are float32; weights are rounded to the inputs' type for their product with the values (bfloat16: half a step of 2^-8
+    each, about as much again as the result's own rounding; float16: times 2^11, as in attend_rows), and the sum that a row is
+    divided by is the rounded weights'. A value that is not finite makes its channel infinite or NaN in the rows that see it,
+    and touches no other. Values from about 2^100 on can overflow the sums."""
     fn = "prompt_rows"
     q, q_row, q_head = _rows(fn, "q", q)
     t, q_heads, width = q.shape

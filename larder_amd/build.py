@@ -25,9 +25,9 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-ffp-contract=off", "-Xclang", "-target-feature",
           "-Xclang", "-packed-fp32-ops", "-Wall", "-Wno-unused-function", "-Wno-unused-variable"]
 
-# Per-file extras. The grouped GEMMs and the attention kernels: MFMA accumulators in arch VGPRs. Left to its heuristics the compiler puts them in
-# AGPRs with the untied MFMA form, and every K step then rotates them through ~130 accvgpr moves; in VGPRs they
-# stay put and the kernel fits two workgroups a CU (237 VGPRs, no AGPRs).
+# Per-file extras. The grouped GEMMs and the attention kernels: MFMA accumulators in arch VGPRs. Left to its
+# heuristics the compiler puts them in AGPRs with the untied MFMA form, and every K step then rotates them through
+# ~130 accvgpr moves; in VGPRs they stay put and the grouped kernel fits two workgroups a CU (237 VGPRs, no AGPRs).
 FILE_FLAGS = {n: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for n in ("grouped.hip", "grouped_any.hip", "attend.hip", "prompt.hip")}
 
 

@@ -3,8 +3,8 @@
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - m),  over the places j < len - (n - 1 - r) of row r of n
 //
 // One pass over the keys and values with a running maximum m. Bound by the cache's bytes: 2 width a token and key head, read
-// once for all the query heads of its group and all of a sequence's rows (up to 16 of these together fill a matrix-core
-// tile's columns).
+// once for every 16 (row, query head of the group) pairs of a sequence, which fill a matrix-core tile's columns: once for a
+// token of up to 16 heads a group, three times for five draft rows of 8, eight times for sixteen.
 //
 // A wavefront takes 32 tokens a step, straight from global memory to registers; no LDS until the end. Products are written
 // so that nothing has to change lanes between them:
@@ -24,8 +24,8 @@
 //
 // Measured: 64 sequences of 1,024 to 16,384 tokens, 32 heads over 4 of 128: 75 us, 5.0 TB/s, and 4.5 to join (chunks of one
 // length on a grid of the longest: 125, two thirds of the workgroups empty and the rest uneven over the XCDs); one sequence of
-// 131,072: 26 and 5.4; heads of 256: 79 (190). One unit takes 5.7 (width 64) to 8.4 us (256) from launch to end: lengths,
-// pages, codes and the wavefronts' join, one after the other.
+// 131,072: 26 and 5.4; heads of 256: 79 (190), with 256 registers and five spilled (24 bytes of scratch a lane). One unit takes
+// 5.7 (width 64) to 8.4 us (256) from launch to end: lengths, pages, codes and the wavefronts' join, one after the other.
 #include "rows.h"
 
 namespace lmoe {

@@ -522,8 +522,11 @@ __global__ void __launch_bounds__(256) k_prompt_join(PromptArgs a) {
   *reinterpret_cast<u32x2 *>(a.out + line * D + d) = u32x2{pack2<BF>(v[0] * inv, v[1] * inv), pack2<BF>(v[2] * inv, v[3] * inv)};
 }
 
-// Chunks of keys, where the rows alone would leave CUs idle: as many as bring the workgroups to two a CU (one at width 256),
-// of 512 keys (eight tiles) at least
+// Chunks of keys, where the rows alone would leave half of the GPU's places idle (two workgroups a CU, one at width 256): as many
+// as fit the places, of 512 keys (eight tiles) at least. Rows' tiles are bounded by T / 128 + B, one more a sequence than there
+// are where rows fill their tiles: one sequence's 1,024 rows over 8,024 keys are 448 workgroups on 512 places with 28 heads of
+// 128, in two chunks, but with 32 heads 256 in one, and with 16 heads of 256 channels 128 on 256. Between half of the places
+// and all of them nothing is split.
 struct PromptPlan {
   int chunk, chunks;
   size_t rows, bytes;  // the workspace's sums, and all of it

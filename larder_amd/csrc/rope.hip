@@ -10,7 +10,8 @@
 //
 // Bound by HBM: 8,192 rows of 32 heads of 128 in float16, neighbouring pairs: 23.5 us, 5.7 TB/s. Threads run over a row's
 // units, pairs and the channels that stay apart; with divisions for every unit and both kinds in one wavefront it took 29.3,
-// and 54 for what takes 32 where a quarter of 256 channels turns.
+// and 54 for what takes 32 where a quarter of 256 channels turns. The choice of tensor for each unit (queries or keys) goes
+// through 24 bytes of scratch a lane in k_rope<8> and k_append.
 //
 // The cache: e4m3 codes [page][head][token of the page][width] and one float32 scale for each page and head, of keys and of
 // values. The scale is the least power of two (2^-100 at least) that brings the largest finite magnitude of the page's head
@@ -18,8 +19,9 @@
 // codes that become subnormal, so a page filled token by token holds what one written at once would, up to those. e4m3 has
 // no infinity: infinities and NaN become NaN, and stay out of the scale.
 //
-// Measured: 64 sequences' tokens (32 + 8 heads of 128) 8.8 us, five dependent loads; 9,344 rows of prompts (16 + 4 heads of
-// 256) with their rotation 40 us, 4.3 TB/s; reading those pages back in 16 bits 11 us.
+// Measured: 64 sequences' tokens (32 + 8 heads of 128) 8.8 us, five dependent loads; 9,349 rows of prompts (16 + 4 heads of
+// 256) with their rotation 51 us, 3.7 TB/s of 192 MB, on tensors that no cache holds (the same ones again and again: 40);
+// reading those pages back in 16 bits 11.5 us, 2.5 TB/s: eight codes a thread, each behind two divisions and a scale's load.
 #include "rows.h"
 
 namespace lmoe {
@@ -499,6 +501,8 @@ extern "C" int lmoe_kv_append(const void *q, long long q_row, long long q_head, 
   // One launch: the rotation hides the latency of the pages' few workgroups (prompts at width 256: 18 + 33 us apart, 46
   // together), and a token's call saves a launch. Pages go first where there are many rows, so that their chain of loads is
   // not what the launch ends with. Apart only where a page's registers would leave the rotation two wavefronts a SIMD.
+  // A page's cos / sin in LDS can bound it as well, which the rule does not look at: whole heads of 128 on pages of 128 (or of
+  // 256 on 64) take 64 KiB a workgroup, two a CU.
   const bool together = rows && (T <= 1024 || page * D <= 16384);
   const int rotating = together ? (T + r.tokens - 1) / r.tokens : 0;
   a.pages_at = T <= 1024 ? rotating : 0;

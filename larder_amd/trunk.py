@@ -3,7 +3,7 @@
     qmv_fits(x, w, scales, group_size, bits, mode, biases)   route_cuda.py:516-522
     qmv_rows(x, w, scales, biases, group_size)               route_cuda.py:525-541 (lmoe_qmv_rows)
     shared_expert_rows(x, gate, up, down)                    mlx_lm's shared_expert MLP on qmv_rows projections
-    attention_rows(x, qkv, out, cache, table, lens, ...)     mlx_lm's attention on qmv_rows projections and the paged cache
+    attention_rows(x, qkv, out, cache, table, lens, ...)     rotary attention on qmv_rows projections and the paged cache
 
 qmv_rows gives every row of x the bits of the reference's kernel (MLX 0.32.4's one-row qmv arithmetic: bf16
 weights, bf16 fused multiply-add slots, a float32 slot sum and lane butterfly), reading the weights once a pass.
@@ -67,13 +67,16 @@ def attention_rows(x, qkv, out, cache, table, lens, cu=None, freq=None, interlea
                    most_rows=None, longest=None):
     """The trunk's attention of x [T, H] bf16 (larder_amd.attention's packed rows): out(attend(rotate(qkv(x)))), with qkv and
     out (w, scales, biases, group_size) 4-bit affine weights run through qmv_rows, qkv's output the query heads, then the key
-    heads, then the value heads of the cache's width. The rows' keys and values are written to the cache, then read by
+    heads, then the value heads of the cache's width. Nothing else stands between the steps: a model with biases on q, k and v,
+    norms of q's and k's heads before the rotation, or a gate on the output calls larder_amd.attention's parts itself. The rows'
+    keys and values are written to the cache, then read by
 
       prompt None              the newest rows of each sequence over its cached tokens (attend_rows; most_rows, longest its)
       prompt True              sequences that begin with this call, over the call's own keys and values (prompt_rows)
       prompt (cu_k, total)     later chunks of prompts: over all the cached tokens, lens of each, total in all, cu_k int32
                                [sequences + 1] where each begins (read_rows, prompt_rows); none of them in a page that is
-                               not there
+                               not there. The chunk's own keys and values are among them, in the cache's 8 bits, where a
+                               first chunk (True) takes its own in 16
     """
     heads, width = cache.k.shape[1], cache.k.shape[3]
     # what a later call would refuse is refused here, before the cache is written
