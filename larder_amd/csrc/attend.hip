@@ -442,13 +442,15 @@ __global__ void __launch_bounds__(64 * kAttendWaves, D == 256 ? 2 : 3) k_attend(
   }
 }
 
-// One workgroup a query row and head: where more than one workgroup of k_attend had its item, their places joined in order
+// One workgroup a query row and head (blockIdx.x first): where more than one workgroup of k_attend had its item, their places joined in order
 template <int D, bool BF>
 __global__ void __launch_bounds__(256) k_attend_join(AttendArgs a) {
   constexpr int LANES = D / 4, PARTS = 256 / LANES;  // threads over the channels, and over the places
   __shared__ float sums[PARTS][D];
   __shared__ float tops[PARTS], weights[PARTS];
-  const int2 join = a.joins[blockIdx.x];
+  const size_t line = blockIdx.x + size_t(blockIdx.y) * gridDim.x;
+  if (line >= size_t(a.T) * a.q_heads) return;
+  const int2 join = a.joins[line];
   if (join.x < 0) return;
   const int in = join.y & 15, w0 = min(join.x >> 1, a.groups - 1), w1 = min(join.y >> 4, a.groups - 1);
   const int part = threadIdx.x / LANES, d = (threadIdx.x - part * LANES) * 4;
@@ -484,7 +486,7 @@ __global__ void __launch_bounds__(256) k_attend_join(AttendArgs a) {
   if (threadIdx.x >= LANES) return;
 #pragma unroll 1
   for (int j = 1; j < PARTS; ++j) add(tops[j], weights[j], *reinterpret_cast<const f32x4 *>(&sums[j][d]));
-  store4<BF>(a.out, size_t(blockIdx.x) * D + d, v, weight);
+  store4<BF>(a.out, line * D + d, v, weight);
 }
 
 // Sequences of up to 512 tokens (four tiles a wavefront) are one unit each: joining would cost what splitting gains
@@ -569,7 +571,9 @@ extern "C" int lmoe_kv_attend(const void *q, int dtype, long long q_row, long lo
     launch(kernel, dim3(unsigned(plan.groups)), dim3(64 * kAttendWaves), lds, st, a);
     LMOE_LAUNCHED(fn);
     if (plan.split) {
-      launch(join, dim3(unsigned(T) * unsigned(q_heads)), dim3(256), 0, st, a);
+      // a grid of 2^32 threads or more is cut without a word: rows and heads over two axes
+      const unsigned lines = unsigned(T) * unsigned(q_heads), x = lines < (1u << 23) ? lines : 1u << 23;
+      launch(join, dim3(x, (lines + x - 1) / x), dim3(256), 0, st, a);
       LMOE_LAUNCHED(fn);
     }
     return 0;

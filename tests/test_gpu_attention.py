@@ -1079,3 +1079,18 @@ def test_offsets_that_fall_touch_nothing_else(n):
     cu = [0, 300, 300, 333]
     got = attention.prompt_rows(q[:333], k[:333], v[:333], ints(cu))
     check_prompt(got, q[:333], k[:333], v[:333], cu, cu, width ** -0.5, F16)
+
+
+def test_attend_more_rows_than_a_grid_has_workgroups():
+    """2^24 rows and heads and some: each is joined. One sequence of more rows than tokens, most of which see none."""
+    from larder_amd import attention
+    rng = np.random.default_rng(37)
+    t, n = (1 << 19) + 1, 600
+    cache = random_cache(rng, 19, 4, 64, 32)
+    table = rng.permutation(19).astype(np.int32)[None]
+    q = torch.ones(t, 32, 64, dtype=F16, device="cuda")
+    q[-n:] = normal(rng, n, 32, 64, dtype=F16)
+    torch.full((t * 32 * 64,), 7.0, dtype=F16, device="cuda")  # what the output is allocated from
+    got = attention.attend_rows(q, cache, ints(table), ints([n]), cu=ints([0, t]))
+    assert not got[:-n].any()
+    check_attend(got[-n:], q[-n:], cache, table, [n], [0, n], 64 ** -0.5, F16)
