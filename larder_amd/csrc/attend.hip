@@ -571,8 +571,7 @@ extern "C" int lmoe_kv_attend(const void *q, int dtype, long long q_row, long lo
     launch(kernel, dim3(unsigned(plan.groups)), dim3(64 * kAttendWaves), lds, st, a);
     LMOE_LAUNCHED(fn);
     if (plan.split) {
-      // a grid of 2^32 threads or more is cut without a word: rows and heads over two axes
-      const unsigned lines = unsigned(T) * unsigned(q_heads), x = lines < (1u << 23) ? lines : 1u << 23;
+      const unsigned lines = unsigned(T) * unsigned(q_heads), x = lines < kMostGroups ? lines : 1u << 23;  // two axes past one's end
       launch(join, dim3(x, (lines + x - 1) / x), dim3(256), 0, st, a);
       LMOE_LAUNCHED(fn);
     }

@@ -577,7 +577,8 @@ extern "C" int lmoe_prompt_attend(const void *q, long long q_row, long long q_he
                "%s: rows of keys %lld and of values %lld elements apart", fn, k_row, v_row);
   const long long tiles = T / kPromptRows + (long long)B;
   const PromptPlan plan = prompt_plan(T, U, q_heads, D, B);
-  LMOE_REQUIRE(tiles * q_heads * plan.chunks < (1ll << 31), LMOE_ESHAPE, "%s: %d rows of %d heads", fn, T, q_heads);
+  LMOE_REQUIRE(tiles * q_heads * plan.chunks <= kMostGroups, LMOE_ESHAPE,
+               "%s: %d rows of %d sequences and %d heads are more than a launch takes", fn, T, B, q_heads);
   LMOE_REQUIRE(plan.bytes == 0 || (workspace && aligned16(workspace) && workspace_bytes >= plan.bytes), LMOE_EWORKSPACE,
                "%s: a 16-byte aligned workspace of %zu bytes is needed", fn, plan.bytes);
   float *part = plan.bytes ? static_cast<float *>(workspace) : nullptr;

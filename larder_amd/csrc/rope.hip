@@ -443,6 +443,7 @@ extern "C" int lmoe_rope_rows(const void *x, int dtype, long long x_row, long lo
   LMOE_REQUIRE(dtype_ok(dtype), LMOE_EINVAL, "%s: dtype %d", fn, dtype);
   LMOE_REQUIRE(T >= 0 && heads > 0 && D > 0 && D <= 1024, LMOE_ESHAPE, "%s: %d rows of %d heads of %d", fn, T, heads, D);
   LMOE_REQUIRE(n_freq >= 0 && 2 * n_freq <= D, LMOE_ESHAPE, "%s: %d pairs in heads of %d", fn, n_freq, D);
+  LMOE_REQUIRE((T + 7ll) / 8 <= kMostGroups, LMOE_ESHAPE, "%s: %d rows are more than a launch takes", fn, T);
   if (T == 0) return 0;
   LMOE_REQUIRE(x && out && positions && (freq || n_freq == 0), LMOE_EINVAL, "%s: null pointer", fn);
   const bool wide = wide_rows(x, x_row, x_head, D, dtype) && wide_rows(out, out_row, out_head, D, dtype) &&
@@ -486,7 +487,8 @@ extern "C" int lmoe_kv_append(const void *q, long long q_row, long long q_head, 
                LMOE_EALIGN, "%s: rows and codes must be 16-byte aligned", fn);
   hipStream_t st = (hipStream_t)stream;
   const long long tasks = (cu ? T / page + 2ll * B : B) * heads * 2;
-  LMOE_REQUIRE(tasks < (1ll << 30), LMOE_ESHAPE, "%s: %d rows of %d sequences and %d heads", fn, T, B, heads);
+  LMOE_REQUIRE(tasks + 1024 + T / 8 <= kMostGroups, LMOE_ESHAPE,
+               "%s: %d rows of %d sequences and %d heads are more than a launch takes", fn, T, B, heads);
   AppendArgs a = {{k, k_row, k_head}, {v, v_row, v_head}, k_codes, v_codes, k_scale, v_scale, table, lens, cu, freq, gain,
                   T, B, heads, D, page, pages, width, n_freq, interleaved, dtype, 0, int(tasks)};
   RopeArgs r = {};
@@ -532,6 +534,8 @@ extern "C" int lmoe_kv_read(const uint8_t *k_codes, const float *k_scale, const 
   LMOE_REQUIRE(dtype_ok(dtype), LMOE_EINVAL, "%s: dtype %d", fn, dtype);
   LMOE_REQUIRE(total >= 0 && B >= 0, LMOE_ESHAPE, "%s: %d rows, %d sequences", fn, total, B);
   if (const int rc = check_cache(fn, heads, D, page, pages, width)) return rc;
+  LMOE_REQUIRE((total + kReadRows - 1ll) / kReadRows <= kMostGroups, LMOE_ESHAPE, "%s: %d rows are more than a launch takes", fn,
+               total);
   if (total == 0) return 0;
   LMOE_REQUIRE(k_codes && k_scale && v_codes && v_scale && (table || B == 0) && (cu || B == 0) && k_out && v_out, LMOE_EINVAL,
                "%s: null pointer", fn);

@@ -8,6 +8,9 @@ namespace lmoe {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+// Workgroups of 256 a launch may have: the runtime cuts a grid of 2^32 threads or more without a word
+constexpr long long kMostGroups = (1ll << 24) - 1;
+
 // The largest b < B with first(cu[b], b) <= t, by one wavefront (-1 if there is none); first never falls with b where cu
 // does not. A load for every factor of 64 in B. Whatever cu holds, the result is in [-1, B); where cu falls, t may lie before what
 // that b begins with, which callers look at before they take it for an index.

@@ -260,6 +260,21 @@ def test_tables_of_places_past_an_int_are_refused(built_lib, page):
         refused(built_lib, _lib.ESHAPE, b"a table of", name, *args)
 
 
+def test_more_than_a_launch_takes_is_refused(built_lib):
+    """Grids of 2^24 workgroups of 256 and more, which the runtime would cut to what is left of them in 32 bits."""
+    def check(name, *args):
+        refused(built_lib, _lib.ESHAPE, b"than a launch takes", name, *args)
+
+    for t in (8 * (2 ** 24 - 1) + 1, 2 ** 31 - 1):
+        check("lmoe_rope_rows", P, 1, 64, 64, P, 0, P, 32, t, 1, 64, 0, 1.0, P, 64, 64)
+    for t, b, cu in ((100, 2 ** 22, P), (2 ** 23, 2 ** 23, None), (2 ** 31 - 1, 1, P)):
+        check("lmoe_kv_append", None, 64, 64, 0, P, 64, 64, P, 64, 64, 1, t, 1, 64, cu, P, b, P, 1, P, P, P, P, 1, 64, P, 0, 0, 1.0,
+              None, None)
+    for total in (16 * (2 ** 24 - 1) + 1, 2 ** 31 - 1):
+        check("lmoe_kv_read", P, P, P, P, 1, 64, 1, 64, P, 1, P, 1, total, P, P, 1)
+    check("lmoe_prompt_attend", P, 64, 64, P, 64, 64, P, 64, 64, 1, 2, 2, 32, 4, 64, P, P, 2 ** 19, 0.1, P, 0, P)
+
+
 @pytest.mark.parametrize("unit,spare", [(32, 2), (64, 2), (128, 2), (128, 1)])
 def test_every_page_and_tile_has_a_workgroup(unit, spare):
     """Sequence b's workgroups begin at cu[b] // unit + spare b. With spare 2 that is room for every page that its rows can
