@@ -206,9 +206,9 @@ def _prompt_workspace(*sizes):
 # ---- the calls -------------------------------------------------------------------------------------------------
 
 def rope_rows(x, positions, freq, interleaved=False, gain=1.0, out=None):
-    """x [T, heads, width] (float16, bfloat16 or float32; width up to 1,024) with the first 2 len(freq) channels of every head rotated by the
-    angles positions[t] * freq (positions int32 or int64 [T], any; freq float64, radians): pairs (i, i + len(freq)), or
-    (2 i, 2 i + 1) where interleaved, multiplied by gain; the other channels as they are. float32 inside, one rounding.
+    """x [T, heads, width] (float16, bfloat16 or float32; width up to 1,024) with the first 2 len(freq) channels of every head
+    rotated by the angles positions[t] * freq (positions int32 or int64 [T], any; freq float64, radians): pairs (i, i + len(freq)),
+    or (2 i, 2 i + 1) where interleaved, multiplied by gain; the other channels as they are. float32 inside, one rounding.
     out: a tensor of x's shape and type, which may be x (and shares no memory with it otherwise); rows of any strides with a
     dense last axis."""
     fn = "rope_rows"
@@ -298,8 +298,8 @@ def attend_rows(q, cache, table, lens, cu=None, most_rows=None, longest=None, sc
     width^-0.5 if None. Made for few rows a sequence: one token of each, or a speculative decoder's draft.
 
     Sums are float32; weights are rounded to float16, times 2^11, so that one keeps all its bits down to 2^-25 of the row's
-    largest (below about 2^-35 it is zero), and the sum that a row is divided by is the rounded weights'. Values from about 2^90 on can
-    overflow the sums.
+    largest (below about 2^-35 it is zero), and the sum that a row is divided by is the rounded weights'. Values from about 2^90
+    on can overflow the sums.
 
     most_rows and longest size the launch: about the most rows of a sequence (1 without cu, else T / sequences) and tokens of
     one (the table's room). Any values give the same sums in another order."""

@@ -27,6 +27,7 @@
 namespace lmoe {
 
 constexpr int kRopeThreads = 256;
+constexpr int kMostWidth = 1 << 30;  // channels of a row, counted in ints
 
 struct Rows {  // [T][heads][D] in place, strides in elements; the last axis is dense
   const void *p;
@@ -441,7 +442,8 @@ extern "C" int lmoe_rope_rows(const void *x, int dtype, long long x_row, long lo
                               float gain, void *out, long long out_row, long long out_head, void *stream) {
   const char *fn = "lmoe_rope_rows";
   LMOE_REQUIRE(dtype_ok(dtype), LMOE_EINVAL, "%s: dtype %d", fn, dtype);
-  LMOE_REQUIRE(T >= 0 && heads > 0 && D > 0 && D <= 1024, LMOE_ESHAPE, "%s: %d rows of %d heads of %d", fn, T, heads, D);
+  LMOE_REQUIRE(T >= 0 && heads > 0 && D > 0 && D <= 1024 && heads <= kMostWidth / D, LMOE_ESHAPE, "%s: %d rows of %d heads of %d", fn,
+               T, heads, D);
   LMOE_REQUIRE(n_freq >= 0 && 2 * n_freq <= D, LMOE_ESHAPE, "%s: %d pairs in heads of %d", fn, n_freq, D);
   LMOE_REQUIRE((T + 7ll) / 8 <= kMostGroups, LMOE_ESHAPE, "%s: %d rows are more than a launch takes", fn, T);
   if (T == 0) return 0;
@@ -476,6 +478,7 @@ extern "C" int lmoe_kv_append(const void *q, long long q_row, long long q_head, 
   LMOE_REQUIRE(T >= 0 && B >= 0 && (!q || q_heads > 0), LMOE_ESHAPE, "%s: %d rows, %d sequences, %d query heads", fn, T, B,
                q_heads);
   if (const int rc = check_cache(fn, heads, D, page, pages, width)) return rc;
+  LMOE_REQUIRE(!q || q_heads <= kMostWidth / D - heads, LMOE_ESHAPE, "%s: %d query heads of %d", fn, q_heads, D);
   LMOE_REQUIRE(n_freq >= 0 && 2 * n_freq <= D && (interleaved ? n_freq % 4 == 0 : n_freq % 8 == 0), LMOE_ESHAPE,
                "%s: %d pairs in heads of %d (multiples of 8, of 4 where interleaved)", fn, n_freq, D);
   if (T == 0 || B == 0) return 0;

@@ -275,6 +275,13 @@ def test_more_than_a_launch_takes_is_refused(built_lib):
     check("lmoe_prompt_attend", P, 64, 64, P, 64, 64, P, 64, 64, 1, 2, 2, 32, 4, 64, P, P, 2 ** 19, 0.1, P, 0, P)
 
 
+@pytest.mark.parametrize("heads", [(1 << 20) + 1, 1 << 24, 2 ** 31 - 1])
+def test_rows_of_more_channels_than_an_int_counts_are_refused(built_lib, heads):
+    refused(built_lib, _lib.ESHAPE, b"heads of 1024", "lmoe_rope_rows", P, 1, 64, 1024, P, 0, P, 32, 2, heads, 1024, 0, 1.0, P, 64, 1024)
+    refused(built_lib, _lib.ESHAPE, b"query heads of 256", "lmoe_kv_append", P, 256, 256, max(heads, 1 << 22), P, 64, 64, P, 64, 64, 1, 2,
+            1, 256, P, P, 1, P, 1, P, P, P, P, 1, 64, P, 0, 0, 1.0, P, None)
+
+
 @pytest.mark.parametrize("unit,spare", [(32, 2), (64, 2), (128, 2), (128, 1)])
 def test_every_page_and_tile_has_a_workgroup(unit, spare):
     """Sequence b's workgroups begin at cu[b] // unit + spare b. With spare 2 that is room for every page that its rows can
