@@ -542,6 +542,44 @@ int lmoe_prompt_attend(const void *q, long long q_row, long long q_head, const v
                        void *stream);
 size_t lmoe_prompt_attend_workspace_bytes(int T, int U, int q_heads, int heads, int D, int B);
 
+/* The pages of the cache as a pool that tables share: refs [pages] int32 counts the places of the tables that hold a page (0: it
+ * is free), table [B][width] int32 has -1 where a sequence has none. All of it is done on the GPU, in an order of its own
+ * definition. No counterpart in the reference, whose sequences have arrays of their own.
+ * lmoe_pages_take: the places that the newest rows (lens, cu as above) fall into become the sequence's own: one
+ * without a page, or whose page has refs > 1, gets the lowest free page, sequence by sequence and place by place, refs 1; the
+ * old page's count falls by one. Where the old page holds tokens before the rows, src[b] and dst[b] [B] are the pair that
+ * lmoe_pages_copy has to copy (else -1, at most one a sequence). Pages are free that have refs 0 when the call begins; places that
+ * find none hold -1, lacking [B] counts them. workspace: lmoe_pages_take_workspace_bytes.
+ * lmoe_pages_free: places from keep[b] [B] tokens on are given back and hold -1.
+ * lmoe_pages_fork: out [n][width] = the rows of table that parents [n] names (outside [0, B): -1); every place of table is given
+ * back and every place of out counted. out does not overlap table.
+ * lmoe_pages_compact: the held pages (refs > 0) past the first `used` (how many are held) numbers move to the free ones among
+ * those, both in order: src and dst [max(pages / 2, 1)] the pairs, -1 behind them; refs follow. to [pages]: the new number
+ * of every page from `used` on, which lmoe_pages_renumber writes into a table's places.
+ * lmoe_pages_copy: codes and scales of src[i] to dst[i] [n]; pairs with a page outside the cache are left out. No page is
+ * in dst twice, or in both lists. */
+size_t lmoe_pages_take_workspace_bytes(int B, int width, int pages);
+int lmoe_pages_take(int *refs, int pages, int *table, int B, int width, const int *lens, const int *cu, int page, int *src, int *dst,
+                    int *lacking, void *workspace, size_t workspace_bytes, void *stream);
+int lmoe_pages_free(int *refs, int pages, int *table, int B, int width, const int *keep, int page, void *stream);
+int lmoe_pages_fork(int *refs, int pages, const int *table, int B, int width, const int *parents, int n, int *out, void *stream);
+int lmoe_pages_compact(int *refs, int pages, int *src, int *dst, int *used, int *to, void *stream);
+int lmoe_pages_renumber(int *table, int B, int width, int pages, const int *used, const int *to, void *stream);
+int lmoe_pages_copy(uint8_t *k_codes, float *k_scale, uint8_t *v_codes, float *v_scale, int pages, int page, int heads, int D,
+                    const int *src, const int *dst, int n, void *stream);
+
+/* Root-mean-square norm of rows x [T][heads][H] (strides in elements between rows and heads, channels dense, any alignment;
+ * heads 1 for whole rows): s = x + residual (optional, in dtype), y = s / sqrt(mean(s^2) + eps) weight[H] (weight in dtype or
+ * float32), float32 inside. out [T][heads][H] dense: y in dtype where group is 0, else e4m3 codes of y / scale with scales
+ * [T][heads][H / group] float32 (group 32, 64, 128, 256 or 512 dividing H, or H): the least power of two >= 2^-100 that brings
+ * the group's largest finite |y| to 448 or less; infinities and NaN are NaN codes. sum (optional, in dtype) gets s. sum may be x
+ * or residual; out may be x where group is 0. The reference's norms are its MLX layers'.
+ * lmoe_read_codes: n codes back, each times its group's scale, rounded once to dtype. */
+int lmoe_norm_rows(const void *x, int dtype, long long x_row, long long x_head, const void *residual, long long r_row,
+                   long long r_head, const void *weight, int wdtype, long long T, int heads, int H, float eps, void *out, int group,
+                   float *scales, void *sum, long long s_row, long long s_head, void *stream);
+int lmoe_read_codes(const uint8_t *codes, const float *scales, long long n, int group, void *out, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

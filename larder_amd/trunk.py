@@ -4,6 +4,8 @@
     qmv_rows(x, w, scales, biases, group_size)               route_cuda.py:525-541 (lmoe_qmv_rows)
     shared_expert_rows(x, gate, up, down)                    mlx_lm's shared_expert MLP on qmv_rows projections
     attention_rows(x, qkv, out, cache, table, lens, ...)     rotary attention on qmv_rows projections and the paged cache
+    norm_rows(x, weight, eps, residual, group, total)        root-mean-square norm, after the residual's addition
+    read_codes(codes, scales, dtype)                         rows that norm_rows gave in 8 bits
 
 qmv_rows gives every row of x the bits of the reference's kernel (MLX 0.32.4's one-row qmv arithmetic: bf16
 weights, bf16 fused multiply-add slots, a float32 slot sum and lane butterfly), reading the weights once a pass.
@@ -13,9 +15,9 @@ bfloat16 [N, K / G].
 import torch
 
 from . import attention
-from ._lib import call, ptr, stream
+from ._lib import call, dcode, ptr, stream
 
-__all__ = ["attention_rows", "qmv_fits", "qmv_rows", "shared_expert_rows"]
+__all__ = ["attention_rows", "norm_rows", "qmv_fits", "qmv_rows", "read_codes", "shared_expert_rows"]
 
 
 def qmv_fits(x, w, scales, group_size, bits, mode, biases):
@@ -105,3 +107,90 @@ def attention_rows(x, qkv, out, cache, table, lens, cu=None, freq=None, interlea
     else:
         o = attention.prompt_rows(q, *attention.read_rows(cache, table, cu_k, total, dtype=x.dtype), cu, cu_k=cu_k)
     return qmv_rows(o.reshape(t, q_heads * width), *out)
+
+
+def _planes(x):
+    """(x, rows, heads, row stride, head stride): x [..., H] as rows of heads, its last axis dense; copied where its leading
+    axes are not two strides."""
+    if x.dim() > 3 or (x.shape[-1] > 1 and x.stride(-1) != 1):
+        x = x.contiguous()
+    if x.dim() == 3:
+        return x, x.shape[0], x.shape[1], x.stride(0), x.stride(1)
+    if x.dim() == 2:
+        return x, x.shape[0], 1, x.stride(0), 0
+    return x, x.numel() // x.shape[-1], 1, x.shape[-1], 0
+
+
+def norm_rows(x, weight, eps=1e-6, residual=None, group=None, total=None):
+    """Root-mean-square norm over the last axis of x [..., H] (float16, bfloat16 or float32; the residual stream, or the heads of
+    q and k before their rotation): with s = x + residual, y = s / sqrt(mean(s^2) + eps) * weight. weight [H] in x's type or
+    float32, residual of x's shape and type. Views with a dense last axis are read as they lie. float32 inside: y is of the sum
+    before that is rounded, and rows whose squares pass float32 (from about 2^64 / sqrt(H) on) keep their values.
+
+    group None: y in x's type. Else y in 8 bits, as (codes float8_e4m3fn, scales float32 [..., H / group]): the scale of `group`
+    neighbouring channels (32, 64, 128, 256 or 512 that divide H, or H itself) is the least power of two (2^-100 or more) that
+    brings their largest finite magnitude to 448 or less, and infinities and NaN are kept as NaN. read_codes gives the rows back.
+    With a residual (or total) the result is followed by s in x's type, rounded once, in total, if that is given: a tensor
+    of x's shape and type with a dense last axis, which may be x or the residual (and shares no memory with them otherwise)."""
+    fn = "norm_rows"
+    if x.dim() == 0 or x.shape[-1] == 0:
+        attention._refuse(fn, "x is [..., channels]")
+    h, shape = x.shape[-1], x.shape
+    dt = dcode(x.dtype)
+    if weight.dim() != 1 or weight.shape[0] != h or weight.dtype not in (x.dtype, torch.float32):
+        attention._refuse(fn, f"weight is [{h}] in x's type or float32, not {weight.dtype} {list(weight.shape)}")
+    if not 0.0 < eps < float("inf"):
+        attention._refuse(fn, f"eps {eps} is not above zero")
+    if residual is not None and (residual.shape != shape or residual.dtype is not x.dtype):
+        attention._refuse(fn, "residual has x's shape and type")
+    if group is not None and group != h and (group not in (32, 64, 128, 256, 512) or h % group):
+        attention._refuse(fn, f"scales of {group} channels in rows of {h} (32, 64, 128, 256 or 512 that divide them, or whole rows)")
+    sums = residual is not None or total is not None
+    if total is None:
+        total = x.new_empty(shape) if sums else None
+    elif total.shape != shape or total.dtype is not x.dtype or (h > 1 and total.stride(-1) != 1) or (
+            total.dim() > 3 and not total.is_contiguous()):
+        attention._refuse(fn, "total has x's shape and type and a dense last axis")
+    dev = attention._device(fn, x, weight, residual, total)
+    weight = weight.contiguous()
+    x, t, heads, x_row, x_head = _planes(x)
+    r_row = r_head = s_row = s_head = 0
+    if residual is not None:
+        residual, _, _, r_row, r_head = _planes(residual)
+    if total is not None:
+        _, _, _, s_row, s_head = _planes(total)
+    scales = None
+    if group is None:
+        out = x.new_empty(shape)
+    else:
+        out = x.new_empty(shape, dtype=torch.float8_e4m3fn)
+        scales = x.new_empty(shape[:-1] + (h // group,), dtype=torch.float32)
+    if t and heads:
+        attention._launch(dev, "lmoe_norm_rows", x.data_ptr(), dt, x_row, x_head, None if residual is None else residual.data_ptr(),
+                          r_row, r_head, weight.data_ptr(), dcode(weight.dtype), t, heads, h, eps, out.data_ptr(), group or 0,
+                          None if scales is None else scales.data_ptr(), None if total is None else total.data_ptr(), s_row, s_head)
+    if group is None:
+        return (out, total) if sums else out
+    return (out, scales, total) if sums else (out, scales)
+
+
+def read_codes(codes, scales, dtype=torch.bfloat16):
+    """Rows in dtype from the 8 bits that norm_rows gave: codes float8_e4m3fn [..., H] times scales float32 [..., H / group], each
+    rounded once (bfloat16 holds them exactly)."""
+    fn = "read_codes"
+    if codes.dtype not in attention._CODES or codes.dim() == 0 or codes.shape[-1] == 0:
+        attention._refuse(fn, "codes are float8_e4m3fn [..., channels]")
+    if scales.dtype is not torch.float32 or scales.dim() != codes.dim() or scales.shape[:-1] != codes.shape[:-1] or (
+            scales.shape[-1] == 0 or codes.shape[-1] % scales.shape[-1]):
+        attention._refuse(fn, f"scales are float32 {list(codes.shape[:-1])} and a divisor of {codes.shape[-1]}, not "
+                              f"{scales.dtype} {list(scales.shape)}")
+    dt = dcode(dtype)
+    dev = attention._device(fn, codes, scales)
+    codes, scales = codes.contiguous(), scales.contiguous()
+    if codes.data_ptr() & 15:
+        codes = codes.clone()
+    out = codes.new_empty(codes.shape, dtype=dtype)
+    if codes.numel():
+        attention._launch(dev, "lmoe_read_codes", codes.data_ptr(), scales.data_ptr(), codes.numel(),
+                          codes.shape[-1] // scales.shape[-1], out.data_ptr(), dt)
+    return out
