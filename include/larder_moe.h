@@ -542,6 +542,16 @@ int lmoe_prompt_attend(const void *q, long long q_row, long long q_head, const v
                        void *stream);
 size_t lmoe_prompt_attend_workspace_bytes(int T, int U, int q_heads, int heads, int D, int B);
 
+/* lmoe_kv_attend's product for chunks of many rows a sequence (lmoe_kv_append's cache, offsets, lengths and tables): row r of a
+ * sequence's n over its first lens - n + r + 1 tokens (none: zero), out [T][q_heads][D] dense. longest: about the most tokens of a
+ * sequence (any value is sound; it sizes the launch). workspace: lmoe_kv_chunk_workspace_bytes of the same numbers (0: none),
+ * 16-byte aligned. The reference runs a later chunk's attention on MLX. */
+size_t lmoe_kv_chunk_workspace_bytes(int T, int q_heads, int heads, int D, int B, int longest);
+int lmoe_kv_chunk(const void *q, int dtype, long long q_row, long long q_head, int T, int q_heads, int heads, int D, const int *cu,
+                  const int *lens, int B, const int *table, int width, const uint8_t *k_codes, const float *k_scale,
+                  const uint8_t *v_codes, const float *v_scale, int pages, int page, int longest, float scale, void *workspace,
+                  size_t workspace_bytes, void *out, void *stream);
+
 /* The pages of the cache as a pool that tables share: refs [pages] int32 counts the places of the tables that hold a page (0: it
  * is free), table [B][width] int32 has -1 where a sequence has none. All of it is done on the GPU, in an order of its own
  * definition. No counterpart in the reference, whose sequences have arrays of their own.

@@ -115,6 +115,8 @@ SIGNATURES = {
     "lmoe_prompt_attend": (_I, [_P, _LL, _LL, _P, _LL, _LL, _P, _LL, _LL, _I, _I, _I, _I, _I, _I, _P, _P, _I, _F, _P, _SZ, _P,
                                 _P]),
     "lmoe_prompt_attend_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I]),
+    "lmoe_kv_chunk_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I]),
+    "lmoe_kv_chunk": (_I, [_P, _I, _LL, _LL, _I, _I, _I, _I, _P, _P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _F, _P, _SZ, _P, _P]),
     "lmoe_norm_rows": (_I, [_P, _I, _LL, _LL, _P, _LL, _LL, _P, _I, _LL, _I, _I, _F, _P, _I, _P, _P, _LL, _LL, _P]),
     "lmoe_read_codes": (_I, [_P, _P, _LL, _I, _P, _I, _P]),
     "lmoe_pages_take_workspace_bytes": (_SZ, [_I, _I, _I]),

@@ -8,6 +8,7 @@ GPU.
     append_rows(cache, q, k, v, table, lens, ...) rotates q and k and writes the rows' keys and values into their pages
     read_rows(cache, table, cu, total)            the first tokens of each sequence back in 16 (or 32) bits
     attend_rows(q, cache, table, lens, ...)       the newest rows of each sequence over its cached tokens
+    chunk_rows(q, cache, table, lens, cu, ...)    many new rows of each sequence over its cached tokens, causal
     prompt_rows(q, k, v, cu, ...)                 packed sequences, causal, over their own keys and values
 
 Rows are packed: tensors [T, heads, width] hold the sequences one after the other, and cu int32 [sequences + 1] says where
@@ -18,7 +19,7 @@ the GPU, and the host does not see them: wrong ones give rows and pages of no me
 
 lens int32 [sequences] counts a sequence's tokens with the rows of the call among them: row r of n stands at place lens -
 n + r. table int32 [sequences, width] lists each sequence's pages in order; entries behind its last page are not read. A
-page outside the cache (or the table) holds nothing: no token is written there and attend_rows sees none. read_rows gives its
+page outside the cache (or the table) holds nothing: no token is written there, attend_rows and chunk_rows see none. read_rows gives its
 tokens back as zeros, which prompt_rows would see as any others: a history with such holes is read through a table, and with
 offsets, that leave them out (the rows see the keys that are left, as attend_rows has them). Sequences may share pages they
 only read; a page that a call writes to stands in one place of one table. A row that sees no token, or only tokens that score
@@ -33,7 +34,7 @@ import torch
 from . import _lib
 from ._lib import call, dcode, stream
 
-__all__ = ["KVCache", "append_rows", "attend_rows", "prompt_rows", "read_rows", "rope_rows", "rotary_freq"]
+__all__ = ["KVCache", "append_rows", "attend_rows", "chunk_rows", "prompt_rows", "read_rows", "rope_rows", "rotary_freq"]
 
 
 class KVCache(NamedTuple):
@@ -199,6 +200,11 @@ def _attend_workspace(*sizes):
 
 
 @functools.lru_cache(maxsize=1024)
+def _chunk_workspace(*sizes):
+    return _lib.lib().lmoe_kv_chunk_workspace_bytes(*sizes)
+
+
+@functools.lru_cache(maxsize=1024)
 def _prompt_workspace(*sizes):
     return _lib.lib().lmoe_prompt_attend_workspace_bytes(*sizes)
 
@@ -323,6 +329,42 @@ def attend_rows(q, cache, table, lens, cu=None, most_rows=None, longest=None, sc
     ws = q.new_empty(need, dtype=torch.uint8) if need else None
     _launch(dev, "lmoe_kv_attend", q.data_ptr(), dcode(dtype), q_row, q_head, t, q_heads, heads, width,
             None if cu is None else cu.data_ptr(), lens.data_ptr(), n, table.data_ptr(), room, *codes, pages, page, most, long,
+            width ** -0.5 if scale is None else scale, None if ws is None else ws.data_ptr(), need, out.data_ptr())
+    return out
+
+
+def chunk_rows(q, cache, table, lens, cu=None, longest=None, scale=None):
+    """softmax(scale q k^T) v of chunks of new rows q [T, query heads, width] (float16 or bfloat16) over the cached tokens of
+    their sequences, causal: row r of a sequence's n sees its first lens - n + r + 1 tokens (a row that sees none is zero), as
+    attend_rows has it, made for many rows a sequence: a later chunk of a prompt, a message after a long history, a tree of
+    drafts. The pages are read as they lie, the chunk's own keys and values among them in the cache's 8 bits. scale is width^-0.5
+    if None.
+
+    Sums are float32; weights are rounded to q's type for their product with the values, and the sum that a row is divided by
+    is the rounded weights', as in prompt_rows. Keys and values keep all their bits (float16: as long as no page's scale is
+    2^22 times that of the page beside it). A value that is NaN makes its channel NaN in the rows that see it, and touches no other.
+
+    longest sizes the launch: about the most tokens of a sequence (the table's room). Any value gives the same sums in another
+    order."""
+    fn = "chunk_rows"
+    pages, heads, page, width, *codes = _cache(fn, cache)
+    q, q_row, q_head = _rows(fn, "q", q, None, width)
+    t, q_heads, _ = q.shape
+    dtype = q.dtype
+    if dtype not in _HALVES:
+        _refuse(fn, f"q is float16 or bfloat16, not {dtype}")
+    if q_heads == 0 or heads == 0 or q_heads % heads:
+        _refuse(fn, f"{q_heads} query heads over {heads} key heads")
+    cu, lens, table, n, room = _sequences(fn, cu, lens, table, t)
+    dev = _device(fn, q, table, lens, cu, *cache)
+    out = q.new_empty((t, q_heads, width))
+    if not t or not n:
+        return out.zero_()
+    long = room * page if longest is None else max(1, min(int(longest), room * page))
+    need = _chunk_workspace(t, q_heads, heads, width, n, long)
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
+    _launch(dev, "lmoe_kv_chunk", q.data_ptr(), dcode(dtype), q_row, q_head, t, q_heads, heads, width,
+            None if cu is None else cu.data_ptr(), lens.data_ptr(), n, table.data_ptr(), room, *codes, pages, page, long,
             width ** -0.5 if scale is None else scale, None if ws is None else ws.data_ptr(), need, out.data_ptr())
     return out
 

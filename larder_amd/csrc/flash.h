@@ -1,0 +1,153 @@
+// What the attention of many rows at a time shares (prompt.hip: over keys in 16 bits; chunk.hip: over the paged cache): matrix
+// products of 32 rows, the layout of keys and values in LDS, weights in 16 bits, values that are not finite, and the joining of
+// rows whose keys were worked in chunks.
+#pragma once
+#include "rows.h"
+
+namespace lmoe {
+
+constexpr int kPromptKeys = 64;  // keys a tile
+
+// A weight is 2^(score - maximum in use + kLift), the maximum lagging at most kLag: float16 weights reach 2^15 at most, and
+// one 2^-25 of the largest is still a normal number
+template <bool BF>
+constexpr float kLift = BF ? 0.0f : 11.0f;
+template <bool BF>
+constexpr float kLag = BF ? 8.0f : 4.0f;
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+template <bool BF>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+
+// 16-byte chunk c of key row r (rows of D / 8 chunks): eight, or sixteen, rows' same chunk lie in different banks
+template <int D>
+__device__ __forceinline__ int k_chunk(int r, int c) {
+  return D == 64 ? c ^ ((r >> 1) & 7) : c ^ (r & 15);
+}
+// 32-byte chunk pair p of value row r: what 32 lanes of a transposing load take (two neighbouring pairs of four rows) lies in
+// different banks
+template <int D>
+__device__ __forceinline__ int v_pair(int r, int p) {
+  return D == 64 ? p ^ (r & 2) : p ^ ((r & 3) << 1) ^ ((r >> 2) & 1);
+}
+
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (BF) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, bf16x2));
+  } else {
+    return __builtin_bit_cast(uint32_t, h2_t{_Float16(a), _Float16(b)});
+  }
+}
+// a + the pair's two values
+template <bool BF>
+__device__ __forceinline__ float add2(uint32_t pair, float a) {
+  if constexpr (BF)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), __builtin_bit_cast(bf16x2, 0x3f803f80u), a, false);
+  else
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2_t, pair), h2_t{1.0f, 1.0f}, a, false);
+}
+
+// Whether a thread's share of a tile's values holds one that is not finite. In LDS order: looked at by key and channel, as
+// take_bad does, 18 prompts of 512 rows take 112 us instead of 107.6 (16 heads of 256)
+template <int D, bool BF>
+__device__ __forceinline__ bool any_bad(const uint8_t *vt) {
+  constexpr uint32_t INF = BF ? 0x7f80u : 0x7c00u;
+  uint32_t over = 0;
+#pragma unroll
+  for (int i = 0; i < kPromptKeys * D / 8 / 256; ++i) {  // a half word's magnitude of INF or more carries into its sign bit
+    const u32x4 w = reinterpret_cast<const u32x4 *>(vt)[i * 256 + threadIdx.x];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) over |= (w[e] & 0x7fff7fffu) + (0x8000u - INF) * 0x10001u;
+  }
+  return over & 0x80008000u;
+}
+
+// Values that are not finite in a tile that some row does not see whole: one thread a key and 32 channels. They are set to zero
+// in LDS and noted in two words of bits, pos (NaN, +inf) and neg (NaN, -inf).
+template <int D, bool BF>
+__device__ __forceinline__ void take_bad(uint8_t *vt, int row, int c32, uint32_t *pos, uint32_t *neg) {
+  constexpr uint32_t INF = BF ? 0x7f80u : 0x7c00u;
+  uint32_t up = 0, down = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    u32x4 *at = reinterpret_cast<u32x4 *>(vt + row * D * 2 + v_pair<D>(row, 2 * c32 + (j >> 1)) * 32 + (j & 1) * 16);
+    u32x4 w = *at;
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t x = (w[e >> 1] >> (16 * (e & 1))) & 0xffffu, mag = x & 0x7fffu;
+      if (mag >= INF) {
+        const bool nan = mag > INF, minus = x >> 15;
+        any = true;
+        if (nan || !minus) up |= 1u << (8 * j + e);
+        if (nan || minus) down |= 1u << (8 * j + e);
+        w[e >> 1] &= ~(0xffffu << (16 * (e & 1)));
+      }
+    }
+    if (any) *at = w;
+  }
+  *pos = up;
+  *neg = down;
+}
+
+// Whether every output product's weights are packed a slot before it: NM score products, NV output products over NP pairs of
+// weights, DT channel tiles, pairs spread over NS slots and packed one slot later
+constexpr bool weights_in_time(int NM, int NV, int NP, int DT, int NS) {
+  for (int k = 0; k < NV; ++k) {
+    const int slots = NM + k - 1 < NS ? NM + k - 1 : NS;
+    if (slots * NP / NS < 4 * (k / DT + 1)) return false;
+  }
+  return true;
+}
+
+// Rows whose keys were worked in more than one chunk: D / 4 threads a row and head, the chunks joined in order
+struct JoinArgs {
+  uint16_t *out;
+  const float *part;  // [chunks][T][q_heads] of [D] sums and {maximum, weight}
+  const int *joins;   // [T][q_heads]: how many chunks (0: the row is done)
+  int T, q_heads, chunks;
+};
+template <int D, bool BF>
+static __global__ void __launch_bounds__(256) k_join_chunks(JoinArgs a) {
+  constexpr int LANES = D / 4;
+  const size_t line = size_t(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES, lines = size_t(a.T) * a.q_heads;
+  if (line >= lines) return;
+  const int parts = min(a.joins[line], a.chunks), d = (threadIdx.x % LANES) * 4;
+  if (parts < 2) return;
+  f32x4 v = {};
+  float top = -INFINITY, weight = 0.0f;
+  for (int c0 = 0; c0 < parts; c0 += 4) {
+    float2 ml[4];
+    f32x4 y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float *part = a.part + (size_t(min(c0 + j, parts - 1)) * lines + line) * (D + 4);
+      ml[j] = *reinterpret_cast<const float2 *>(part + D);
+      y[j] = *reinterpret_cast<const f32x4 *>(part + d);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (c0 + j >= parts || ml[j].y == 0.0f) continue;  // (a chunk that the row sees nothing of weighs 0; NaN goes on)
+      const float to = fmaxf(top, ml[j].x), f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml[j].x - to);
+      const float keep = weight == 0.0f ? 0.0f : to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - to);
+      top = to;
+      weight = fmaf(ml[j].y, f, weight * keep);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = fmaf(y[j][e], f, v[e] * keep);
+    }
+  }
+  const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
+  *reinterpret_cast<u32x2 *>(a.out + line * D + d) = u32x2{pack2<BF>(v[0] * inv, v[1] * inv), pack2<BF>(v[2] * inv, v[3] * inv)};
+}
+
+}  // namespace lmoe

@@ -23,11 +23,11 @@
 //
 // Values that a row must not see are multiplied by a weight of zero; where one is not finite in a tile that some row does
 // not see whole, it is taken out and given to the rows that do see it alone.
-#include "rows.h"
+#include "flash.h"
 
 namespace lmoe {
 
-constexpr int kPromptRows = 128, kPromptKeys = 64;  // a workgroup's rows, and keys a tile
+constexpr int kPromptRows = 128;  // a workgroup's rows
 constexpr int kAhead = 3;  // products that a fragment is read ahead of its own
 
 struct PromptArgs {
@@ -41,46 +41,6 @@ struct PromptArgs {
   int T, U, B, q_heads, heads, tiles, chunk, chunks;  // chunk: keys, the last of `chunks` goes on to the end
 };
 
-// A weight is 2^(score - maximum in use + kLift), the maximum lagging at most kLag: float16 weights reach 2^15 at most, and
-// one 2^-25 of the largest is still a normal number
-template <bool BF>
-constexpr float kLift = BF ? 0.0f : 11.0f;
-template <bool BF>
-constexpr float kLag = BF ? 8.0f : 4.0f;
-
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-
-template <bool BF>
-__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
-  if constexpr (BF)
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
-}
-
-// 16-byte chunk c of key row r (rows of D / 8 chunks): eight, or sixteen, rows' same chunk lie in different banks
-template <int D>
-__device__ __forceinline__ int k_chunk(int r, int c) {
-  return D == 64 ? c ^ ((r >> 1) & 7) : c ^ (r & 15);
-}
-// 32-byte chunk pair p of value row r: what 32 lanes of a transposing load take (two neighbouring pairs of four rows) lies in
-// different banks
-template <int D>
-__device__ __forceinline__ int v_pair(int r, int p) {
-  return D == 64 ? p ^ (r & 2) : p ^ ((r & 3) << 1) ^ ((r >> 2) & 1);
-}
-
-template <bool BF>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (BF) {
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, bf16x2));
-  } else {
-    return __builtin_bit_cast(uint32_t, h2_t{_Float16(a), _Float16(b)});
-  }
-}
 // One wavefront-wide copy of 16 bytes a lane, from voff in what the descriptor covers, to LDS address lds + 16 lane
 __device__ __forceinline__ void dma_rows(u32x4 rows, uint32_t voff, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rows), "s"(lds) : "memory");
@@ -89,68 +49,6 @@ __device__ __forceinline__ void dma_rows(u32x4 rows, uint32_t voff, uint32_t lds
 // The same from an address of each lane's own
 __device__ __forceinline__ void dma_lanes(const void *from, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds) : "memory");
-}
-
-// a + the pair's two values
-template <bool BF>
-__device__ __forceinline__ float add2(uint32_t pair, float a) {
-  if constexpr (BF)
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), __builtin_bit_cast(bf16x2, 0x3f803f80u), a, false);
-  else
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2_t, pair), h2_t{1.0f, 1.0f}, a, false);
-}
-
-// Whether a thread's share of a tile's values holds one that is not finite. In LDS order: looked at by key and channel, as
-// take_bad does, 18 prompts of 512 rows take 112 us instead of 107.6 (16 heads of 256)
-template <int D, bool BF>
-__device__ __forceinline__ bool any_bad(const uint8_t *vt) {
-  constexpr uint32_t INF = BF ? 0x7f80u : 0x7c00u;
-  uint32_t over = 0;
-#pragma unroll
-  for (int i = 0; i < kPromptKeys * D / 8 / 256; ++i) {  // a half word's magnitude of INF or more carries into its sign bit
-    const u32x4 w = reinterpret_cast<const u32x4 *>(vt)[i * 256 + threadIdx.x];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) over |= (w[e] & 0x7fff7fffu) + (0x8000u - INF) * 0x10001u;
-  }
-  return over & 0x80008000u;
-}
-
-// Values that are not finite in a tile that some row does not see whole: one thread a key and 32 channels. They are set to zero
-// in LDS and noted in two words of bits, pos (NaN, +inf) and neg (NaN, -inf).
-template <int D, bool BF>
-__device__ __forceinline__ void take_bad(uint8_t *vt, int row, int c32, uint32_t *pos, uint32_t *neg) {
-  constexpr uint32_t INF = BF ? 0x7f80u : 0x7c00u;
-  uint32_t up = 0, down = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    u32x4 *at = reinterpret_cast<u32x4 *>(vt + row * D * 2 + v_pair<D>(row, 2 * c32 + (j >> 1)) * 32 + (j & 1) * 16);
-    u32x4 w = *at;
-    bool any = false;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t x = (w[e >> 1] >> (16 * (e & 1))) & 0xffffu, mag = x & 0x7fffu;
-      if (mag >= INF) {
-        const bool nan = mag > INF, minus = x >> 15;
-        any = true;
-        if (nan || !minus) up |= 1u << (8 * j + e);
-        if (nan || minus) down |= 1u << (8 * j + e);
-        w[e >> 1] &= ~(0xffffu << (16 * (e & 1)));
-      }
-    }
-    if (any) *at = w;
-  }
-  *pos = up;
-  *neg = down;
-}
-
-// Whether every output product's weights are packed a slot before it: NM score products, NV output products over NP pairs of
-// weights, DT channel tiles, pairs spread over NS slots and packed one slot later
-constexpr bool weights_in_time(int NM, int NV, int NP, int DT, int NS) {
-  for (int k = 0; k < NV; ++k) {
-    const int slots = NM + k - 1 < NS ? NM + k - 1 : NS;
-    if (slots * NP / NS < 4 * (k / DT + 1)) return false;
-  }
-  return true;
 }
 
 // The nth tile of rows that is worked, by one wavefront. Up to 64 sequences: the tiles furthest into their sequences first,
@@ -488,40 +386,6 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_prompt(PromptArgs a) 
   }
 }
 
-// Rows whose keys were worked in more than one chunk: D / 4 threads a row and head, the chunks joined in order
-template <int D, bool BF>
-__global__ void __launch_bounds__(256) k_prompt_join(PromptArgs a) {
-  constexpr int LANES = D / 4;
-  const size_t line = size_t(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES, lines = size_t(a.T) * a.q_heads;
-  if (line >= lines) return;
-  const int parts = min(a.joins[line], a.chunks), d = (threadIdx.x % LANES) * 4;
-  if (parts < 2) return;
-  f32x4 v = {};
-  float top = -INFINITY, weight = 0.0f;
-  for (int c0 = 0; c0 < parts; c0 += 4) {
-    float2 ml[4];
-    f32x4 y[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float *part = a.part + (size_t(min(c0 + j, parts - 1)) * lines + line) * (D + 4);
-      ml[j] = *reinterpret_cast<const float2 *>(part + D);
-      y[j] = *reinterpret_cast<const f32x4 *>(part + d);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (c0 + j >= parts || ml[j].y == 0.0f) continue;  // (a chunk that the row sees nothing of weighs 0; NaN goes on)
-      const float to = fmaxf(top, ml[j].x), f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml[j].x - to);
-      const float keep = weight == 0.0f ? 0.0f : to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - to);
-      top = to;
-      weight = fmaf(ml[j].y, f, weight * keep);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = fmaf(y[j][e], f, v[e] * keep);
-    }
-  }
-  const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
-  *reinterpret_cast<u32x2 *>(a.out + line * D + d) = u32x2{pack2<BF>(v[0] * inv, v[1] * inv), pack2<BF>(v[2] * inv, v[3] * inv)};
-}
-
 // Chunks of keys, where the rows alone would leave half of the GPU's places idle (two workgroups a CU, one at width 256): as many
 // as fit the places, of 512 keys (eight tiles) at least. Rows' tiles are bounded by T / 128 + B, one more a sequence than there
 // are where rows fill their tiles: one sequence's 1,024 rows over 8,024 keys are 448 workgroups on 512 places with 28 heads of
@@ -592,13 +456,14 @@ extern "C" int lmoe_prompt_attend(const void *q, long long q_row, long long q_he
     launch(kernel, dim3(unsigned(tiles * q_heads * plan.chunks)), dim3(256), lds, (hipStream_t)stream, a);
     LMOE_LAUNCHED(fn);
     if (part) {
-      launch(join, dim3(unsigned(((long long)T * q_heads * (D / 4) + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a);
+      launch(join, dim3(unsigned(((long long)T * q_heads * (D / 4) + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
+             JoinArgs{a.out, part, joins, T, q_heads, plan.chunks});
       LMOE_LAUNCHED(fn);
     }
     return 0;
   };
   const bool bf = dtype == LMOE_BF16;
-  if (D == 64) return bf ? go(k_prompt<64, true>, k_prompt_join<64, true>) : go(k_prompt<64, false>, k_prompt_join<64, false>);
-  if (D == 128) return bf ? go(k_prompt<128, true>, k_prompt_join<128, true>) : go(k_prompt<128, false>, k_prompt_join<128, false>);
-  return bf ? go(k_prompt<256, true>, k_prompt_join<256, true>) : go(k_prompt<256, false>, k_prompt_join<256, false>);
+  if (D == 64) return bf ? go(k_prompt<64, true>, k_join_chunks<64, true>) : go(k_prompt<64, false>, k_join_chunks<64, false>);
+  if (D == 128) return bf ? go(k_prompt<128, true>, k_join_chunks<128, true>) : go(k_prompt<128, false>, k_join_chunks<128, false>);
+  return bf ? go(k_prompt<256, true>, k_join_chunks<256, true>) : go(k_prompt<256, false>, k_join_chunks<256, false>);
 }
