@@ -11,6 +11,7 @@
 // moves, and the sums with it, when a page's scale leaves 2^-15 .. 2^7 of it, so that the conversion stays exact.
 //
 // Products, weights, sums and values that are not finite: as in prompt.hip.
+#include <cmath>
 #include "flash.h"
 
 namespace lmoe {
@@ -96,24 +97,19 @@ __device__ __forceinline__ ChunkTile nth_chunk_tile(const ChunkArgs &a, int nth)
   return w;
 }
 
-// 16 codes times a power of two as 16-bit floats
+// Eight codes times a power of two as 16-bit floats
 template <bool BF>
-__device__ __forceinline__ void widen(u32x4 w, float scale, u32x4 &lo, u32x4 &hi) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    uint32_t a, b;
-    if constexpr (BF) {
-      a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[e], scale, false));
-      b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[e], scale, true));
-    } else {
-      a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[e], scale, false));
-      b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[e], scale, true));
-    }
-    if (e < 2)
-      lo[2 * e] = a, lo[2 * e + 1] = b;
-    else
-      hi[2 * e - 4] = a, hi[2 * e - 3] = b;
-  }
+__device__ __forceinline__ u32x4 widen8(uint32_t a, uint32_t b, float scale) {
+  if constexpr (BF)
+    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, true)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, true))};
+  else
+    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, scale, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, scale, true)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, scale, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, scale, true))};
 }
 
 // The codes of half a tile (32 tokens of a page's head): rows past `rows` read as zeros
@@ -122,23 +118,40 @@ __device__ __forceinline__ u32x4 load_rows(const uint8_t *from, int bytes, int a
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0));
 }
 
-template <int D, bool BF>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_chunk_rows(ChunkArgs a) {
-  constexpr int ROWS = 128, BN = kPromptKeys, KS = D / 16, DT = D / 32, COPIES = D / 64;
+constexpr int kAhead = 3;  // fragments that are read ahead of their products
+
+// Whether every output product's weights are packed a slot before it: NM score products, NV output products, of which each 16 keys
+// take `per`, over NP pairs of weights (four for 16 keys), spread over NS slots and packed one slot later
+constexpr bool weights_in_time(int NM, int NV, int NP, int per, int NS) {
+  for (int k = 0; k < NV; ++k) {
+    const int slots = NM + k - 1 < NS ? NM + k - 1 : NS;
+    if (slots * NP / NS < 4 * (k / per + 1)) return false;
+  }
+  return true;
+}
+
+// NW wavefronts of 32 pairs
+template <int D, bool BF, int NW>
+__global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) k_chunk_rows(ChunkArgs a) {
+  constexpr int ROWS = 32 * NW, THREADS = 64 * NW, BN = kPromptKeys, KS = D / 16, DT = D / 32;
+  constexpr int COPIES = D / (16 * NW), COPY_ROWS = 1024 * NW / D;  // 16 codes a thread
   constexpr int kTileBytes = BN * D * 2;
-  extern __shared__ uint8_t lds[];  // [2 stages][K tile, V tile]
+  extern __shared__ uint8_t lds[];  // [2 stages] of keys, [2 stages] of values
   __shared__ uint32_t marks[2 * BN * DT];  // of take_bad: [pos, neg][key][32 channels]
-  __shared__ uint32_t flags[4];            // of any_bad: a wavefront's
+  __shared__ uint32_t flags[NW];           // of any_bad: a wavefront's
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
-  const int kv = blockIdx.x % a.heads, chunk = int(blockIdx.x) / a.heads % a.chunks;
-  const ChunkTile work = nth_chunk_tile<ROWS>(a, int(blockIdx.x) / (a.heads * a.chunks));
+  // chunk by chunk: XCDs take workgroups in turn, and a chunk's ones, of which short sequences have none, are spread over all
+  const int kv = blockIdx.x % a.heads, chunk = int(blockIdx.x) / a.heads / a.tiles;
+  ChunkTile work = nth_chunk_tile<ROWS>(a, int(blockIdx.x) / a.heads % a.tiles);
+  work = {__builtin_amdgcn_readfirstlane(work.b), __builtin_amdgcn_readfirstlane(work.tile), __builtin_amdgcn_readfirstlane(work.row0),
+          __builtin_amdgcn_readfirstlane(work.n), __builtin_amdgcn_readfirstlane(work.len)};
   const int b = work.b, n = work.n, group = a.group;
   if (b < 0) return;
   if (work.tile == 0 && chunk == 0 && a.cu && (b == 0 || b == a.B - 1)) {
     // rows before the first sequence or behind the last one come back zero
     const int lo = b == 0 ? min(max(a.cu[0], 0), a.T) : 0, hi = b == a.B - 1 ? min(max(a.cu[a.B], 0), a.T) : a.T;
     const int per = group * (D / 8);
-    for (long long i = tid; i < (long long)(lo + (a.T - hi)) * per; i += 256) {
+    for (long long i = tid; i < (long long)(lo + (a.T - hi)) * per; i += THREADS) {
       const int row = int(i / per), c = int(i - (long long)row * per);
       const size_t line = size_t(row < lo ? row : hi + row - lo) * a.q_heads + kv * group + c / (D / 8);
       *reinterpret_cast<u32x4 *>(a.out + line * D + (c % (D / 8)) * 8) = u32x4{};
@@ -154,21 +167,22 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_chunk_rows(ChunkArgs 
   if (chunk > 0 && begin >= most_keys) return;
   const int keys = chunk + 1 < a.chunks ? min(most_keys, begin + a.chunk) : most_keys;
   const int parts = a.part ? min(a.chunks, (most_keys - 1) / a.chunk + 1) : 1;  // chunks that the tile's keys take
-  const int flat = min(first + 32 * wave + r, pairs - 1), mine = flat / group, sees = min(mine + off + 1, room);
-  const int all = min(off + (first + 32 * wave) / group + 1, room);  // what every row of the wavefront sees
+  const int own = first + 32 * wave;  // the wavefront's first pair
+  const int all = min(off + min(own, pairs - 1) / group + 1, room);  // what every row of the wavefront sees
   const int all_rows = min(off + first / group + 1, room);           // and of the workgroup
-
+  const int flat = min(own + r, pairs - 1), mine = flat / group, sees = min(mine + off + 1, room);
   u32x4 qf[KS];
   {
     const uint16_t *q = a.q + size_t(work.row0 + mine) * a.q_row + size_t(kv * group + flat - mine * group) * a.q_head + 8 * h;
 #pragma unroll
     for (int j = 0; j < KS; ++j) qf[j] = *reinterpret_cast<const u32x4 *>(q + 16 * j);
   }
-  // pages and scales of the halves of 64 tiles, a tile a lane
+  // pages and scales of the halves of 64 tiles from `base` on, a tile a lane
   const int tiles = keys > begin ? (keys - begin + BN - 1) / BN : 0;
-  int number[2];
+  int base = 0, number[2];
   float k_scale[2], v_scale[2];
   auto look_up = [&](int t0) {
+    base = t0;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       number[x] = -1, k_scale[x] = 1.0f, v_scale[x] = 0.0f;
@@ -183,26 +197,33 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_chunk_rows(ChunkArgs 
       }
     }
   };
+  // Tiles of keys are shifted by half a tile against those of values: tile T of keys are the halves 2 T - 1 and 2 T, so that
+  // the scores of the next 32 keys are always to be had beside the values of the present 32
   const int page_tokens = 1 << a.page_shift;
+  const uint32_t page_bytes = uint32_t(a.heads) * uint32_t(page_tokens * D);
+  const uint8_t *const kc = a.kc + uint32_t(kv) * uint32_t(page_tokens * D), *const vc = a.vc + uint32_t(kv) * uint32_t(page_tokens * D);
   u32x4 kr[COPIES], vr[COPIES];
-  auto fetch = [&](int t) {  // tile t's codes to registers
-#pragma unroll
-    for (int i = 0; i < COPIES; ++i) {
-      const int row0 = (i * 256 + 64 * wave) / (D / 16), x = row0 >> 5;  // (the wavefront's rows of a copy are in one half)
-      const int page = x ? __builtin_amdgcn_readlane(number[1], t & 63) : __builtin_amdgcn_readlane(number[0], t & 63);
-      const int token = begin + t * BN + 32 * x, rows = page < 0 ? 0 : min(32, max(0, most_keys - token));
-      const size_t at = ((size_t(max(page, 0)) * a.heads + kv) * page_tokens + (token & (page_tokens - 1))) * D;
-      const int j = i * 256 + tid, voff = (j / (D / 16) & 31) * D + j % (D / 16) * 16;
-      kr[i] = load_rows(a.kc + at, rows * D, voff);
-      vr[i] = load_rows(a.vc + at, rows * D, voff);
-    }
+  const int crow = tid / (D / 16), cchunk = tid % (D / 16);  // the thread's row and 16 codes of copy 0; copy i is i COPY_ROWS on
+  // (the wavefront's rows of a copy are in one half)
+  auto half_of = [&](int i) { return COPY_ROWS == 64 ? wave / (NW / 2) : i * COPY_ROWS >> 5; };
+  auto rows_at = [&](const uint8_t *codes, int t, int x, int voff) {  // 16 codes of half x of tile t
+    const int found = __builtin_amdgcn_readlane(x ? number[1] : number[0], (t - base) & 63), page = t < 0 ? -1 : found;
+    const int token = begin + t * BN + 32 * x, rows = __builtin_amdgcn_readfirstlane(min(32, max(0, most_keys - token)));
+    const uint64_t at = uint64_t(uint32_t(max(page, 0))) * page_bytes + uint32_t((token & (page_tokens - 1)) * D);
+    return load_rows(codes + at, page < 0 ? 0 : rows * D, voff);
   };
-  float ref = BF ? 1.0f : 0.0f;  // float16: values in LDS are in units of it
-  // tile t from registers to LDS; the factor that brings the sums to the tile's reference
-  auto store = [&](int t, int stage) {
-    float vs[2] = {lane_value(v_scale[0], t & 63), lane_value(v_scale[1], t & 63)}, move = 1.0f;
+  const int voff = (crow & 31) * D + cchunk * 16;
+  auto fetch_k = [&](int T, int i) {
+    kr[i] = rows_at(kc, half_of(i) ? T : T - 1, half_of(i) ^ 1, voff + (i * COPY_ROWS & 31) * D);
+  };
+  auto fetch_v = [&](int t, int i) { vr[i] = rows_at(vc, t, half_of(i), voff + (i * COPY_ROWS & 31) * D); };
+  float ref = BF ? 1.0f : 0.0f, vs[2], move = 1.0f;  // float16: values in LDS are in units of ref
+  // the factors that tile t's codes of values take, and the one that brings the sums to its reference
+  auto scales_of = [&](int t) {
+    vs[0] = lane_value(v_scale[0], (t - base) & 63), vs[1] = lane_value(v_scale[1], (t - base) & 63);
     if constexpr (!BF) {
       const float big = fmaxf(vs[0], vs[1]), small = vs[0] == 0.0f ? vs[1] : vs[1] == 0.0f ? vs[0] : fminf(vs[0], vs[1]);
+      move = 1.0f;
       if (big > 0.0f && (big > ref * 0x1p7f || small < ref * 0x1p-15f)) {
         const float to = fmaxf(big, 0x1p-40f);  // (2^-40 448 is nothing in float16)
         move = ref == 0.0f ? 1.0f : fminf(ref / to, 0x1p120f);
@@ -210,110 +231,178 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_chunk_rows(ChunkArgs 
       }
       if (ref != 0.0f) vs[0] /= ref, vs[1] /= ref;
     }
-    uint8_t *kt = lds + stage * kTileBytes, *vt = lds + (2 + stage) * kTileBytes;
-#pragma unroll
-    for (int i = 0; i < COPIES; ++i) {
-      const int j = i * 256 + tid, row = j / (D / 16), c = j % (D / 16);
-      const int x = (i * 256 + 64 * wave) / (D / 16) >> 5;
-      u32x4 lo, hi;
-      widen<BF>(kr[i], 1.0f, lo, hi);
-      *reinterpret_cast<u32x4 *>(kt + row * D * 2 + k_chunk<D>(row, 2 * c) * 16) = lo;
-      *reinterpret_cast<u32x4 *>(kt + row * D * 2 + k_chunk<D>(row, 2 * c + 1) * 16) = hi;
-      widen<BF>(vr[i], vs[x], lo, hi);
-      u32x4 *to = reinterpret_cast<u32x4 *>(vt + row * D * 2 + v_pair<D>(row, c) * 32);
-      to[0] = lo, to[1] = hi;
-    }
-    return move;
   };
+  uint8_t *const k_lds = lds, *const v_lds = lds + 2 * kTileBytes;
+  auto store_k = [&](int stage, int i, int part) {
+    const int row = i * COPY_ROWS + crow;
+    *reinterpret_cast<u32x4 *>(k_lds + stage * kTileBytes + row * D * 2 + k_chunk<D>(crow, 2 * cchunk + part) * 16) =
+        widen8<BF>(kr[i][2 * part], kr[i][2 * part + 1], 1.0f);
+  };
+  auto store_v = [&](int stage, int i, int part) {
+    const int row = i * COPY_ROWS + crow;
+    *reinterpret_cast<u32x4 *>(v_lds + stage * kTileBytes + row * D * 2 + v_pair<D>(crow, cchunk) * 32 + part * 16) =
+        widen8<BF>(vr[i][2 * part], vr[i][2 * part + 1], half_of(i) ? vs[1] : vs[0]);
+  };
+  // a transposing load: 16 lanes take 4 keys x 16 channels, lane i of them gets channel i of the 4
   const int vrow = 4 * h + ((lane & 15) >> 2), vpair = (lane >> 4) & 1, vbyte = (lane & 3) * 8;
-  auto k_frag = [&](const uint8_t *kt, int t, int j) {
-    const int row = 32 * t + r;
-    return *reinterpret_cast<const u32x4 *>(kt + row * D * 2 + k_chunk<D>(row, 2 * j + h) * 16);
+  auto k_frag = [&](const uint8_t *kt, int x, int j) {
+    return *reinterpret_cast<const u32x4 *>(kt + (32 * x + r) * D * 2 + k_chunk<D>(r, 2 * j + h) * 16);
   };
-  auto v_frag = [&](const uint8_t *vt, int d, int ks) {
+  auto v_frag = [&](const uint8_t *vt, int ks, int d) {
     u32x4 f;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const int row = 16 * ks + 8 * x + vrow;
-      const uint8_t *src = vt + row * D * 2 + v_pair<D>(row, 2 * d + vpair) * 32 + vbyte;
+      const uint8_t *src = vt + row * D * 2 + v_pair<D>(vrow, 2 * d + vpair) * 32 + vbyte;
       const u32x2 g = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(src)));
       f[2 * x] = g.x, f[2 * x + 1] = g.y;
     }
     return f;
   };
-  f32x16 o[DT] = {};
-  float m = -INFINITY, l = 0.0f, move = 1.0f;
+  auto largest = [](const f32x16 &x) {
+    float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int e = 0; e < 16; ++e) y[e & 3] = fmaxf(y[e & 3], x[e]);
+    return fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+  };
+  f32x16 o[DT] = {}, s = {}, other;
+  float m = -INFINITY, l = 0.0f, top = -INFINITY;
   if (tiles > 0) {
     look_up(0);
-    fetch(0);
-    move = store(0, 0);
+    u32x4 next[COPIES];
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) fetch_k(1, i), next[i] = kr[i];
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) fetch_k(0, i), fetch_v(0, i);
+    scales_of(0);
+    move = 1.0f;
+    static_for<0, 2 * COPIES>([&](auto q) { store_k(0, q / 2, q % 2), store_v(0, q / 2, q % 2); });
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) kr[i] = next[i];
+    static_for<0, 2 * COPIES>([&](auto q) { store_k(1, q / 2, q % 2); });
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) fetch_k(2, i), fetch_v(1, i);
+    barrier_lds();
+#pragma unroll
+    for (int j = 0; j < KS; ++j) s = mfma32<BF>(k_frag(k_lds, 1, j), qf[j], s);
+    top = largest(s);
   }
-  for (int t = 0; t < tiles; ++t) {
-    const int at = begin + t * BN, stage = t & 1;
-    __syncthreads();
+  // 32 keys, half x of tile t: their scores s become next, the following half's. Called with the two in turn, so that nothing is
+  // moved. Beside the products, tile t + 2 of keys (x = 0) or t + 1 of values (x = 1) goes from registers to LDS, and the codes of
+  // the one after it are asked for.
+  auto half = [&](int t, auto xc, auto stage_c, f32x16 &s, f32x16 &next) {
+    constexpr int x = decltype(xc)::value, stage = decltype(stage_c)::value;
+    const uint8_t *kt = k_lds + (stage ^ 1) * kTileBytes, *vt = v_lds + stage * kTileBytes + 32 * x * D * 2;
+    const int at = begin + t * BN + 32 * x;
     // (never zero: -infinity times that would be NaN)
-    const float c[2] = {fmaxf(lane_value(k_scale[0], t & 63) * a.scale, 0x1p-126f), fmaxf(lane_value(k_scale[1], t & 63) * a.scale, 0x1p-126f)};
-    const bool hole[2] = {__builtin_amdgcn_readlane(number[0], t & 63) < 0, __builtin_amdgcn_readlane(number[1], t & 63) < 0};
-    if (t + 1 < tiles) {
-      if (((t + 1) & 63) == 0) look_up(t + 1);
-      fetch(t + 1);
+    const float c = fmaxf(lane_value(k_scale[x], t - base) * a.scale, 0x1p-126f);
+    const bool hole = __builtin_amdgcn_readlane(number[x], t - base) < 0;
+    if (at + 32 > all || hole) {
+      const int left = opaque(hole ? 0 : sees - at - 4 * h);  // opaque: a branch, not selects in every half
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (8 * (e >> 2) + (e & 3) >= left) s[e] = -INFINITY;
+      top = largest(s);
     }
-    uint8_t *kt = lds + stage * kTileBytes, *vt = lds + (2 + stage) * kTileBytes;
-    bool bad = false;
-    if (at + BN > all_rows) {
-      const bool found = __any(any_bad<D, BF>(vt));
-      if (lane == 0) flags[wave] = found;
-      __syncthreads();
-      bad = __builtin_amdgcn_readfirstlane(flags[0] | flags[1] | flags[2] | flags[3]);
-      if (bad) {
-        for (int i = tid; i < BN * DT; i += 256) take_bad<D, BF>(vt, i / DT, i % DT, &marks[i], &marks[BN * DT + i]);
-        __syncthreads();
-      }
-    }
-    f32x16 s[2] = {};
+    constexpr int NM = KS, NV = 2 * DT, NP = 8;
+    // 192 registers of queries and sums: the queries stay in accumulation registers, which the products read as they are
+    if constexpr (D == 256)
 #pragma unroll
-    for (int j = 0; j < KS; ++j)
-#pragma unroll
-      for (int x = 0; x < 2; ++x) s[x] = mfma32<BF>(k_frag(kt, x, j), qf[j], s[x]);
-    if (at + BN > all || hole[0] || hole[1]) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int left = hole[x] ? 0 : sees - at - 4 * h - 32 * x;
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (8 * (e >> 2) + (e & 3) >= left) s[x][e] = -INFINITY;
-      }
-    }
-    float top = -INFINITY;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      float y = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) y = fmaxf(y, s[x][e]);
-      top = fmaxf(top, y * c[x]);
-    }
-    top = fmaxf(top, lane_xor32(top));
-    if (__any(top > m + kLag<BF>) || move != 1.0f) {
+      for (int j = 0; j < KS; ++j) asm volatile("" : "+a"(qf[j]));
+    u32x4 ring[kAhead + 1];
+    auto frag = [&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      if constexpr (i < KS)
+        ring[i % (kAhead + 1)] = k_frag(kt, x, i);
+      else if constexpr (i < KS + 2 * DT)
+        ring[i % (kAhead + 1)] = v_frag(vt, (i - KS) / DT, (i - KS) % DT);
+    };
+    static_for<0, kAhead>([&](auto ic) { frag(ic); });
+    __builtin_amdgcn_sched_barrier(0);
+    top = fmaxf(top, lane_xor32(top)) * c;
+    const float moved = x == 0 ? move : 1.0f;
+    if (__any(top > m + kLag<BF>) || (!BF && moved != 1.0f)) {
       const float to = fmaxf(m, top), keep = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
       m = to;
       l *= keep;
 #pragma unroll
-      for (int d = 0; d < DT; ++d) o[d] *= keep * move;
+      for (int d = 0; d < DT; ++d) o[d] *= keep * moved;
     }
     const float lift = m == -INFINITY ? 0.0f : kLift<BF> - m;
-    u32x4 p[4];
+    float peak[2] = {-INFINITY, -INFINITY}, ex[NP][2];
+    if constexpr (x == 1) scales_of(t + 1);
+    constexpr int NS = NM + NV / 2 - 2, NR = NM + NV - NS, PIECES = 2 * COPIES;  // slots with exponentials, and with the maximum
+    static_assert(weights_in_time(NM, NV, NP, DT, NS), "an output product before its weights");
+    u32x4 p[2];
+    auto each = [&](auto slot, auto f) {  // the pairs of a slot
+      constexpr int i = decltype(slot)::value;
+      if constexpr (i >= 0 && i < NS) static_for<i * NP / NS, (i + 1) * NP / NS>(f);
+    };
+    static_for<0, NM + NV>([&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      frag(IC<i + kAhead>{});
+      if constexpr (i < NM)
+        next = mfma32<BF>(ring[i % (kAhead + 1)], qf[i], i == 0 ? f32x16{} : next);
+      else
+        o[(i - NM) % DT] = mfma32<BF>(ring[i % (kAhead + 1)], p[(i - NM) / DT], o[(i - NM) % DT]);
+      each(IC<i>{}, [&](auto ec) {
+        constexpr int e = decltype(ec)::value;
+        ex[e][0] = __builtin_amdgcn_exp2f(fmaf(s[2 * e], c, lift));
+        ex[e][1] = __builtin_amdgcn_exp2f(fmaf(s[2 * e + 1], c, lift));
+      });
+      each(IC<i - 1>{}, [&](auto ec) {
+        constexpr int e = decltype(ec)::value;
+        p[e / 4][e % 4] = pack2<BF>(ex[e][0], ex[e][1]);
+      });
+      each(IC<i - 2>{}, [&](auto ec) {
+        constexpr int e = decltype(ec)::value;
+        l = opaque(add2<BF>(p[e / 4][e % 4], l));  // opaque: here, not after the branch
+      });
+      // a piece of a tile: eight codes; then, a copy being out of its registers, the next one's load
+      static_for<(i * PIECES + NM + NV - 1) / (NM + NV), ((i + 1) * PIECES + NM + NV - 1) / (NM + NV)>([&](auto qc) {
+        constexpr int q = decltype(qc)::value;
+        if constexpr (x == 0)
+          store_k(stage, q / 2, q % 2);
+        else
+          store_v(stage ^ 1, q / 2, q % 2);
+        if constexpr (q % 2) {
+          if constexpr (x == 0)
+            fetch_k(t + 3, q / 2);
+          else
+            fetch_v(t + 2, q / 2);
+        }
+      });
+      if constexpr (i >= NS)
+        static_for<(i - NS) * NP / NR, (i - NS + 1) * NP / NR>([&](auto ec) {
+          constexpr int e = decltype(ec)::value;
+          peak[e & 1] = opaque(fmaxf(fmaxf(next[2 * e], next[2 * e + 1]), peak[e & 1]));
+        });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    top = fmaxf(peak[0], peak[1]);
+  };
+  auto step = [&](int t, auto stage_c) {
+    constexpr int stage = decltype(stage_c)::value;
+    if (t + 4 > base + 64) look_up(t);
+    barrier_lds();  // this tile's values and the next one's keys are there, and what they replace has been read
+    const int at = begin + t * BN;
+    uint8_t *vt = v_lds + stage * kTileBytes;
+    bool bad = false;
+    if (at + BN > all_rows) {  // the workgroup's first row does not see all of it
+      const bool found = __any(any_bad<D, BF, THREADS>(vt));
+      if (lane == 0) flags[wave] = found;
+      barrier_lds();
+      uint32_t any = 0;
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float u = __builtin_amdgcn_exp2f(fmaf(s[x][2 * e], c[x], lift)), w = __builtin_amdgcn_exp2f(fmaf(s[x][2 * e + 1], c[x], lift));
-        p[2 * x + (e >> 2)][e & 3] = pack2<BF>(u, w);
-        l = add2<BF>(p[2 * x + (e >> 2)][e & 3], l);
+      for (int w = 0; w < NW; ++w) any |= flags[w];
+      bad = __builtin_amdgcn_readfirstlane(any);
+      if (bad) {
+        for (int i = tid; i < BN * DT; i += THREADS) take_bad<D, BF>(vt, i / DT, i % DT, &marks[i], &marks[BN * DT + i]);
+        barrier_lds();
       }
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-      for (int d = 0; d < DT; ++d) o[d] = mfma32<BF>(v_frag(vt, d, ks), p[ks], o[d]);
+    }
+    half(t, IC<0>{}, stage_c, s, other);
+    half(t, IC<1>{}, stage_c, other, s);
     if (bad) {
       for (int j = 0; j < BN; ++j)
 #pragma unroll
@@ -327,16 +416,19 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_chunk_rows(ChunkArgs 
           }
         }
     }
-    if (t + 1 < tiles) move = store(t + 1, stage ^ 1);
+  };
+  for (int t = 0; t < tiles; t += 2) {
+    step(t, IC<0>{});
+    if (t + 1 >= tiles) break;
+    step(t + 1, IC<1>{});
   }
-  __syncthreads();
-  l += lane_xor32(l);
-  const int own = first + 32 * wave;  // the wavefront's first pair
-  const bool there = own + r < pairs;
+  barrier_lds();
   auto line_of = [&](int f) {  // of a pair [T][q_heads]
     const int row = f / group;
     return size_t(work.row0 + row) * a.q_heads + kv * group + (f - row * group);
   };
+  const bool there = own + r < pairs;
+  const float weight = l + lane_xor32(l);
   if (a.part) {
     if (there && chunk == 0 && h == 0) a.joins[line_of(own + r)] = parts > 1 ? parts : 0;
     if (parts > 1) {
@@ -355,11 +447,11 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_chunk_rows(ChunkArgs 
         const f32x4 w = *reinterpret_cast<const f32x4 *>(rows + row * D + (c ^ (row & 15)) * 4);
         if (own + row < pairs) *reinterpret_cast<f32x4 *>(part + line_of(own + row) * (D + 4) + c * 4) = w;
       }
-      if (there && h == 0) *reinterpret_cast<float2 *>(part + line_of(own + r) * (D + 4) + D) = float2{m, l};
+      if (there && h == 0) *reinterpret_cast<float2 *>(part + line_of(own + r) * (D + 4) + D) = float2{m, weight};
       return;
     }
   }
-  const float inv = l == 0.0f ? 0.0f : ref / l;
+  const float inv = weight == 0.0f ? 0.0f : ref / weight;
   uint8_t *rows = lds + wave * 32 * D * 2;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -376,28 +468,46 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) k_chunk_rows(ChunkArgs 
   }
 }
 
-// Chunks of keys where the rows alone would leave half of the GPU's places idle (two workgroups a CU, one at width 256): as many
-// as fit the places, of 512 keys at least
+// How a call is laid out: wavefronts a workgroup, and chunks of keys where the rows alone would not fill the GPU's places, or not
+// evenly. Priced in us, as measured: what a workgroup takes for a key (all places of the GPU at work) and for its beginning and
+// end, rounds of workgroups (of several sequences, which rarely are as long as the longest: 0.6 of that; the last round half
+// full), and chunks' sums written and read at 4 TB/s by a second kernel. Eight wavefronts a workgroup convert each key once for 256
+// pairs instead of 128 (2,048 rows over 34,816 tokens, 32 heads over 4 of 128: 1,158 -> 1,067 us), but leave coarser work.
 struct ChunkPlan {
-  int chunk, chunks;
+  int waves, chunk, chunks;
+  long long tiles;
   size_t rows, bytes;  // the workspace's sums, and all of it
 };
-static long long chunk_tiles(int T, int B, int group) { return (long long)T * group / 128 + B; }
 static ChunkPlan chunk_plan(int T, int q_heads, int heads, int D, int B, int longest) {
-  ChunkPlan p = {1 << 30, 1, 0, 0};
-  const long long work = chunk_tiles(T, B, q_heads / heads) * heads, full = D == 256 ? 256 : 512;
-  if (work <= 0 || 2 * work > full) return p;
-  const int splits = int(full / work);
-  long long chunk = ((long long)longest + splits - 1) / splits;
-  chunk = (chunk < 512 ? 512 : chunk) + kPromptKeys - 1;
-  chunk -= chunk % kPromptKeys;
-  const long long chunks = (longest + chunk - 1) / chunk;
-  if (chunks <= 1) return p;
-  p.chunk = int(chunk);
-  p.chunks = int(chunks);
-  p.rows = size_t(p.chunks) * T * q_heads * (D + 4) * sizeof(float);
-  p.bytes = p.rows + size_t(T) * q_heads * sizeof(int);
-  return p;
+  const int group = q_heads / heads;
+  const double all = B == 1 ? 1.0 : 0.6, sums = 2.0 * T * q_heads * (D + 4) * sizeof(float) * all / 4e6;
+  ChunkPlan best = {4, 1 << 30, 1, 0, 0, 0};
+  double least = 0.0;
+  for (int waves = 4; waves <= (D == 128 ? 8 : 4); waves += 4) {
+    const int rows = 32 * waves, places = D == 256 || waves == 8 ? 256 : 512;
+    const long long tiles = B == 1 ? ((long long)T * group + rows - 1) / rows : (long long)T * group / rows + B, work = tiles * heads;
+    const double key = D == 64 ? 0.022 : D == 256 ? 0.036 : waves == 8 ? 0.031 : 0.034;
+    auto look = [&](long long n) {
+      if (n < 1 || (n > 1 && (n > longest / 192 || n > 512))) return;
+      const double piece = longest * key / n + 6.0, rounds = double(work) * n / places;
+      const double us = (B == 1 ? ceil(rounds) : fmax(1.0, rounds * all + 0.5)) * piece + (n > 1 ? 4.0 + sums * n : 0.0);
+      if (best.tiles && us >= least) return;
+      least = us;
+      best.waves = waves, best.tiles = tiles, best.chunks = int(n);
+    };
+    for (long long n = 1; n <= 8; ++n) look(n);
+    for (long long k = 1; k <= 4 && work; ++k) look(k * places / work);
+  }
+  if (best.chunks == 1) return best;
+  best.chunk = ((longest + best.chunks - 1) / best.chunks + kPromptKeys - 1) / kPromptKeys * kPromptKeys;
+  best.chunks = (longest + best.chunk - 1) / best.chunk;
+  if (best.chunks == 1) {
+    best.chunk = 1 << 30;
+    return best;
+  }
+  best.rows = size_t(best.chunks) * T * q_heads * (D + 4) * sizeof(float);
+  best.bytes = best.rows + size_t(T) * q_heads * sizeof(int);
+  return best;
 }
 
 }  // namespace lmoe
@@ -422,6 +532,8 @@ extern "C" int lmoe_kv_chunk(const void *q, int dtype, long long q_row, long lon
                heads);
   LMOE_REQUIRE(pages > 0 && width > 0 && width <= 0x7fffffff / page, LMOE_ESHAPE, "%s: %d pages, a table of %d places", fn, pages,
                width);
+  LMOE_REQUIRE((long long)heads * page * D <= 0x7fffffff, LMOE_ESHAPE, "%s: pages of %d heads, %d tokens and %d channels", fn, heads,
+               page, D);
   LMOE_REQUIRE(T >= 0 && B >= 0 && longest > 0, LMOE_ESHAPE, "%s: %d rows of %d sequences of %d tokens", fn, T, B, longest);
   if (T == 0) return 0;
   LMOE_REQUIRE(B > 0, LMOE_ESHAPE, "%s: %d rows of no sequence", fn, T);
@@ -433,7 +545,7 @@ extern "C" int lmoe_kv_chunk(const void *q, int dtype, long long q_row, long lon
   LMOE_REQUIRE((long long)T * q_heads / heads <= 0x7fffff00 && T <= (1 << 30), LMOE_ESHAPE, "%s: %d rows of %d heads a group", fn, T,
                q_heads / heads);
   const ChunkPlan plan = chunk_plan(T, q_heads, heads, D, B, longest);
-  const long long tiles = chunk_tiles(T, B, q_heads / heads), groups = tiles * heads * plan.chunks;
+  const long long groups = plan.tiles * heads * plan.chunks;
   LMOE_REQUIRE(groups <= kMostGroups && ((long long)T * q_heads * (D / 4) + 255) / 256 <= (plan.bytes ? kMostGroups : 1ll << 62),
                LMOE_ESHAPE, "%s: %d rows of %d sequences and %d heads are more than a launch takes", fn, T, B, q_heads);
   LMOE_REQUIRE(plan.bytes == 0 || (workspace && aligned16(workspace) && workspace_bytes >= plan.bytes), LMOE_EWORKSPACE,
@@ -442,11 +554,12 @@ extern "C" int lmoe_kv_chunk(const void *q, int dtype, long long q_row, long lon
   int *joins = plan.bytes ? reinterpret_cast<int *>(static_cast<char *>(workspace) + plan.rows) : nullptr;
   ChunkArgs a = {static_cast<const uint16_t *>(q), q_row, q_head, k_codes, v_codes, k_scale, v_scale, table, lens, cu,
                  static_cast<uint16_t *>(out), part, joins, scale * 1.4426950408889634f, T, B, q_heads, heads, q_heads / heads, pages,
-                 width, page == 32 ? 5 : page == 64 ? 6 : 7, int(tiles), plan.chunk, plan.chunks};
+                 width, page == 32 ? 5 : page == 64 ? 6 : 7, int(plan.tiles), plan.chunk, plan.chunks};
   auto go = [&](auto kernel, auto join) -> int {
-    const size_t lds = size_t(kPromptKeys) * D * 2 * 4;
-    if (const int rc = allow_lds(kernel, lds + 4112, fn)) return rc;  // with what the kernel declares itself
-    launch(kernel, dim3(unsigned(groups)), dim3(256), lds, (hipStream_t)stream, a);
+    // two stages of a tile of keys and of values; sums in float32, which the wavefronts store through LDS, may take more
+    const size_t tiles = size_t(kPromptKeys) * D * 2 * 4, sums = part ? size_t(plan.waves) * 32 * D * 4 : 0, lds = tiles > sums ? tiles : sums;
+    if (const int rc = allow_lds(kernel, lds + 4128, fn)) return rc;  // with what the kernel declares itself
+    launch(kernel, dim3(unsigned(groups)), dim3(unsigned(64 * plan.waves)), lds, (hipStream_t)stream, a);
     LMOE_LAUNCHED(fn);
     if (part) {
       launch(join, dim3(unsigned(((long long)T * q_heads * (D / 4) + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
@@ -455,9 +568,12 @@ extern "C" int lmoe_kv_chunk(const void *q, int dtype, long long q_row, long lon
     }
     return 0;
   };
-  const bool bf = dtype == LMOE_BF16;
-  if (D == 64) return bf ? go(k_chunk_rows<64, true>, k_join_chunks<64, true>) : go(k_chunk_rows<64, false>, k_join_chunks<64, false>);
-  if (D == 128)
-    return bf ? go(k_chunk_rows<128, true>, k_join_chunks<128, true>) : go(k_chunk_rows<128, false>, k_join_chunks<128, false>);
-  return bf ? go(k_chunk_rows<256, true>, k_join_chunks<256, true>) : go(k_chunk_rows<256, false>, k_join_chunks<256, false>);
+  auto type = [&](auto d, auto waves) -> int {
+    constexpr int W = decltype(d)::value, NW = decltype(waves)::value;
+    return dtype == LMOE_BF16 ? go(k_chunk_rows<W, true, NW>, k_join_chunks<W, true>)
+                              : go(k_chunk_rows<W, false, NW>, k_join_chunks<W, false>);
+  };
+  if (D == 64) return type(IC<64>{}, IC<4>{});
+  if (D == 128) return plan.waves == 8 ? type(IC<128>{}, IC<8>{}) : type(IC<128>{}, IC<4>{});
+  return type(IC<256>{}, IC<4>{});
 }

@@ -59,13 +59,13 @@ __device__ __forceinline__ float add2(uint32_t pair, float a) {
 
 // Whether a thread's share of a tile's values holds one that is not finite. In LDS order: looked at by key and channel, as
 // take_bad does, 18 prompts of 512 rows take 112 us instead of 107.6 (16 heads of 256)
-template <int D, bool BF>
+template <int D, bool BF, int THREADS = 256>
 __device__ __forceinline__ bool any_bad(const uint8_t *vt) {
   constexpr uint32_t INF = BF ? 0x7f80u : 0x7c00u;
   uint32_t over = 0;
 #pragma unroll
-  for (int i = 0; i < kPromptKeys * D / 8 / 256; ++i) {  // a half word's magnitude of INF or more carries into its sign bit
-    const u32x4 w = reinterpret_cast<const u32x4 *>(vt)[i * 256 + threadIdx.x];
+  for (int i = 0; i < kPromptKeys * D / 8 / THREADS; ++i) {  // a half word's magnitude of INF or more carries into its sign bit
+    const u32x4 w = reinterpret_cast<const u32x4 *>(vt)[i * THREADS + threadIdx.x];
 #pragma unroll
     for (int e = 0; e < 4; ++e) over |= (w[e] & 0x7fff7fffu) + (0x8000u - INF) * 0x10001u;
   }
@@ -98,16 +98,6 @@ __device__ __forceinline__ void take_bad(uint8_t *vt, int row, int c32, uint32_t
   }
   *pos = up;
   *neg = down;
-}
-
-// Whether every output product's weights are packed a slot before it: NM score products, NV output products over NP pairs of
-// weights, DT channel tiles, pairs spread over NS slots and packed one slot later
-constexpr bool weights_in_time(int NM, int NV, int NP, int DT, int NS) {
-  for (int k = 0; k < NV; ++k) {
-    const int slots = NM + k - 1 < NS ? NM + k - 1 : NS;
-    if (slots * NP / NS < 4 * (k / DT + 1)) return false;
-  }
-  return true;
 }
 
 // Rows whose keys were worked in more than one chunk: D / 4 threads a row and head, the chunks joined in order

@@ -51,6 +51,16 @@ __device__ __forceinline__ void dma_lanes(const void *from, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds) : "memory");
 }
 
+// Whether every output product's weights are packed a slot before it: NM score products, NV output products over NP pairs of
+// weights, DT channel tiles, pairs spread over NS slots and packed one slot later
+constexpr bool weights_in_time(int NM, int NV, int NP, int DT, int NS) {
+  for (int k = 0; k < NV; ++k) {
+    const int slots = NM + k - 1 < NS ? NM + k - 1 : NS;
+    if (slots * NP / NS < 4 * (k / DT + 1)) return false;
+  }
+  return true;
+}
+
 // The nth tile of rows that is worked, by one wavefront. Up to 64 sequences: the tiles furthest into their sequences first,
 // which see the most keys, so that what is left for the end is short (16 prompts of up to 4,000 rows at width 64: 160 -> 134
 // us, of up to 900 at 128: 37 -> 30; long prompts lose up to 5 % by sharing less of L2: 12 of up to 3,500 rows 332 -> 345).
