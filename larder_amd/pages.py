@@ -68,7 +68,7 @@ def take_pages(refs, table, lens, cu=None, page=64):
     if cu is not None:
         cu = _ints(fn, "cu", cu, n + 1)
     dev = _device(fn, refs, table, lens, cu)
-    src, dst, lacking = (refs.new_empty(n) for _ in range(3))
+    src, dst, lacking = refs.new_empty((3, n)).unbind(0)
     if n:
         need = _take_workspace(n, places, pages)
         ws = refs.new_empty(need, dtype=torch.uint8)

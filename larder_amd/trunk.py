@@ -15,7 +15,7 @@ bfloat16 [N, K / G].
 import torch
 
 from . import attention
-from ._lib import call, dcode, ptr, stream
+from ._lib import F32, call, dcode, ptr, stream
 
 __all__ = ["attention_rows", "norm_rows", "qmv_fits", "qmv_rows", "read_codes", "shared_expert_rows"]
 
@@ -112,12 +112,14 @@ def attention_rows(x, qkv, out, cache, table, lens, cu=None, freq=None, interlea
 def _planes(x):
     """(x, rows, heads, row stride, head stride): x [..., H] as rows of heads, its last axis dense; copied where its leading
     axes are not two strides."""
-    if x.dim() > 3 or (x.shape[-1] > 1 and x.stride(-1) != 1):
+    n, st = x.dim(), x.stride()
+    if n > 3 or (st[-1] != 1 and x.shape[-1] > 1):
         x = x.contiguous()
-    if x.dim() == 3:
-        return x, x.shape[0], x.shape[1], x.stride(0), x.stride(1)
-    if x.dim() == 2:
-        return x, x.shape[0], 1, x.stride(0), 0
+        st = x.stride()
+    if n == 2:
+        return x, x.shape[0], 1, st[0], 0
+    if n == 3:
+        return x, x.shape[0], x.shape[1], st[0], st[1]
     return x, x.numel() // x.shape[-1], 1, x.shape[-1], 0
 
 
@@ -135,30 +137,33 @@ def norm_rows(x, weight, eps=1e-6, residual=None, group=None, total=None):
     fn = "norm_rows"
     if x.dim() == 0 or x.shape[-1] == 0:
         attention._refuse(fn, "x is [..., channels]")
-    h, shape = x.shape[-1], x.shape
-    dt = dcode(x.dtype)
-    if weight.dim() != 1 or weight.shape[0] != h or weight.dtype not in (x.dtype, torch.float32):
+    shape, dtype = x.shape, x.dtype
+    h, plain = shape[-1], len(shape) == 2  # [rows, channels]: the most common, with the host's time in mind
+    dt = dcode(dtype)
+    if weight.dim() != 1 or weight.shape[0] != h or (weight.dtype is not dtype and weight.dtype is not torch.float32):
         attention._refuse(fn, f"weight is [{h}] in x's type or float32, not {weight.dtype} {list(weight.shape)}")
     if not 0.0 < eps < float("inf"):
         attention._refuse(fn, f"eps {eps} is not above zero")
-    if residual is not None and (residual.shape != shape or residual.dtype is not x.dtype):
+    if residual is not None and (residual.shape != shape or residual.dtype is not dtype):
         attention._refuse(fn, "residual has x's shape and type")
     if group is not None and group != h and (group not in (32, 64, 128, 256, 512) or h % group):
         attention._refuse(fn, f"scales of {group} channels in rows of {h} (32, 64, 128, 256 or 512 that divide them, or whole rows)")
     sums = residual is not None or total is not None
-    if total is None:
+    own = total is None  # the sum's tensor is this call's
+    if own:
         total = x.new_empty(shape) if sums else None
-    elif total.shape != shape or total.dtype is not x.dtype or (h > 1 and total.stride(-1) != 1) or (
+    elif total.shape != shape or total.dtype is not dtype or (h > 1 and total.stride(-1) != 1) or (
             total.dim() > 3 and not total.is_contiguous()):
         attention._refuse(fn, "total has x's shape and type and a dense last axis")
     dev = attention._device(fn, x, weight, residual, total)
-    weight = weight.contiguous()
+    if h > 1 and weight.stride(0) != 1:
+        weight = weight.contiguous()
     x, t, heads, x_row, x_head = _planes(x)
     r_row = r_head = s_row = s_head = 0
     if residual is not None:
         residual, _, _, r_row, r_head = _planes(residual)
     if total is not None:
-        _, _, _, s_row, s_head = _planes(total)
+        s_row, s_head = (h, 0) if own and plain else _planes(total)[3:]
     scales = None
     if group is None:
         out = x.new_empty(shape)
@@ -167,8 +172,9 @@ def norm_rows(x, weight, eps=1e-6, residual=None, group=None, total=None):
         scales = x.new_empty(shape[:-1] + (h // group,), dtype=torch.float32)
     if t and heads:
         attention._launch(dev, "lmoe_norm_rows", x.data_ptr(), dt, x_row, x_head, None if residual is None else residual.data_ptr(),
-                          r_row, r_head, weight.data_ptr(), dcode(weight.dtype), t, heads, h, eps, out.data_ptr(), group or 0,
-                          None if scales is None else scales.data_ptr(), None if total is None else total.data_ptr(), s_row, s_head)
+                          r_row, r_head, weight.data_ptr(), dt if weight.dtype is dtype else F32, t, heads, h, eps, out.data_ptr(),
+                          0 if group is None else group, None if scales is None else scales.data_ptr(),
+                          None if total is None else total.data_ptr(), s_row, s_head)
     if group is None:
         return (out, total) if sums else out
     return (out, scales, total) if sums else (out, scales)
