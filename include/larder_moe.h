@@ -565,7 +565,8 @@ int lmoe_kv_chunk(const void *q, int dtype, long long q_row, long long q_head, i
  * back and every place of out counted. out does not overlap table.
  * lmoe_pages_compact: the held pages (refs > 0) past the first `used` (how many are held) numbers move to the free ones among
  * those, both in order: src and dst [max(pages / 2, 1)] the pairs, -1 behind them; refs follow. to [pages]: the new number
- * of every page from `used` on, which lmoe_pages_renumber writes into a table's places.
+ * of every page from `used` on, which lmoe_pages_renumber writes into a table's places. workspace:
+ * lmoe_pages_compact_workspace_bytes.
  * lmoe_pages_copy: codes and scales of src[i] to dst[i] [n]; pairs with a page outside the cache are left out. No page is
  * in dst twice, or in both lists. */
 size_t lmoe_pages_take_workspace_bytes(int B, int width, int pages);
@@ -573,7 +574,9 @@ int lmoe_pages_take(int *refs, int pages, int *table, int B, int width, const in
                     int *lacking, void *workspace, size_t workspace_bytes, void *stream);
 int lmoe_pages_free(int *refs, int pages, int *table, int B, int width, const int *keep, int page, void *stream);
 int lmoe_pages_fork(int *refs, int pages, const int *table, int B, int width, const int *parents, int n, int *out, void *stream);
-int lmoe_pages_compact(int *refs, int pages, int *src, int *dst, int *used, int *to, void *stream);
+size_t lmoe_pages_compact_workspace_bytes(int pages);
+int lmoe_pages_compact(int *refs, int pages, int *src, int *dst, int *used, int *to, void *workspace, size_t workspace_bytes,
+                       void *stream);
 int lmoe_pages_renumber(int *table, int B, int width, int pages, const int *used, const int *to, void *stream);
 int lmoe_pages_copy(uint8_t *k_codes, float *k_scale, uint8_t *v_codes, float *v_scale, int pages, int page, int heads, int D,
                     const int *src, const int *dst, int n, void *stream);

@@ -123,7 +123,8 @@ SIGNATURES = {
     "lmoe_pages_take": (_I, [_P, _I, _P, _I, _I, _P, _P, _I, _P, _P, _P, _P, _SZ, _P]),
     "lmoe_pages_free": (_I, [_P, _I, _P, _I, _I, _P, _I, _P]),
     "lmoe_pages_fork": (_I, [_P, _I, _P, _I, _I, _P, _I, _P, _P]),
-    "lmoe_pages_compact": (_I, [_P, _I, _P, _P, _P, _P, _P]),
+    "lmoe_pages_compact_workspace_bytes": (_SZ, [_I]),
+    "lmoe_pages_compact": (_I, [_P, _I, _P, _P, _P, _P, _P, _SZ, _P]),
     "lmoe_pages_renumber": (_I, [_P, _I, _I, _I, _P, _P, _P]),
     "lmoe_pages_copy": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _P]),
 }

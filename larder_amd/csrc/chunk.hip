@@ -26,11 +26,11 @@ struct ChunkArgs {
   float *part;    // [chunks][T][q_heads] of [D] sums and {maximum, weight}: rows whose keys are worked in more than one chunk
   int *joins;     // [T][q_heads]: how many chunks (0: one, the row is done)
   float scale;    // times log2 e
-  int T, B, q_heads, heads, group, pages, width, page_shift, tiles, chunk, chunks;  // chunk: keys, the last goes on to the end
+  int T, B, q_heads, heads, group, pages, width, page_shift, tiles, chunk, chunks, sorted;  // chunk: keys, the last goes on to the end
 };
 
 // The nth tile of ROWS pairs that is worked, by one wavefront. Up to 64 sequences: those that see the most keys first (to 256
-// keys), so that what is left for the end is short. More: the sequences from the last on, each from its end, eight tiles in
+// keys), so that what is left for the end is short (sorted; where all find a place at once, in the order of sequences). More: the sequences from the last on, each from its end, eight tiles in
 // turn shifted against the next eight (prompt.hip says why); sequence b's tiles begin at cu[b] group / ROWS + b, which leaves
 // it room for all of them. b < 0: there is none. The first and the last sequence have a tile even without rows.
 struct ChunkTile {
@@ -70,7 +70,7 @@ __device__ __forceinline__ ChunkTile nth_chunk_tile(const ChunkArgs &a, int nth)
     return at >= tiles ? 0 : tiles - int(at);
   };
   auto from = [&](int x) { return int(wave_sum(float(count(x)))); };  // (counts below 2^24: exact in float32)
-  int lo = 0, hi = (int(wave_max(tiles > 0 ? float(past) + float(tiles) * ROWS / a.group : 0.0f)) >> 8) + 2, behind = 0;
+  int lo = 0, hi = !a.sorted ? 1 : (int(wave_max(tiles > 0 ? float(past) + float(tiles) * ROWS / a.group : 0.0f)) >> 8) + 2, behind = 0;
   if (nth >= from(0)) return w;
   while (hi - lo > 1) {  // the largest x with more than nth tiles from it on
     const int mid = lo + ((hi - lo) >> 1), c = from(mid);
@@ -80,7 +80,7 @@ __device__ __forceinline__ ChunkTile nth_chunk_tile(const ChunkArgs &a, int nth)
       hi = mid, behind = c;
   }
   // of the tiles that see 256 lo keys and not 256 more, the lane's sequence has `mine`; in the order of sequences
-  const int above = count(lo + 1), mine = count(lo) - above;
+  const int above = a.sorted ? count(lo + 1) : 0, mine = count(lo) - above;
   int ends = mine;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -499,8 +499,8 @@ static ChunkPlan chunk_plan(int T, int q_heads, int heads, int D, int B, int lon
     for (long long k = 1; k <= 4 && work; ++k) look(k * places / work);
   }
   if (best.chunks == 1) return best;
-  best.chunk = ((longest + best.chunks - 1) / best.chunks + kPromptKeys - 1) / kPromptKeys * kPromptKeys;
-  best.chunks = (longest + best.chunk - 1) / best.chunk;
+  best.chunk = int((((long long)longest + best.chunks - 1) / best.chunks + kPromptKeys - 1) / kPromptKeys * kPromptKeys);
+  best.chunks = int(((long long)longest + best.chunk - 1) / best.chunk);
   if (best.chunks == 1) {
     best.chunk = 1 << 30;
     return best;
@@ -542,7 +542,7 @@ extern "C" int lmoe_kv_chunk(const void *q, int dtype, long long q_row, long lon
   LMOE_REQUIRE(q && out && lens && table && k_codes && k_scale && v_codes && v_scale, LMOE_EINVAL, "%s: null pointer", fn);
   LMOE_REQUIRE(aligned16(q) && aligned16(out) && aligned16(k_codes) && aligned16(v_codes) && q_row % 8 == 0 && q_head % 8 == 0,
                LMOE_EALIGN, "%s: rows and codes must be 16-byte aligned", fn);
-  LMOE_REQUIRE((long long)T * q_heads / heads <= 0x7fffff00 && T <= (1 << 30), LMOE_ESHAPE, "%s: %d rows of %d heads a group", fn, T,
+  LMOE_REQUIRE((long long)T * q_heads / heads <= 0x7ffff000, LMOE_ESHAPE, "%s: %d rows of %d heads a group", fn, T,
                q_heads / heads);
   const ChunkPlan plan = chunk_plan(T, q_heads, heads, D, B, longest);
   const long long groups = plan.tiles * heads * plan.chunks;
@@ -554,7 +554,8 @@ extern "C" int lmoe_kv_chunk(const void *q, int dtype, long long q_row, long lon
   int *joins = plan.bytes ? reinterpret_cast<int *>(static_cast<char *>(workspace) + plan.rows) : nullptr;
   ChunkArgs a = {static_cast<const uint16_t *>(q), q_row, q_head, k_codes, v_codes, k_scale, v_scale, table, lens, cu,
                  static_cast<uint16_t *>(out), part, joins, scale * 1.4426950408889634f, T, B, q_heads, heads, q_heads / heads, pages,
-                 width, page == 32 ? 5 : page == 64 ? 6 : 7, int(plan.tiles), plan.chunk, plan.chunks};
+                 width, page == 32 ? 5 : page == 64 ? 6 : 7, int(plan.tiles), plan.chunk, plan.chunks,
+                 groups > (D == 256 || plan.waves == 8 ? 256 : 512)};
   auto go = [&](auto kernel, auto join) -> int {
     // two stages of a tile of keys and of values; sums in float32, which the wavefronts store through LDS, may take more
     const size_t tiles = size_t(kPromptKeys) * D * 2 * 4, sums = part ? size_t(plan.waves) * 32 * D * 4 : 0, lds = tiles > sums ? tiles : sums;

@@ -42,7 +42,7 @@ __device__ __forceinline__ int block_scan(int v, int *lds, int *total) {
 
 // Ranks of the pages of a stretch of J kTakers from p0 on that `is` holds for, in order, by the whole workgroup: rank(p, k), k = how
 // many come before p in the stretch. Returns how many there are. J loads are on their way at a time, and ballots count them
-// (a page a thread and shuffles: 18 us instead of 11 for a pool of 8,192 in k_compact).
+// (a page a thread and shuffles: 18 us instead of 11 for a pool of 8,192 compacted by one workgroup).
 template <int J, typename Is, typename Rank>
 __device__ __forceinline__ int rank_stretch(int p0, int pages, const int *refs, int *lds, Is &&is, Rank &&rank) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = p0 + wave * (64 * J) + lane;
@@ -74,6 +74,16 @@ __device__ __forceinline__ int rank_stretch(int p0, int pages, const int *refs, 
   return total;
 }
 
+constexpr int kStretch = 8 * kTakers;  // pages that one workgroup looks at at a time
+
+// How many pages of each stretch are free, or held
+__global__ void __launch_bounds__(kTakers) k_count(const int *refs, int pages, int *counts, int held) {
+  __shared__ int sums[kTakers / 64];
+  const int n = rank_stretch<8>(blockIdx.x * kStretch, pages, refs, sums, [&](int, int r) { return held ? r > 0 : r == 0; },
+                                [](int, int) {});
+  if (threadIdx.x == 0) counts[blockIdx.x] = n;
+}
+
 struct TakeArgs {
   int *refs, *table;
   const int *lens, *cu;
@@ -81,6 +91,7 @@ struct TakeArgs {
   int *begins;  // [B] where a sequence's tasks begin (more than kSeqsInLds sequences)
   int *ranks;   // [tasks]
   int *given;   // [pages that are needed]
+  int *counts;  // [stretches] of free pages, or null
   int pages, B, width, page_shift;
 };
 
@@ -102,7 +113,7 @@ struct Fallen {
 // One workgroup. A task is a place that rows fall into, in the order of sequences and places. 1: where each sequence's tasks
 // begin; 2: which need a page, and their ranks; 3: as many of the lowest free pages; 4: the places get them.
 __global__ void __launch_bounds__(kTakers) k_take(TakeArgs a) {
-  __shared__ int sums[kTakers / 64 + 1], begins_lds[kSeqsInLds];
+  __shared__ int sums[kTakers / 64 + 1], begins_lds[kSeqsInLds], counts[kTakers];
   const int tid = threadIdx.x;
   int *begins = a.B <= kSeqsInLds ? begins_lds : a.begins;
   int tasks = 0;
@@ -150,8 +161,19 @@ __global__ void __launch_bounds__(kTakers) k_take(TakeArgs a) {
                                                 if (found + rank < needs) a.given[found + rank] = p;
                                               });
   };
-  free_from(IC<1>{}, 0);  // (a few pages are often found among the first ones: 6.9 us of kernel instead of 9.8)
-  for (int p0 = kTakers; p0 < a.pages && found < needs; p0 += 8 * kTakers) free_from(IC<8>{}, p0);
+  if (!a.counts) {
+    free_from(IC<1>{}, 0);  // (a few pages are often found among the first ones: 6.9 us of kernel instead of 9.8)
+    for (int p0 = kTakers; p0 < a.pages && found < needs; p0 += kStretch) free_from(IC<8>{}, p0);
+  } else {  // only the stretches that have any
+    const int stretches = (a.pages + kStretch - 1) / kStretch;
+    for (int s0 = 0; s0 < stretches && found < needs; s0 += kTakers) {
+      __syncthreads();
+      counts[tid] = s0 + tid < stretches ? a.counts[s0 + tid] : 0;
+      __syncthreads();
+      for (int i = 0; i < min(kTakers, stretches - s0) && found < needs; ++i)
+        if (counts[i]) free_from(IC<8>{}, (s0 + i) * kStretch);
+    }
+  }
   __syncthreads();
   for (int t = tid; t < tasks; t += kTakers) {
     const int rank = a.ranks[t];
@@ -203,35 +225,49 @@ __global__ void __launch_bounds__(256) k_fork(int *refs, int pages, const int *t
   }
 }
 
-// One workgroup: which held pages lie past the first `used` numbers, and the free ones among those that they go to, both in order
-__global__ void __launch_bounds__(kTakers) k_compact(int *refs, int pages, int *src, int *dst, int most, int *used_out, int *to) {
+// A workgroup for each stretch, after k_count of the held pages: which held pages lie past the first `used` numbers, and the free
+// ones among those that they go to, both in order. Held pages before p are p's rank among them; what lies before `used` itself
+// is counted by every workgroup.
+__global__ void __launch_bounds__(kTakers) k_moves(const int *refs, int pages, int *counts, int *src, int *dst, int *used_out,
+                                                   int *to) {
   __shared__ int sums[kTakers / 64 + 1];
-  const int tid = threadIdx.x;
-  int used = 0;
-  for (int p0 = 0; p0 < pages; p0 += 8 * kTakers)
-    used += rank_stretch<8>(p0, pages, refs, sums, [](int, int r) { return r > 0; }, [](int, int) {});
-  int leave = 0, take = 0;
-  for (int p0 = 0; p0 < used; p0 += 8 * kTakers)
-    take += rank_stretch<8>(p0, pages, refs, sums, [&](int p, int r) { return p < used && r <= 0; },
-                         [&](int p, int rank) { dst[take + rank] = p; });
-  for (int p0 = used - used % kTakers; p0 < pages; p0 += 8 * kTakers)
-    leave += rank_stretch<8>(p0, pages, refs, sums,
-                          [&](int p, int r) {
-                            if (p >= used) to[p] = p;  // (a page that only a table knows of stays what it is)
-                            return p >= used && r > 0;
-                          },
-                          [&](int p, int rank) { src[leave + rank] = p; });
-  __syncthreads();
-  if (tid == 0) *used_out = used;
-  for (int i = tid; i < most; i += kTakers) {
-    if (i < leave) {
-      const int a = src[i], b = dst[i];
-      refs[b] = refs[a];
-      refs[a] = 0;
-      to[a] = b;
-    } else {
-      src[i] = -1, dst[i] = -1;
-    }
+  const int tid = threadIdx.x, stretches = gridDim.x, mine = blockIdx.x;
+  auto held_in = [&](int end) {  // in the stretches before `end`
+    int n = 0, total;
+    for (int i = tid; i < end; i += kTakers) n += counts[i];
+    block_scan(n, sums, &total);
+    return total;
+  };
+  const int used = held_in(stretches), edge = used / kStretch;
+  if (mine == 0 && tid == 0) *used_out = used;
+  int below = held_in(edge);  // held pages before `used`
+  if (edge < stretches)
+    below += rank_stretch<8>(edge * kStretch, pages, refs, sums, [&](int p, int r) { return p < used && r > 0; }, [](int, int) {});
+  if (mine == 0 && tid == 0) counts[stretches] = used - below;  // moves: as many as are free there
+  const int before = held_in(mine), first = mine * kStretch;
+  if (first < used)
+    rank_stretch<8>(first, pages, refs, sums, [&](int p, int r) { return p < used && r <= 0; },
+                    [&](int p, int rank) { dst[first - before + rank] = p; });
+  if (first + kStretch > used)
+    rank_stretch<8>(first, pages, refs, sums,
+                    [&](int p, int r) {
+                      if (p >= used) to[p] = p;  // (a page that only a table knows of stays what it is)
+                      return p >= used && r > 0;
+                    },
+                    [&](int p, int rank) { src[max(before - below, 0) + rank] = p; });
+}
+
+// The moved pages' counts and new numbers; -1 behind the last pair
+__global__ void __launch_bounds__(256) k_move(int *refs, const int *moves, int *src, int *dst, int most, int *to) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= most) return;
+  if (i < *moves) {
+    const int a = src[i], b = dst[i];
+    refs[b] = refs[a];
+    refs[a] = 0;
+    to[a] = b;
+  } else {
+    src[i] = -1, dst[i] = -1;
   }
 }
 
@@ -278,6 +314,10 @@ __global__ void __launch_bounds__(256) k_copy(CopyArgs a) {
   }
 }
 
+static bool pages_ok(int pages) { return pages > 0 && pages <= 1 << 30; }
+
+static int stretches(int pages) { return (pages + kStretch - 1) / kStretch; }
+
 static int page_shift(int page) { return page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : -1; }
 
 }  // namespace lmoe
@@ -287,13 +327,13 @@ using namespace lmoe;
 extern "C" size_t lmoe_pages_take_workspace_bytes(int B, int width, int pages) {
   if (B <= 0 || width <= 0 || pages <= 0) return 0;
   const long long places = (long long)B * width;
-  return size_t(B + places + (places < pages ? places : pages)) * sizeof(int);
+  return size_t(B + places + (places < pages ? places : pages) + stretches(pages)) * sizeof(int);
 }
 
 extern "C" int lmoe_pages_take(int *refs, int pages, int *table, int B, int width, const int *lens, const int *cu, int page, int *src,
                                int *dst, int *lacking, void *workspace, size_t workspace_bytes, void *stream) {
   const char *fn = "lmoe_pages_take";
-  LMOE_REQUIRE(pages > 0 && B >= 0 && width > 0, LMOE_ESHAPE, "%s: %d pages, %d sequences of %d places", fn, pages, B, width);
+  LMOE_REQUIRE(pages_ok(pages) && B >= 0 && width > 0, LMOE_ESHAPE, "%s: %d pages, %d sequences of %d places", fn, pages, B, width);
   LMOE_REQUIRE(page_shift(page) > 0, LMOE_ESHAPE, "%s: pages of %d tokens (32, 64 and 128 are served)", fn, page);
   LMOE_REQUIRE(width <= 0x7fffffff / page && (long long)B * width <= 0x7fffffff - kTakers, LMOE_ESHAPE,
                "%s: %d sequences of %d places of %d tokens are more than an int counts", fn, B, width, page);
@@ -303,15 +343,22 @@ extern "C" int lmoe_pages_take(int *refs, int pages, int *table, int B, int widt
   LMOE_REQUIRE(workspace && aligned4(workspace) && workspace_bytes >= need, LMOE_EWORKSPACE, "%s: a workspace of %zu bytes is needed",
                fn, need);
   int *begins = static_cast<int *>(workspace), *ranks = begins + B, *given = ranks + (long long)B * width;
+  // One workgroup looks at 8,192 pages in 3.4 us: from three times as many on, a launch that counts all of them at once is worth
+  // it (65,536 pages of which the last are free: 31 us without it, 11 with it)
+  int *counts = pages > 2 * kStretch ? given + ((long long)B * width < pages ? (long long)B * width : pages) : nullptr;
+  if (counts) {
+    launch(k_count, dim3(stretches(pages)), dim3(kTakers), 0, (hipStream_t)stream, refs, pages, counts, 0);
+    LMOE_LAUNCHED(fn);
+  }
   launch(k_take, dim3(1), dim3(kTakers), 0, (hipStream_t)stream,
-         TakeArgs{refs, table, lens, cu, src, dst, lacking, begins, ranks, given, pages, B, width, page_shift(page)});
+         TakeArgs{refs, table, lens, cu, src, dst, lacking, begins, ranks, given, counts, pages, B, width, page_shift(page)});
   LMOE_LAUNCHED(fn);
   return 0;
 }
 
 extern "C" int lmoe_pages_free(int *refs, int pages, int *table, int B, int width, const int *keep, int page, void *stream) {
   const char *fn = "lmoe_pages_free";
-  LMOE_REQUIRE(pages > 0 && B >= 0 && width > 0, LMOE_ESHAPE, "%s: %d pages, %d sequences of %d places", fn, pages, B, width);
+  LMOE_REQUIRE(pages_ok(pages) && B >= 0 && width > 0, LMOE_ESHAPE, "%s: %d pages, %d sequences of %d places", fn, pages, B, width);
   LMOE_REQUIRE(page_shift(page) > 0, LMOE_ESHAPE, "%s: pages of %d tokens (32, 64 and 128 are served)", fn, page);
   const long long places = (long long)B * width, groups = (places + 255) / 256;
   LMOE_REQUIRE(groups <= kMostGroups, LMOE_ESHAPE, "%s: %d sequences of %d places are more than a launch takes", fn, B, width);
@@ -325,7 +372,7 @@ extern "C" int lmoe_pages_free(int *refs, int pages, int *table, int B, int widt
 extern "C" int lmoe_pages_fork(int *refs, int pages, const int *table, int B, int width, const int *parents, int n, int *out,
                                void *stream) {
   const char *fn = "lmoe_pages_fork";
-  LMOE_REQUIRE(pages > 0 && B >= 0 && n >= 0 && width > 0, LMOE_ESHAPE, "%s: %d pages, %d sequences of %d places, %d new ones", fn,
+  LMOE_REQUIRE(pages_ok(pages) && B >= 0 && n >= 0 && width > 0, LMOE_ESHAPE, "%s: %d pages, %d sequences of %d places, %d new ones", fn,
                pages, B, width, n);
   const long long groups = ((long long)(B > n ? B : n) * width + 255) / 256;
   LMOE_REQUIRE(groups <= kMostGroups, LMOE_ESHAPE, "%s: %d and %d sequences of %d places are more than a launch takes", fn, B, n,
@@ -337,18 +384,31 @@ extern "C" int lmoe_pages_fork(int *refs, int pages, const int *table, int B, in
   return 0;
 }
 
-extern "C" int lmoe_pages_compact(int *refs, int pages, int *src, int *dst, int *used, int *to, void *stream) {
+extern "C" size_t lmoe_pages_compact_workspace_bytes(int pages) { return pages_ok(pages) ? size_t(stretches(pages) + 1) * sizeof(int) : 0; }
+
+extern "C" int lmoe_pages_compact(int *refs, int pages, int *src, int *dst, int *used, int *to, void *workspace, size_t workspace_bytes,
+                                  void *stream) {
   const char *fn = "lmoe_pages_compact";
-  LMOE_REQUIRE(pages > 0, LMOE_ESHAPE, "%s: %d pages", fn, pages);
+  LMOE_REQUIRE(pages_ok(pages), LMOE_ESHAPE, "%s: %d pages", fn, pages);
   LMOE_REQUIRE(refs && src && dst && used && to, LMOE_EINVAL, "%s: null pointer", fn);
-  launch(k_compact, dim3(1), dim3(kTakers), 0, (hipStream_t)stream, refs, pages, src, dst, pages > 1 ? pages / 2 : 1, used, to);
+  const size_t need = lmoe_pages_compact_workspace_bytes(pages);
+  LMOE_REQUIRE(workspace && aligned4(workspace) && workspace_bytes >= need, LMOE_EWORKSPACE, "%s: a workspace of %zu bytes is needed",
+               fn, need);
+  int *counts = static_cast<int *>(workspace);
+  hipStream_t st = (hipStream_t)stream;
+  const int n = stretches(pages), most = pages > 1 ? pages / 2 : 1;
+  launch(k_count, dim3(n), dim3(kTakers), 0, st, refs, pages, counts, 1);
+  LMOE_LAUNCHED(fn);
+  launch(k_moves, dim3(n), dim3(kTakers), 0, st, refs, pages, counts, src, dst, used, to);
+  LMOE_LAUNCHED(fn);
+  launch(k_move, dim3((most + 255) / 256), dim3(256), 0, st, refs, counts + n, src, dst, most, to);
   LMOE_LAUNCHED(fn);
   return 0;
 }
 
 extern "C" int lmoe_pages_renumber(int *table, int B, int width, int pages, const int *used, const int *to, void *stream) {
   const char *fn = "lmoe_pages_renumber";
-  LMOE_REQUIRE(pages > 0 && B >= 0 && width > 0, LMOE_ESHAPE, "%s: %d pages, %d sequences of %d places", fn, pages, B, width);
+  LMOE_REQUIRE(pages_ok(pages) && B >= 0 && width > 0, LMOE_ESHAPE, "%s: %d pages, %d sequences of %d places", fn, pages, B, width);
   const long long places = (long long)B * width, groups = (places + 255) / 256;
   LMOE_REQUIRE(groups <= kMostGroups, LMOE_ESHAPE, "%s: %d sequences of %d places are more than a launch takes", fn, B, width);
   if (B == 0) return 0;
@@ -363,7 +423,7 @@ extern "C" int lmoe_pages_copy(uint8_t *k_codes, float *k_scale, uint8_t *v_code
   const char *fn = "lmoe_pages_copy";
   LMOE_REQUIRE(D == 64 || D == 128 || D == 256, LMOE_ESHAPE, "%s: heads of %d channels (64, 128 and 256 are served)", fn, D);
   LMOE_REQUIRE(page_shift(page) > 0, LMOE_ESHAPE, "%s: pages of %d tokens (32, 64 and 128 are served)", fn, page);
-  LMOE_REQUIRE(pages > 0 && heads > 0 && n >= 0, LMOE_ESHAPE, "%s: %d pages of %d heads, %d copies", fn, pages, heads, n);
+  LMOE_REQUIRE(pages_ok(pages) && heads > 0 && n >= 0, LMOE_ESHAPE, "%s: %d pages of %d heads, %d copies", fn, pages, heads, n);
   if (n == 0) return 0;
   LMOE_REQUIRE(k_codes && k_scale && v_codes && v_scale && src && dst, LMOE_EINVAL, "%s: null pointer", fn);
   LMOE_REQUIRE(aligned16(k_codes) && aligned16(v_codes), LMOE_EALIGN, "%s: codes must be 16-byte aligned", fn);

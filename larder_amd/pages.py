@@ -52,6 +52,11 @@ def _take_workspace(*sizes):
     return _lib.lib().lmoe_pages_take_workspace_bytes(*sizes)
 
 
+@functools.lru_cache(maxsize=64)
+def _compact_workspace(pages):
+    return _lib.lib().lmoe_pages_compact_workspace_bytes(pages)
+
+
 def take_pages(refs, table, lens, cu=None, page=64):
     """Gives every place of the table that the newest rows fall into a page that is its sequence's alone: the lowest free one
     (refs 0 when the call begins) where it has none, or where its page has other holders. lens, cu as append_rows takes them (the
@@ -60,7 +65,7 @@ def take_pages(refs, table, lens, cu=None, page=64):
     (src, dst, lacking), int32 [sequences] each: the pages to copy before the rows are appended, where a sequence had shared
     a page that holds tokens before them (-1: none; a sequence has one at most), and how many of its places found no page left.
     Those hold -1 and what they shared is no longer theirs: append_rows writes nothing there, and such a sequence is cut
-    (free_pages) and taken up again when there is room."""
+    (free_pages) and taken up again when there is room. Tokens past the table's places have none, and lack none."""
     fn = "take_pages"
     pages, n, places = _pool(fn, refs, table)
     _page(fn, page)
@@ -135,7 +140,10 @@ def compact_pages(refs, *tables):
     pages = refs.shape[0]
     src, dst = (refs.new_empty(max(pages // 2, 1)) for _ in range(2))
     used, to = refs.new_empty(1), refs.new_empty(pages)
-    _launch(dev, "lmoe_pages_compact", refs.data_ptr(), pages, src.data_ptr(), dst.data_ptr(), used.data_ptr(), to.data_ptr())
+    need = _compact_workspace(pages)
+    ws = refs.new_empty(need, dtype=torch.uint8)
+    _launch(dev, "lmoe_pages_compact", refs.data_ptr(), pages, src.data_ptr(), dst.data_ptr(), used.data_ptr(), to.data_ptr(),
+            ws.data_ptr(), need)
     for t, (_, n, places) in zip(tables, sizes):
         if n:
             _launch(dev, "lmoe_pages_renumber", t.data_ptr(), n, places, pages, used.data_ptr(), to.data_ptr())

@@ -3,7 +3,8 @@
     qmv_fits(x, w, scales, group_size, bits, mode, biases)   route_cuda.py:516-522
     qmv_rows(x, w, scales, biases, group_size)               route_cuda.py:525-541 (lmoe_qmv_rows)
     shared_expert_rows(x, gate, up, down)                    mlx_lm's shared_expert MLP on qmv_rows projections
-    attention_rows(x, qkv, out, cache, table, lens, ...)     rotary attention on qmv_rows projections and the paged cache
+    attention_rows(x, qkv, out, cache, table, lens, ...)     rotary attention on qmv_rows projections and the paged cache,
+                                                             its heads normed first where asked
     norm_rows(x, weight, eps, residual, group, total)        root-mean-square norm, after the residual's addition
     read_codes(codes, scales, dtype)                         rows that norm_rows gave in 8 bits
 
@@ -66,14 +67,17 @@ def shared_expert_rows(x, gate, up, down):
 
 
 def attention_rows(x, qkv, out, cache, table, lens, cu=None, freq=None, interleaved=False, gain=1.0, prompt=None,
-                   most_rows=None, longest=None):
-    """The trunk's attention of x [T, H] bf16 (larder_amd.attention's packed rows): out(attend(rotate(qkv(x)))), with qkv and
+                   most_rows=None, longest=None, norms=None):
+    """The trunk's attention of x [T, H] bf16 (larder_amd.attention's packed rows): out(attend(rotate(norm(qkv(x))))), with qkv and
     out (w, scales, biases, group_size) 4-bit affine weights run through qmv_rows, qkv's output the query heads, then the key
-    heads, then the value heads of the cache's width. Nothing else stands between the steps: a model with biases on q, k and v,
-    norms of q's and k's heads before the rotation, or a gate on the output calls larder_amd.attention's parts itself. The rows'
-    keys and values are written to the cache, then read by
+    heads, then the value heads of the cache's width. norms (query weight, key weight, eps): the heads of q and k are normed by
+    norm_rows before their rotation (None: they are not). Nothing else stands between the steps: a model with biases on q, k and
+    v, or a gate on the output calls larder_amd.attention's parts itself. The rows' keys and values are written to the cache,
+    then read by
 
       prompt None              the newest rows of each sequence over its cached tokens (attend_rows; most_rows, longest its)
+      prompt "chunk"           many new rows of each sequence over its cached tokens, straight from the pages: a prompt's first
+                               or a later chunk (chunk_rows; longest its). All keys and values are in the cache's 8 bits
       prompt True              sequences that begin with this call, over the call's own keys and values (prompt_rows)
       prompt (cu_k, total)     later chunks of prompts: over all the cached tokens, lens of each, total in all, cu_k int32
                                [sequences + 1] where each begins (read_rows, prompt_rows); none of them in a page that is
@@ -84,9 +88,11 @@ def attention_rows(x, qkv, out, cache, table, lens, cu=None, freq=None, interlea
     # what a later call would refuse is refused here, before the cache is written
     if prompt is not None and cu is None:
         raise ValueError("attention_rows: a prompt's rows need their offsets cu")
-    whole = prompt is True
+    whole, chunk = prompt is True, prompt == "chunk" if isinstance(prompt, str) else False
+    if isinstance(prompt, str) and not chunk:
+        raise ValueError(f"attention_rows: prompt {prompt!r} is not \"chunk\"")
     cu_k = total = None
-    if prompt is not None and not whole:
+    if prompt is not None and not whole and not chunk:
         cu_k, total = prompt
         cu_k = attention._ints("attention_rows", "cu_k", cu_k, table.shape[0] + 1)
         if cu_k.device != x.device or total < 0:
@@ -99,9 +105,13 @@ def attention_rows(x, qkv, out, cache, table, lens, cu=None, freq=None, interlea
     if not qmv_fits(y[:, :q_heads * width], w, scales, group_size, 4, "affine", biases):
         raise ValueError(f"attention_rows: out is a 4-bit affine weight of {q_heads} heads of {width}")
     q, k, v = y.view(t, y.shape[1] // width, width).split([q_heads, heads, heads], 1)
+    if norms is not None:
+        q, k = norm_rows(q, norms[0], norms[2]), norm_rows(k, norms[1], norms[2])
     q, k = attention.append_rows(cache, q, k, v, table, lens, cu=cu, freq=freq, interleaved=interleaved, gain=gain, keys=whole)
     if prompt is None:
         o = attention.attend_rows(q, cache, table, lens, cu=cu, most_rows=most_rows, longest=longest)
+    elif chunk:
+        o = attention.chunk_rows(q, cache, table, lens, cu, longest=longest)
     elif whole:
         o = attention.prompt_rows(q, k, v, cu)
     else:

@@ -380,3 +380,27 @@ def test_serving_run():
         assert torch.equal(x.nan_to_num(7.0), y.nan_to_num(7.0))
     assert int(table.max()) < u
     step([5, 1, 1, 40, 1, 1])
+
+
+def test_trunk_attention_rows_in_chunks():
+    """The trunk's call with norms of the heads and chunks over the pages: equal to its parts, a token among them."""
+    from larder_amd import attention, trunk
+    from test_gpu_attention import affine4
+    rng = np.random.default_rng(18)
+    hidden, q_heads, heads, width = 512, 4, 1, 128
+    qkv, out = affine4(rng, (q_heads + 2 * heads) * width, hidden), affine4(rng, hidden, q_heads * width)
+    norms = (normal(rng, width), normal(rng, width), 1e-5)
+    freq, _ = attention.rotary_freq(64)
+    table = ints([[1, 0, 2]])
+    caches = [attention.KVCache.empty(3, heads, width) for _ in range(2)]
+    for lens, n, prompt in ((66, 66, "chunk"), (100, 34, "chunk"), (101, 1, None)):
+        x, cu = normal(rng, n, hidden), ints([0, n])
+        got = trunk.attention_rows(x, qkv, out, caches[0], table, ints([lens]), cu=cu, freq=freq, prompt=prompt, norms=norms)
+        q, k, v = trunk.qmv_rows(x, *qkv).view(n, -1, width).split([q_heads, heads, heads], 1)
+        q, k = (trunk.norm_rows(y, w, norms[2]) for y, w in zip((q, k), norms))
+        q, _ = attention.append_rows(caches[1], q, k, v, table, ints([lens]), cu=cu, freq=freq)
+        o = (attention.chunk_rows if prompt else attention.attend_rows)(q, caches[1], table, ints([lens]), cu)
+        assert torch.equal(got, trunk.qmv_rows(o.reshape(n, -1), *out))
+        check(o, q, caches[1], np.array([[1, 0, 2]]), [lens], [0, n], width ** -0.5, BF16)
+    none = trunk.attention_rows(x[:0], qkv, out, caches[0], table, ints([101]), cu=ints([0, 0]), freq=freq, prompt="chunk", norms=norms)
+    assert none.shape == (0, hidden)

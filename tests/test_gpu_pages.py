@@ -42,7 +42,8 @@ def pool(rng, pages, n, places, page, share=0.4, fill=0.5):
 
 
 SIZES = [(1, 1, 1, 32), (7, 3, 2, 64), (64, 5, 9, 128), (1000, 40, 30, 64), (5000, 64, 70, 32), (1024, 1500, 3, 64),
-         (2048, 2100, 4, 32), (70000, 9, 1100, 64)]
+         (2048, 2100, 4, 32), (70000, 9, 1100, 64), (16384, 20, 300, 64), (16385, 3, 5, 32),
+         (200000, 5, 3, 128)]
 
 
 @pytest.mark.parametrize("pages,n,places,page", SIZES)
