@@ -546,8 +546,12 @@ extern "C" int lmoe_kv_chunk(const void *q, int dtype, long long q_row, long lon
                q_heads / heads);
   const ChunkPlan plan = chunk_plan(T, q_heads, heads, D, B, longest);
   const long long groups = plan.tiles * heads * plan.chunks;
-  LMOE_REQUIRE(groups <= kMostGroups && ((long long)T * q_heads * (D / 4) + 255) / 256 <= (plan.bytes ? kMostGroups : 1ll << 62),
-               LMOE_ESHAPE, "%s: %d rows of %d sequences and %d heads are more than a launch takes", fn, T, B, q_heads);
+  // A workgroup joins one line by all of its threads from eight chunks on (48 rows of 32 heads in 42 chunks: 14.4 us with D / 4
+  // threads a line, 10.3 so)
+  const bool shared = plan.chunks >= 8;
+  const long long join_groups = !plan.bytes ? 0 : shared ? (long long)T * q_heads : ((long long)T * q_heads * (D / 4) + 255) / 256;
+  LMOE_REQUIRE(groups <= kMostGroups && join_groups <= kMostGroups, LMOE_ESHAPE,
+               "%s: %d rows of %d sequences and %d heads are more than a launch takes", fn, T, B, q_heads);
   LMOE_REQUIRE(plan.bytes == 0 || (workspace && aligned16(workspace) && workspace_bytes >= plan.bytes), LMOE_EWORKSPACE,
                "%s: a 16-byte aligned workspace of %zu bytes is needed", fn, plan.bytes);
   float *part = plan.bytes ? static_cast<float *>(workspace) : nullptr;
@@ -556,14 +560,14 @@ extern "C" int lmoe_kv_chunk(const void *q, int dtype, long long q_row, long lon
                  static_cast<uint16_t *>(out), part, joins, scale * 1.4426950408889634f, T, B, q_heads, heads, q_heads / heads, pages,
                  width, page == 32 ? 5 : page == 64 ? 6 : 7, int(plan.tiles), plan.chunk, plan.chunks,
                  groups > (D == 256 || plan.waves == 8 ? 256 : 512)};
-  auto go = [&](auto kernel, auto join) -> int {
+  auto go = [&](auto kernel, auto join, auto join_shared) -> int {
     // two stages of a tile of keys and of values; sums in float32, which the wavefronts store through LDS, may take more
     const size_t tiles = size_t(kPromptKeys) * D * 2 * 4, sums = part ? size_t(plan.waves) * 32 * D * 4 : 0, lds = tiles > sums ? tiles : sums;
     if (const int rc = allow_lds(kernel, lds + 4128, fn)) return rc;  // with what the kernel declares itself
     launch(kernel, dim3(unsigned(groups)), dim3(unsigned(64 * plan.waves)), lds, (hipStream_t)stream, a);
     LMOE_LAUNCHED(fn);
     if (part) {
-      launch(join, dim3(unsigned(((long long)T * q_heads * (D / 4) + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
+      launch(shared ? join_shared : join, dim3(unsigned(join_groups)), dim3(256), 0, (hipStream_t)stream,
              JoinArgs{a.out, part, joins, T, q_heads, plan.chunks});
       LMOE_LAUNCHED(fn);
     }
@@ -571,8 +575,8 @@ extern "C" int lmoe_kv_chunk(const void *q, int dtype, long long q_row, long lon
   };
   auto type = [&](auto d, auto waves) -> int {
     constexpr int W = decltype(d)::value, NW = decltype(waves)::value;
-    return dtype == LMOE_BF16 ? go(k_chunk_rows<W, true, NW>, k_join_chunks<W, true>)
-                              : go(k_chunk_rows<W, false, NW>, k_join_chunks<W, false>);
+    return dtype == LMOE_BF16 ? go(k_chunk_rows<W, true, NW>, k_join_chunks<W, true>, k_join_chunks<W, true, 1024 / W>)
+                              : go(k_chunk_rows<W, false, NW>, k_join_chunks<W, false>, k_join_chunks<W, false, 1024 / W>);
   };
   if (D == 64) return type(IC<64>{}, IC<4>{});
   if (D == 128) return plan.waves == 8 ? type(IC<128>{}, IC<8>{}) : type(IC<128>{}, IC<4>{});

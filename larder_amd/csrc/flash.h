@@ -107,33 +107,50 @@ struct JoinArgs {
   const int *joins;   // [T][q_heads]: how many chunks (0: the row is done)
   int T, q_heads, chunks;
 };
-template <int D, bool BF>
+// G: groups of D / 4 threads that share a line's chunks, every Gth each, where there are many chunks and few lines
+template <int D, bool BF, int G = 1>
 static __global__ void __launch_bounds__(256) k_join_chunks(JoinArgs a) {
   constexpr int LANES = D / 4;
-  const size_t line = size_t(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES, lines = size_t(a.T) * a.q_heads;
-  if (line >= lines) return;
-  const int parts = min(a.joins[line], a.chunks), d = (threadIdx.x % LANES) * 4;
-  if (parts < 2) return;
+  const int thread = threadIdx.x % LANES, group = threadIdx.x / LANES % G;
+  const size_t line = size_t(blockIdx.x) * (256 / (LANES * G)) + threadIdx.x / (LANES * G), lines = size_t(a.T) * a.q_heads;
+  if (G == 1 && line >= lines) return;
+  const int parts = line < lines ? min(a.joins[line], a.chunks) : 0, d = thread * 4;
+  if (G == 1 && parts < 2) return;
   f32x4 v = {};
   float top = -INFINITY, weight = 0.0f;
-  for (int c0 = 0; c0 < parts; c0 += 4) {
+  auto join = [&](float m, float l, f32x4 y) {
+    if (l == 0.0f) return;  // (a chunk that the row sees nothing of weighs 0; NaN goes on)
+    const float to = fmaxf(top, m), f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+    const float keep = weight == 0.0f ? 0.0f : to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - to);
+    top = to;
+    weight = fmaf(l, f, weight * keep);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = fmaf(y[e], f, v[e] * keep);
+  };
+  for (int c0 = group; c0 < parts; c0 += 4 * G) {
     float2 ml[4];
     f32x4 y[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float *part = a.part + (size_t(min(c0 + j, parts - 1)) * lines + line) * (D + 4);
+      const float *part = a.part + (size_t(min(c0 + j * G, parts - 1)) * lines + line) * (D + 4);
       ml[j] = *reinterpret_cast<const float2 *>(part + D);
       y[j] = *reinterpret_cast<const f32x4 *>(part + d);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (c0 + j >= parts || ml[j].y == 0.0f) continue;  // (a chunk that the row sees nothing of weighs 0; NaN goes on)
-      const float to = fmaxf(top, ml[j].x), f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml[j].x - to);
-      const float keep = weight == 0.0f ? 0.0f : to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - to);
-      top = to;
-      weight = fmaf(ml[j].y, f, weight * keep);
+    for (int j = 0; j < 4; ++j)
+      if (c0 + j * G < parts) join(ml[j].x, ml[j].y, y[j]);
+  }
+  if constexpr (G > 1) {
+    __shared__ float sums[256][6];
+    float *mine = sums[threadIdx.x];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = fmaf(y[j][e], f, v[e] * keep);
+    for (int e = 0; e < 4; ++e) mine[e] = v[e];
+    mine[4] = top, mine[5] = weight;
+    __syncthreads();
+    if (group || parts < 2) return;
+    for (int g = 1; g < G; ++g) {
+      const float *other = sums[threadIdx.x + g * LANES];
+      join(other[4], other[5], f32x4{other[0], other[1], other[2], other[3]});
     }
   }
   const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;

@@ -7,8 +7,10 @@
 // the product. float32 inside: y is of the sum before that is rounded, one rounding each for y (or its code) and for s.
 //
 // A row is taken by `lanes` neighbouring threads, eight channels a thread and step: 8 to 64 lanes of a wavefront (up to 512
-// channels, several rows a workgroup), or a workgroup of 256 (up to 16,384 in registers, longer ones read twice, the second
-// time from L2). Rows may begin anywhere: loads and stores are of 16 bytes whatever their alignment (the hardware splits what
+// channels, 1,536 where rows are many; several rows a workgroup), or a workgroup of 256 (up to 16,384 in registers, longer ones
+// read twice, the second time from L2). Measured: 8,192 rows of 4,096 in bf16 with their residual 48.6-53.7 us, 5.0-5.5 TB/s
+// (with codes 51, read back 19); 2,048 rows of 32 heads of 128 7.9; one row 2.8 of kernel under 9 of the call; 4,000 rows of an
+// odd 5,001 3.6 TB/s, 2,000 of 20,000 3.1. Rows may begin anywhere: loads and stores are of 16 bytes whatever their alignment (the hardware splits what
 // crosses a line), and the last, partial eight go one by one.
 #include "codes.h"
 
@@ -343,7 +345,11 @@ __global__ void __launch_bounds__(256) k_read_codes(CodesArgs a) {
 template <int DT>
 static int go_norm(const char *fn, const NormArgs &a, hipStream_t st) {
   const int chunks = (a.H + 7) / 8;
-  const int lanes = chunks <= 8 ? 8 : chunks <= 16 ? 16 : chunks <= 32 ? 32 : chunks <= 64 ? 64 : 256;
+  // A wavefront a row where there are many that would leave a quarter or more of a workgroup's threads without channels (16,000
+  // rows of 513, bf16, residual: 21.5 -> 16.3 us; 8,000 of 1,111: 26.4 -> 23.3; 16,384 of 2,048 lose, 45 -> 55). Few rows take a
+  // workgroup each, for latency
+  const bool many = a.rows >= 2048 && chunks <= 192;
+  const int lanes = chunks <= 8 ? 8 : chunks <= 16 ? 16 : chunks <= 32 ? 32 : chunks <= 64 || many ? 64 : 256;
   const long long groups = (a.rows + 256 / lanes - 1) / (256 / lanes);
   LMOE_REQUIRE(groups <= (1ll << 24) - 1, LMOE_ESHAPE, "%s: %lld rows are more than a launch takes", fn, a.rows);
   auto go = [&](auto kernel) -> int {
@@ -355,7 +361,7 @@ static int go_norm(const char *fn, const NormArgs &a, hipStream_t st) {
     case 8: return go(k_norm<DT, 8, 1>);
     case 16: return go(k_norm<DT, 16, 1>);
     case 32: return go(k_norm<DT, 32, 1>);
-    case 64: return go(k_norm<DT, 64, 1>);
+    case 64: return chunks <= 64 ? go(k_norm<DT, 64, 1>) : chunks <= 128 ? go(k_norm<DT, 64, 2>) : go(k_norm<DT, 64, 3>);
   }
   const int steps = (chunks + 255) / 256;
   return steps == 1   ? go(k_norm<DT, 256, 1>)

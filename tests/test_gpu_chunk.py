@@ -90,7 +90,7 @@ def test_chunk(dtype, q_heads, heads, width, page, longest):
     (4, 4, 64, 32, [700], [700]), (8, 1, 128, 64, [129, 500], [5000, 500]), (28, 4, 128, 32, [64, 200, 31], [4097, 1000, 9000]),
     (4, 2, 256, 64, [300], [4500]), (6, 2, 256, 128, [1, 90], [4200, 8300]), (1, 1, 128, 128, [1500], [1500]),
     (16, 2, 64, 64, [40] * 9, [4100, 64, 40, 1000, 41, 129, 8191, 8192, 8193]), (32, 4, 128, 64, [48], [20000]),
-    (4, 1, 64, 32, [2000], [6000])])
+    (4, 1, 64, 32, [2000], [6000]), (32, 4, 128, 64, [2048], [4096]), (32, 4, 128, 32, [600], [9001]), (16, 2, 128, 128, [5], [40000])])
 @pytest.mark.parametrize("longest", [None, 100])
 def test_chunk_long(dtype, q_heads, heads, width, page, rows, lens, longest):
     """Past 64 tiles of keys; keys in chunks (longest None) and in one (100)."""

@@ -69,7 +69,8 @@ def check(x, r, w, eps, **kw):
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("t,h", [(1, 1), (3, 7), (1, 64), (33, 65), (5, 100), (300, 128), (2, 255), (70, 512), (9, 513), (1, 2048),
-                                 (17, 2051), (4, 4096), (3, 5000), (2, 8191), (3, 16384), (2, 16385), (1, 20001)])
+                                 (17, 2051), (4, 4096), (3, 5000), (2, 8191), (3, 16384), (2, 16385), (1, 20001),
+                                 (2048, 513), (2300, 1024), (2049, 1100), (2050, 1536)])
 def test_norm(dtype, t, h):
     gen = torch.Generator(device="cuda").manual_seed(h)
     x, w = normal(gen, t, h, dtype=dtype) * torch.exp(normal(gen, h)).to(dtype), normal(gen, h, dtype=dtype)
