@@ -153,7 +153,19 @@ def test_chunk_holes_and_nan(dtype, longest, page, heads, width):
     got = attention.chunk_rows(q, cache, ints(table), ints(lens), ints(cu), longest=longest)
     check(got, q, cache, table, lens, cu, width ** -0.5, dtype)
     assert torch.isnan(got[43, :4, 5]).all() and not torch.isnan(got[42, :4, 5]).any()
-    # a sequence none of whose pages is there
+    # a page that is not there, far before the rows, in a cache whose first page is all NaN
+    far, most = page_table(rng, [9], width=9)
+    far = far + 1
+    deep = random_cache(rng, most + 1, heads, width, page)
+    for t in (deep.k, deep.v):
+        t.view(torch.uint8)[0] = 0x7f
+    far[0, 2] = -1
+    few = q[:40]
+    got = attention.chunk_rows(few, deep, ints(far), ints([9 * page]), ints([0, 40]), longest=longest)
+    check(got, few, deep, far, [9 * page], [0, 40], width ** -0.5, dtype)
+    assert not torch.isnan(got).any()
+    # a sequence none of whose pages is there, whatever the first page of the cache holds
+    v[0], k[0] = 0x7f, 0x7f
     gone = attention.chunk_rows(q, cache, ints(np.full_like(table, n)), ints(lens), ints(cu), longest=longest)
     assert (gone == 0).all()
 
