@@ -16,11 +16,14 @@
 // next tile's conversion are issued in one stream of slots, a product and about seven other instructions each. Tiles of keys lie
 // half a tile off those of values for that.
 //
-// Bound by the matrix cores (4 width products a visible pair), at the rate that their power allows: products alone on constant
-// data reach 2.2 PFLOP/s, the library's largest 1.21. Measured (2,048 rows over 34,816 tokens, 32 heads over 4 of 128, bf16): 1,052-
-// 1,078 us, 1.05-1.08 PFLOP/s; without LDS reads and staging 943. One after the other instead of slots 1,252; 128 pairs a workgroup
-// 1,158; 64 pairs a wavefront, which halves the LDS reads and leaves one wavefront a SIMD, 1,156. Width 256: one wavefront a SIMD,
-// 0.93-0.95 PFLOP/s where all places work. A short call's workgroup: 3.3 us to its first scores, 1.45 a tile, 2.5 of output.
+// Bound by the matrix cores (4 width products a visible pair), at the rate that their power allows: products alone reach 2.2-2.4
+// PFLOP/s on constant data and 1.84 on random data (the clock falls to 1.86 GHz); with six vector instructions beside each, which
+// is what the exponentials and the conversion need, 1.56; the library's largest product 1.21. Measured (2,048 rows over 34,816
+// tokens, 32 heads over 4 of 128, bf16): 1,052-1,078 us, 1.05-1.08 PFLOP/s; without LDS reads and staging 943. One after the
+// other instead of slots 1,252; 128 pairs a workgroup 1,158; 64 pairs a wavefront, which halves the LDS reads and leaves one
+// wavefront a SIMD (it issues a vector instruction every eight or nine cycles, each of two every four or five), 1,156; codes two
+// tiles ahead, or loads of single lanes' addresses, 1-3 % more. Width 256: one wavefront a SIMD, 0.93-0.95 PFLOP/s where all
+// places work. A short call's workgroup: 3.3 us to its first scores, 1.45 a tile, 2.5 of output.
 //
 // Weights, their sums and values that are not finite: as in prompt.hip.
 #include <cmath>
