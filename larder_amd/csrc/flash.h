@@ -106,15 +106,26 @@ struct JoinArgs {
   const float *part;  // [chunks][T][q_heads] of [D] sums and {maximum, weight}
   const int *joins;   // [T][q_heads]: how many chunks (0: the row is done)
   int T, q_heads, chunks;
+  const int2 *placed = nullptr;  // PLACED: [T][q_heads] of the first piece's line in part (-1: the row is done) and the last one's
+  int next = 0, step = 0, most = 0;  // from the first piece's line to the second's, from there to each further one's; lines in all
 };
 // G: groups of D / 4 threads that share a line's chunks, every Gth each, where there are many chunks and few lines
-template <int D, bool BF, int G = 1>
+template <int D, bool BF, int G = 1, bool PLACED = false>
 static __global__ void __launch_bounds__(256) k_join_chunks(JoinArgs a) {
   constexpr int LANES = D / 4;
   const int thread = threadIdx.x % LANES, group = threadIdx.x / LANES % G;
   const size_t line = size_t(blockIdx.x) * (256 / (LANES * G)) + threadIdx.x / (LANES * G), lines = size_t(a.T) * a.q_heads;
   if (G == 1 && line >= lines) return;
-  const int parts = line < lines ? min(a.joins[line], a.chunks) : 0, d = thread * 4;
+  const int d = thread * 4;
+  int parts = 0, from = 0;
+  if constexpr (PLACED) {
+    const int2 place = line < lines ? a.placed[line] : int2{-1, 0};
+    from = place.x;
+    const int rest = min(place.y, a.most - 1) - from - a.next;
+    parts = from < 0 || from >= a.most || rest < 0 ? 0 : 2 + rest / a.step;
+  } else if (line < lines) {
+    parts = min(a.joins[line], a.chunks);
+  }
   if (G == 1 && parts < 2) return;
   f32x4 v = {};
   float top = -INFINITY, weight = 0.0f;
@@ -132,7 +143,9 @@ static __global__ void __launch_bounds__(256) k_join_chunks(JoinArgs a) {
     f32x4 y[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float *part = a.part + (size_t(min(c0 + j * G, parts - 1)) * lines + line) * (D + 4);
+      const int c = min(c0 + j * G, parts - 1);
+      const float *part =
+          a.part + (PLACED ? size_t(from + (c ? a.next + (c - 1) * a.step : 0)) : size_t(c) * lines + line) * (D + 4);
       ml[j] = *reinterpret_cast<const float2 *>(part + D);
       y[j] = *reinterpret_cast<const f32x4 *>(part + d);
     }

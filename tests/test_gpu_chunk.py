@@ -128,6 +128,31 @@ def test_chunk_many_sequences(dtype, n, rows):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("q_heads,heads,width,page", [(7, 1, 128, 32), (4, 4, 64, 32), (16, 1, 256, 64), (3, 3, 128, 128), (200, 1, 64, 32)])
+@pytest.mark.parametrize("kind", ["few", "many", "one"])
+def test_chunk_far_shorter_than_said(dtype, q_heads, heads, width, page, kind):
+    """`longest` far above the lengths, so that a call is laid out for long ones: few and short pieces, tiles that are shared and
+    tiles that are not, sequences without rows between, more than 64 of them in a row, rows before and behind."""
+    from larder_amd import attention
+    rng = np.random.default_rng(31 * q_heads + width)
+    if kind == "few":
+        rows, lens = [5, 0, 90, 1, 0, 33], [200, 64, 1500, 129, 3, 1021]
+    elif kind == "one":
+        rows, lens = [130], [777]
+    else:
+        rows = [int(x) for x in rng.choice([0, 1, 2, 40], 90)] + [0] * 150 + [3] + [0] * 70 + [65, 0]
+        lens = [int(x) for x in rng.choice([0, 1, 63, 65, 300, 500], len(rows))]
+    cu = [2] + [2 + int(x) for x in np.cumsum(rows)]
+    table, n = page_table(rng, [-(-x // page) for x in lens], width=65536 // page)
+    cache = random_cache(rng, n, heads, width, page)
+    q = normal(rng, cu[-1] + 3, q_heads, width, dtype=dtype)
+    got = attention.chunk_rows(q, cache, ints(table), ints(lens), ints(cu))
+    assert (got[:2] == 0).all() and (got[cu[-1]:] == 0).all()
+    check(got, q, cache, table, lens, cu, width ** -0.5, dtype)
+    assert torch.equal(got, attention.chunk_rows(q, cache, ints(table), ints(lens), ints(cu)))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("longest", [None, 64])
 @pytest.mark.parametrize("page,heads,width", [(32, 2, 128), (64, 1, 64), (32, 1, 256)])
 def test_chunk_holes_and_nan(dtype, longest, page, heads, width):

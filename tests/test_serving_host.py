@@ -1,6 +1,7 @@
 """Host logic of the norms, the pages and the chunks over the cache: refusals, workspaces and what a launch covers, without a
 GPU."""
 import ctypes
+import math
 import random
 
 import numpy as np
@@ -114,13 +115,12 @@ def test_chunks_refuse(built_lib):
 
 
 def test_chunk_workspace(built_lib):
-    """One place for a row, head and chunk of keys: width sums, a maximum and a weight; how many chunks a row has. A long history
+    """Two places for each workgroup's pairs: width sums, a maximum and a weight; where each row and head has its own. A long history
     under few rows is split, many rows are not, and the largest sizes stay in bounds."""
     f = built_lib.lmoe_kv_chunk_workspace_bytes
     for t, q, h, d, b, n in ((48, 32, 4, 128, 1, 131048), (17, 4, 4, 64, 3, 2 ** 31 - 1), (100, 16, 2, 256, 5, 9000)):
-        line = t * q * (d + 4) * 4
-        chunks, rest = divmod(f(t, q, h, d, b, n), line)
-        assert chunks > 1 and rest == t * q * 4
+        groups, rest = divmod(f(t, q, h, d, b, n) - t * q * 8, 2 * 128 * (d + 4) * 4)
+        assert rest == 0 and groups % h == 0 and h < groups <= (256 if d == 256 else 512)
     assert f(8192, 32, 4, 128, 1, 8192) == 0 and f(48, 32, 4, 128, 1, 60) == 0
     assert f(0, 4, 4, 64, 1, 100) == 0 and f(4, 3, 2, 64, 1, 100) == 0 and f(4, 4, 4, 64, 0, 100) == 0
 
@@ -194,3 +194,64 @@ def test_the_trunks_attention_in_chunks_refuses_before_it_writes(monkeypatch):
         with pytest.raises(ValueError, match=why):
             trunk.attention_rows(torch.zeros(2, 128, dtype=torch.bfloat16), **{**args, **kw})
     assert not written
+
+
+@pytest.mark.parametrize("rows", [128, 256])
+def test_stretches_hold_every_key_once(rows):
+    """TileLine's two ways of cutting a head's tiles, restated: stretches one behind another hold every tile's keys once, in order,
+    none but a tile's first piece without keys, and two stretches never begin inside a tile at the same key."""
+    rng = random.Random(rows + 1)
+    for turn in range(400):
+        group, n, room = rng.choice([1, 2, 3, 7, 8, 40, 200]), rng.choice([1, 1, 2, 5, 64, 70]), rng.choice([64, 640, 10 ** 9])
+        counts = [rng.choice([0, 1, 3, 17, 128, 700]) for _ in range(n)]
+        lens = [rng.choice([0, 1, c // 2, c, c + 63, c + 64, c + 1000, c + 30000]) for c in counts]
+        tiles = [-(-c * group // rows) for c in counts]
+
+        def seen(b, t):
+            return min(lens[b] - counts[b] + (min(t * rows + rows, counts[b] * group) - 1) // group + 1, room)
+
+        def cost(b, t):
+            return t * (group * (max(lens[b] - counts[b], 0) + 192) + rows / 2 * (t + 1))
+
+        want = [(b, t) for b in range(n) for t in range(tiles[b])]
+        total = sum(cost(b, tiles[b]) for b in range(n))
+        of = rng.choice([2, 3, 16, 60, 128, 512])
+
+        def place(x):
+            for b in range(n):
+                if x < cost(b, tiles[b]):
+                    t = max(t for t in range(tiles[b]) if cost(b, t) <= x)
+                    key = int(max((x - cost(b, t)) / group - 192, 0.0)) & -64
+                    return (b, t + 1, 0) if key and seen(b, t) - key < 64 else (b, t, key)
+                x -= cost(b, tiles[b])
+            return (n, 0, 0)
+
+        each = total / of
+        if each / group < 128:
+            of = max(int(total / group / 128), 1)
+            each = total / of
+        ends = [place(math.floor(each * i)) for i in range(of)] + [(n, 0, 0)]
+        ways = [list(zip(ends, ends[1:]))]
+        if n == 1 and tiles[0]:
+            per = rng.choice([2, 3, 8, 42])
+            cut = []
+            for one in range(tiles[0] * per):
+                t, i = divmod(one, per)
+                step = ((max(seen(0, t), 1) - 1) // (per * 64) + 1) * 64
+                if i == 0 or i < -(-seen(0, t) // step):
+                    cut.append(((0, t, i * step), (0, t, (i + 1) * step) if (i + 1) * step < seen(0, t) else (0, t + 1, 0)))
+            ways.append(cut)
+        for stretches in ways:
+            held = []
+            for (b, t, key), end in stretches:
+                while b < n and (b, t, key) < end:
+                    if t >= tiles[b]:
+                        b, t, key = b + 1, 0, 0
+                        continue
+                    stop = min(seen(b, t), end[2]) if end[:2] == (b, t) else seen(b, t)
+                    assert key == 0 or stop > key
+                    held.append((b, t, key, stop))
+                    t, key = t + 1, 0
+            assert [x[:2] for x in held if x[2] == 0] == want
+            for a, z in zip(held, held[1:] + [(n, 0, 0, 0)]):
+                assert z[2] == a[3] and z[:2] == a[:2] if z[2] else a[3] == seen(*a[:2])
