@@ -419,14 +419,15 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) k_chunk_rows(ChunkA
     // a transposing load: 16 lanes take 4 keys x 16 channels, lane i of them gets channel i of the 4
     const int vrow = 4 * h + ((lane & 15) >> 2), vpair = (lane >> 4) & 1, vbyte = (lane & 3) * 8;
     auto k_frag = [&](const uint8_t *kt, int x, int j) {
-      return *reinterpret_cast<const u32x4 *>(kt + (32 * x + r) * D * 2 + k_chunk<D>(r, 2 * j + h) * 16);
+      // (256 bytes apart the swizzle is the same: eight addresses for all of them)
+      return *reinterpret_cast<const u32x4 *>(kt + (32 * x + r) * D * 2 + k_chunk<D>(r, 2 * (j & 7) + h) * 16 + (j >> 3) * 256);
     };
     auto v_frag = [&](const uint8_t *vt, int ks, int d) {
       u32x4 f;
   #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int row = 16 * ks + 8 * x + vrow;
-        const uint8_t *src = vt + row * D * 2 + v_pair<D>(vrow, 2 * d + vpair) * 32 + vbyte;
+        const uint8_t *src = vt + row * D * 2 + v_pair<D>(vrow, 2 * (d & 3) + vpair) * 32 + (d >> 2) * 256 + vbyte;
         const u32x2 g = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(src)));
         f[2 * x] = g.x, f[2 * x + 1] = g.y;
       }
