@@ -684,8 +684,10 @@ static ChunkPlan chunk_plan(int T, int q_heads, int heads, int D, int B, int lon
     auto fewest = [&](double key) { return B == 1 ? fmax(longest - T, 0.0) * key + ends : ends; };
     auto mean = [&](double key) { return B == 1 ? (most(key) + fewest(key)) / 2.0 : 0.5 * longest * key + ends; };
     const double alone = D == 256 ? 0.1 : waves == 8 ? 0.15 : 0.3, key = full * (1.0 - alone + alone * fmin(rounds, 1.0));
-    look(0, 0, fmax(fmax(most(key), B == 1 ? ceil(rounds) * fewest(key) : 0.0),
-                    rounds * mean(key) + (B == 1 ? 0.5 * fewest(key) : 0.35 * most(key) / fmax(1.0, rounds))));
+    // (the last round's end: of one sequence, half of a tile; of several, sorted, less the more there are)
+    const double rest = B == 1 ? 0.5 * fewest(key) : 0.35 * most(key) / rounds;
+    const double least_of = fmax(most(key), B == 1 ? ceil(rounds) * fewest(key) : 0.0);
+    look(0, 0, rounds <= 1.0 ? most(key) : fmax(least_of, rounds * mean(key) + rest));
     const double held = double(T) * group / tiles;  // rows of a piece
     auto price = [&](long long pieces) { return pieces * heads * held * (D + 4.0) * 8.0 / 4e6; };
     auto fits = [&](long long n) { return n >= 2 && n * heads <= places && n <= tiles * longest / kLeastStretch; };
