@@ -120,7 +120,7 @@ __device__ __forceinline__ ChunkTile nth_chunk_tile(const ChunkArgs &a, int nth)
 // call may be laid out as one line instead, all tiles one behind another, cut into as many equal stretches as a head has places:
 // a workgroup works what its stretch holds, the end of one tile, whole ones and the beginning of another, say. Tile t of a
 // sequence takes kTileStart, and a key for each that its last row sees: past + (t + 1) ROWS / group.
-constexpr int kTileStart = 192;    // what a tile's beginning and end take, in keys
+constexpr int kTileStart = 192;     // what a tile's beginning and end take, in keys
 constexpr int kLeastStretch = 128;  // keys: two do not begin at the same 64 keys of a tile then
 struct LinePlace {
   int b, tile, key;  // key: a multiple of a tile of keys, below what the tile's last row sees
@@ -206,7 +206,7 @@ struct TileLine {
       hi = min(hi, lo + step);
     }
     const double at = (x - cost(off, lo)) * a.per_group - kTileStart;
-    int key = int(fmin(fmax(at, 0.0), 0x1p30)) & -kPromptKeys;
+    int key = int(fmin(fmax(at, 0.0), double(0x7fffffff))) & -kPromptKeys;
     if (key && seen(off, lo, its_n * a.group) - key < kPromptKeys) ++lo, key = 0;
     return {b + i, lo, key};
   }
@@ -216,12 +216,13 @@ struct TileLine {
     const int tile = one / per, i = one - tile * per;
     *from = *to = {a.B, 0, 0};
     if ((long long)tile * ROWS >= (long long)n * a.group) return;
-    const int most = seen(len - n, tile, n * a.group), step = ((max(most, 1) - 1) / (per * kPromptKeys) + 1) * kPromptKeys;
-    if (i > 0 && i >= (most + step - 1) / step) return;
+    // (pieces' ends pass 31 bits where a table has room for as many tokens)
+    const uint32_t most = max(seen(len - n, tile, n * a.group), 1), step = ((most - 1) / uint32_t(per * kPromptKeys) + 1) * kPromptKeys;
+    const uint32_t begin = i * step;
+    if (i > 0 && begin >= most) return;
     *first = {0, 0, row0, n, len};
-    *from = {0, tile, i * step};
-    if ((i + 1) * step < most) *to = {0, tile, (i + 1) * step};
-    else *to = {0, tile + 1, 0};
+    *from = {0, tile, int(begin)};
+    *to = begin + step < most ? LinePlace{0, tile, int(begin + step)} : LinePlace{0, tile + 1, 0};
   }
   // how many keys a tile's last row sees
   __device__ __forceinline__ int seen(int off, int tile, int pairs) const {
