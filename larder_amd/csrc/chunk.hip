@@ -119,13 +119,14 @@ __device__ __forceinline__ ChunkTile nth_chunk_tile(const ChunkArgs &a, int nth)
 // Where one workgroup of a key head takes all of a tile's keys, the longest tile decides, and few tiles leave places free. So a
 // call may be laid out as one line instead, all tiles one behind another, cut into as many equal stretches as a head has places:
 // a workgroup works what its stretch holds, the end of one tile, whole ones and the beginning of another, say. Tile t of a
-// sequence takes kTileStart, and a key for each that its last row sees: past + (t + 1) ROWS / group.
-constexpr int kTileStart = 192;     // what a tile's beginning and end take, in keys
+// sequence takes START, what its beginning and end cost in keys, and a key for each that its last row sees: past + (t + 1) ROWS /
+// group. START is 192 where two workgroups share a CU, which hides a part of it, and 320 where one has it alone (12 sequences of 48 to
+// 700 rows over up to 9,700 tokens, 28 heads over 4 of 128: 264 -> 241 us; the former with 320 is 1 % slower).
 constexpr int kLeastStretch = 128;  // keys: two do not begin at the same 64 keys of a tile then
 struct LinePlace {
   int b, tile, key;  // key: a multiple of a tile of keys, below what the tile's last row sees
 };
-template <int ROWS>
+template <int ROWS, int START>
 struct TileLine {
   const ChunkArgs &a;
   int row0, n, len, tiles;  // of the lane's sequence
@@ -140,7 +141,7 @@ struct TileLine {
   // of the first t tiles of a sequence, times group (float64: a 64-bit product is an instruction; whole numbers below 2^53, and
   // past that places are rounded, in the same way for all)
   __device__ __forceinline__ double cost(int past, int t) const {
-    return double(t) * (double(a.group) * (max(past, 0) + kTileStart) + double(ROWS / 2) * (t + 1));
+    return double(t) * (double(a.group) * (max(past, 0) + START) + double(ROWS / 2) * (t + 1));
   }
   // of the lane's sequence and those before it in the wavefront (lanes past the last sequence: of some of them)
   __device__ __forceinline__ double ends() const {
@@ -205,7 +206,7 @@ struct TileLine {
       lo += step * (__popcll(__ballot(t < hi && cost(off, t) <= x)) - 1);
       hi = min(hi, lo + step);
     }
-    const double at = (x - cost(off, lo)) * a.per_group - kTileStart;
+    const double at = (x - cost(off, lo)) * a.per_group - START;
     int key = int(fmin(fmax(at, 0.0), double(0x7fffffff))) & -kPromptKeys;
     if (key && seen(off, lo, its_n * a.group) - key < kPromptKeys) ++lo, key = 0;
     return {b + i, lo, key};
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) k_chunk_rows(ChunkA
   };
   auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
   ChunkTile work;
-  [[maybe_unused]] TileLine<ROWS> line_of_tiles{a};
+  [[maybe_unused]] TileLine<ROWS, D == 256 || NW == 8 ? 320 : 192> line_of_tiles{a};
   [[maybe_unused]] LinePlace at_line, to_line;
   if constexpr (SPLIT) {
     const int one = int(blockIdx.x) / a.heads;
