@@ -19,7 +19,7 @@
 // Bound by the matrix cores (4 width products a visible pair), at the rate that their power allows: products alone reach 2.2-2.4
 // PFLOP/s on constant data and 1.84 on random data (the clock falls to 1.86 GHz); with six vector instructions beside each, which
 // is what the exponentials and the conversion need, 1.56; the library's largest product 1.21. Measured (2,048 rows over 34,816
-// tokens, 32 heads over 4 of 128, bf16): 1,030-1,078 us, 1.05-1.10 PFLOP/s, with float16, whose products take more power, 8 %
+// tokens, 32 heads over 4 of 128, bf16): 1,030-1,067 us, 1.06-1.10 PFLOP/s, with float16, whose products take more power, 8 %
 // more; without LDS reads and staging 943. One after the other instead of slots 1,252; 128 pairs a workgroup 1,158; 64 pairs a
 // wavefront, which halves the LDS reads and leaves one wavefront a SIMD (it issues a vector instruction every eight or nine
 // cycles, each of two every four or five), 1,156; codes two tiles ahead, or loads of single lanes' addresses, 1-3 % more. Width
@@ -120,8 +120,8 @@ __device__ __forceinline__ ChunkTile nth_chunk_tile(const ChunkArgs &a, int nth)
 // call may be laid out as one line instead, all tiles one behind another, cut into as many equal stretches as a head has places:
 // a workgroup works what its stretch holds, the end of one tile, whole ones and the beginning of another, say. Tile t of a
 // sequence takes START, what its beginning and end cost in keys, and a key for each that its last row sees: past + (t + 1) ROWS /
-// group. START is 192 where two workgroups share a CU, which hides a part of it, and 320 where one has it alone (12 sequences of 48 to
-// 700 rows over up to 9,700 tokens, 28 heads over 4 of 128: 264 -> 241 us; the former with 320 is 1 % slower).
+// group. START is 192 where two workgroups share a CU, which hides a part of it, and 320 where one has it alone (12 sequences of
+// 48 to 700 rows over up to 9,700 tokens, 28 heads over 4 of 128: 253 -> 232 us; the former with 320 is 1 % slower).
 constexpr int kLeastStretch = 128;  // keys: two do not begin at the same 64 keys of a tile then
 struct LinePlace {
   int b, tile, key;  // key: a multiple of a tile of keys, below what the tile's last row sees
@@ -656,12 +656,12 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) k_chunk_rows(ChunkA
 // How a call is laid out: wavefronts a workgroup, and whether in stretches, where tiles alone would not fill the GPU's places, or
 // not evenly. Priced in us, as measured: what a workgroup takes for a key (all places at work, or few) and for a tile's beginning
 // and end; tiles one after the other, those that see the most first (of several sequences, which rarely are as long as the
-// longest: half of that on the mean); and pieces' sums written and read at 4 TB/s, by a second kernel. Eight wavefronts a workgroup
-// convert each key once for 256 pairs instead of 128 (2,048 rows over 34,816 tokens, 32 heads over 4 of 128: 1,158 -> 1,067 us),
-// but leave coarser work. Against one cut of all tiles at the same keys, sized for the longest sequence: 1,110 rows over 2,291
-// tokens before them, 16 heads over 2 of 256, 118 -> 91 us; 100 single rows over up to 8,000, 32 over 4 of 128, 113 -> 92; 64
-// sequences of up to 16 rows over up to 4,000 56 -> 48. Beginning and end of a stretch cost 1-2 us more to find: 106 rows of
-// four sequences over up to 948 20 -> 21.
+// longest: half of that on the mean); and pieces' sums written and read at 4 TB/s, by a second kernel. Eight wavefronts a
+// workgroup convert each key once for 256 pairs instead of 128 (2,048 rows over 34,816 tokens, 32 heads over 4 of 128: 1,158 ->
+// 1,067 us), but leave coarser work. Against one cut of all tiles at the same keys, sized for the longest sequence: 1,110 rows
+// over 2,291 tokens before them, 16 heads over 2 of 256, 118 -> 91 us; 100 single rows over up to 8,000, 32 over 4 of 128, 113 ->
+// 92; 64 sequences of up to 16 rows over up to 4,000 56 -> 48. 1,857 rows of three over up to 9,024, 16 over 2 of 256, 235 ->
+// 201. Beginning and end of a stretch cost 1-2 us more to find: 106 rows of four sequences over up to 948 16.4 -> 17.7.
 struct ChunkPlan {
   int waves, stretches, per;  // no stretches: a workgroup a tile; per: stretches a tile
   long long tiles;
