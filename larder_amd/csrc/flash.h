@@ -2,6 +2,7 @@
 // products of 32 rows, the layout of keys and values in LDS, weights in 16 bits, values that are not finite, and the joining of
 // rows whose keys were worked in chunks.
 #pragma once
+#include "lines.h"
 #include "rows.h"
 
 namespace lmoe {
@@ -121,8 +122,7 @@ static __global__ void __launch_bounds__(256) k_join_chunks(JoinArgs a) {
   if constexpr (PLACED) {
     const int2 place = line < lines ? a.placed[line] : int2{-1, 0};
     from = place.x;
-    const int rest = min(place.y, a.most - 1) - from - a.next;
-    parts = from < 0 || from >= a.most || rest < 0 ? 0 : 2 + rest / a.step;
+    parts = joined_pieces(from, place.y, a.next, a.step, a.most);
   } else if (line < lines) {
     parts = min(a.joins[line], a.chunks);
   }
