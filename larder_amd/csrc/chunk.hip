@@ -751,7 +751,8 @@ extern "C" int lmoe_kv_chunk(const void *q, int dtype, long long q_row, long lon
   // D / 4 threads a line, 10.3 so)
   const bool shared = plan.stretches >= 8 * plan.tiles;
   const long long join_groups = !plan.bytes ? 0 : shared ? (long long)T * q_heads : ((long long)T * q_heads * (D / 4) + 255) / 256;
-  LMOE_REQUIRE(groups <= kMostGroups && join_groups <= kMostGroups, LMOE_ESHAPE,
+  // (kMostGroups are of 256 threads)
+  LMOE_REQUIRE(groups <= kMostGroups * 4 / plan.waves && join_groups <= kMostGroups, LMOE_ESHAPE,
                "%s: %d rows of %d sequences and %d heads are more than a launch takes", fn, T, B, q_heads);
   LMOE_REQUIRE(plan.bytes == 0 || (workspace && aligned16(workspace) && workspace_bytes >= plan.bytes), LMOE_EWORKSPACE,
                "%s: a 16-byte aligned workspace of %zu bytes is needed", fn, plan.bytes);
