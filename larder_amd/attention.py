@@ -341,8 +341,9 @@ def chunk_rows(q, cache, table, lens, cu=None, longest=None, scale=None):
     if None.
 
     Sums are float32; weights are rounded to q's type for their product with the values, and the sum that a row is divided by
-    is the rounded weights', as in prompt_rows. Keys and values keep all their bits (float16: as long as no page's scale is
-    2^22 times that of the page beside it). A value that is NaN makes its channel NaN in the rows that see it, and touches no other.
+    is the rounded weights', as in prompt_rows. Keys and values keep all their bits (float16: as long as the scales of two 32-token
+    pages beside each other are at most 2^22 apart). Scales of values are powers of two, as append_rows writes them: of others only
+    the exponent counts here. A value that is NaN makes its channel NaN in the rows that see it, and touches no other.
 
     longest sizes the launch: about the most tokens of a sequence (the table's room). Any value gives the same sums in another
     order."""

@@ -9,8 +9,9 @@
 //   scores^T = K Q^T   A = 32 keys x 16 channels, B = Q^T from registers: a lane ends with 16 of 32 keys' scores of one row
 //   out^T += V^T P^T   B = those weights as they lie, A = the same keys' values by LDS loads that transpose
 // Pages hold 32 tokens at least, so a half of a tile has one page, one scale of keys and one of values: the former multiplies
-// float32 scores, the latter goes into the conversion. bfloat16 takes any scale; float16 takes it relative to a reference that
-// moves, and the sums with it, when a page's scale leaves 2^-15 .. 2^7 of it, so that the conversion stays exact.
+// float32 scores, the latter goes into the conversion (its exponent: scales are powers of two). bfloat16 takes any scale; float16
+// takes it relative to a reference that moves, and the sums with it, when a page's scale leaves 2^-15 .. 2^7 of it, so that the
+// conversion stays exact for a tile's two pages up to 2^22 apart.
 //
 // 32 keys are worked at a time: the next 32 keys' score products, these ones' exponentials, their output products and a part of the
 // next tile's conversion are issued in one stream of slots, a product and about seven other instructions each. Tiles of keys lie
@@ -400,7 +401,9 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) k_chunk_rows(ChunkA
         const float big = fmaxf(vs[0], vs[1]), small = vs[0] == 0.0f ? vs[1] : vs[1] == 0.0f ? vs[0] : fminf(vs[0], vs[1]);
         move = 1.0f;
         if (big > 0.0f && (big > ref * 0x1p7f || small < ref * 0x1p-15f)) {
-          const float to = fmaxf(big, 0x1p-40f);  // (2^-40 448 is nothing in float16)
+          // the larger page's own scale where the smaller one's values stay exact beside it, down to 2^-7 of it (448 2^7 is finite)
+          // where they lie further apart; (2^-40 448 is nothing in float16)
+          const float to = fmaxf(fmaxf(fminf(big, small * 0x1p15f), big * 0x1p-7f), 0x1p-40f);
           move = ref == 0.0f ? 1.0f : fminf(ref / to, 0x1p120f);
           ref = to;
         }

@@ -1,0 +1,41 @@
+"""GPU parity at the ends of what the norms, the pages and the chunks over the cache take, against float64 and the oracles.
+
+Tolerances: those of test_gpu_chunk.py and test_gpu_norm.py, or equality."""
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_attention import F16, ints, normal, random_cache
+from test_gpu_chunk import check
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("longest", [None, 64])
+@pytest.mark.parametrize("heads,width", [(2, 64), (1, 128), (1, 256)])
+@pytest.mark.parametrize("apart", [7, 15, 16, 19, 22])
+def test_chunk_float16_pages_far_apart(apart, heads, width, longest):
+    """Values of two pages of one tile, the larger scale 2^apart times the other: rows that see the smaller page alone, or give all of
+    their weight to it, have its values to the last bit. (Rows of both stay finite: the larger page's codes are 1 at most, and the
+    smaller one's scale is 2^7 or less: 448 2^7 < 65504.)"""
+    from larder_amd import attention
+    rng = np.random.default_rng(apart)
+    cache = random_cache(rng, 4, heads, width, 32)
+    codes = rng.choice([1, 2, 5, 0x2d, 0x33, 0x38, 0x39, 0x3d, 0x41, 0x59, 0x7e], (4, heads, 32, width)) | rng.integers(0, 2, (4, heads, 32, width)) << 7
+    codes[2:] = rng.integers(0, 0x39, (2, heads, 32, width))
+    cache.v.view(torch.uint8).copy_(torch.from_numpy(codes.astype(np.uint8)))
+    cache.v_scale[:2], cache.v_scale[2:] = 2.0 ** (14 - apart), 2.0 ** 14
+    # (a sequence whose smaller page comes first; one whose larger page comes first, with keys that no row gives any weight to)
+    table, lens, cu = np.array([[0, 2], [3, 1]]), [64, 60], [0, 64, 90]
+    cache.k_scale.fill_(2.0 ** -6)
+    cache.k.view(torch.uint8)[3] = 0xf8  # -256
+    cache.k.view(torch.uint8)[1] &= 0x3f
+    q = normal(rng, 90, 3 * heads, width, dtype=F16)
+    q[64:] = 16.0
+    got = attention.chunk_rows(q, cache, ints(table), ints(lens), ints(cu), longest=longest)
+    check(got, q, cache, table, lens, cu, width ** -0.5, F16)
+    # a row of one token is that token, and each of a page's first rows lies within the page's own values
+    first = cache.v[0, :, 0].float() * cache.v_scale[0, 0]
+    assert torch.equal(got[0].view(heads, 3, width), first[:, None].expand(heads, 3, width).to(F16))
+    alone = attention.chunk_rows(q[:32], cache, ints(table[:1, :1]), ints([32]), ints([0, 32]), longest=64)
+    assert (got[:32].double() - alone.double()).abs().max() <= 2.0 ** -10 * alone.double().abs().max()
