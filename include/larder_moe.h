@@ -559,7 +559,8 @@ int lmoe_kv_chunk(const void *q, int dtype, long long q_row, long long q_head, i
  * without a page, or whose page has refs > 1, gets the lowest free page, sequence by sequence and place by place, refs 1; the
  * old page's count falls by one. Where the old page holds tokens before the rows, src[b] and dst[b] [B] are the pair that
  * lmoe_pages_copy has to copy (else -1, at most one a sequence). Pages are free that have refs 0 when the call begins; places that
- * find none hold -1, lacking [B] counts them. workspace: lmoe_pages_take_workspace_bytes.
+ * find none hold -1, lacking [B] counts them; but a page that all of its holders would leave stays with the last of those that
+ * find none. workspace: lmoe_pages_take_workspace_bytes.
  * lmoe_pages_free: places from keep[b] [B] tokens on are given back and hold -1.
  * lmoe_pages_fork: out [n][width] = the rows of table that parents [n] names (outside [0, B): -1); every place of table is given
  * back and every place of out counted. out does not overlap table.

@@ -111,7 +111,8 @@ struct Fallen {
 };
 
 // One workgroup. A task is a place that rows fall into, in the order of sequences and places. 1: where each sequence's tasks
-// begin; 2: which need a page, and their ranks; 3: as many of the lowest free pages; 4: the places get them.
+// begin; 2: which need a page, and their ranks; 3: as many of the lowest free pages; 4: the places get them; 5: where that was
+// not enough, a page that all of its holders gave up stays with the last of those that found none.
 __global__ void __launch_bounds__(kTakers) k_take(TakeArgs a) {
   __shared__ int sums[kTakers / 64 + 1], begins_lds[kSeqsInLds], counts[kTakers];
   const int tid = threadIdx.x;
@@ -183,16 +184,40 @@ __global__ void __launch_bounds__(kTakers) k_take(TakeArgs a) {
     const int i = at.first + t - begins[b];
     int *place = a.table + size_t(b) * a.width + i;
     const int old = *place, page = rank < found ? a.given[rank] : -1;
-    *place = page;
-    if (page >= 0)
-      a.refs[page] = 1;
-    else
-      atomicAdd(a.lacking + b, 1);
+    if (page >= 0) *place = page, a.refs[page] = 1;
     if (uint32_t(old) < uint32_t(a.pages)) {
       atomicSub(a.refs + old, 1);
       if (page >= 0 && at.start > i << a.page_shift) a.src[b] = old, a.dst[b] = page;
     }
   }
+  if (found >= needs) return;
+  // Places that found no page still hold what they shared, or none
+  auto each_without = [&](auto &&f) {  // f(task, sequence, place, page)
+    __syncthreads();
+    for (int t = tid; t < tasks; t += kTakers) {
+      const int rank = a.ranks[t];
+      if (rank == -1 || (rank >= 0 && rank < found)) continue;
+      const int b = sequence_of(t);
+      int *place = a.table + size_t(b) * a.width + Fallen(a, b).first + t - begins[b];
+      f(t, b, place, *place);
+    }
+  };
+  auto holders = [&](int p) { return __hip_atomic_load(a.refs + p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+  constexpr int kLeft = -2;  // for a rank: nobody holds what this place shared
+  each_without([&](int t, int, int *, int p) {
+    if (uint32_t(p) < uint32_t(a.pages) && holders(p) == 0) a.ranks[t] = kLeft;
+  });
+  each_without([&](int t, int, int *, int p) {
+    if (a.ranks[t] == kLeft) atomicMin(a.refs + p, -1 - t);
+  });
+  each_without([&](int t, int b, int *place, int p) {
+    if (a.ranks[t] == kLeft && holders(p) == -1 - t) {
+      a.refs[p] = 1;
+    } else {
+      *place = -1;
+      atomicAdd(a.lacking + b, 1);
+    }
+  });
 }
 
 // The places of a table from keep[b] tokens on are given back

@@ -65,7 +65,8 @@ def take_pages(refs, table, lens, cu=None, page=64):
     (src, dst, lacking), int32 [sequences] each: the pages to copy before the rows are appended, where a sequence had shared
     a page that holds tokens before them (-1: none; a sequence has one at most), and how many of its places found no page left.
     Those hold -1 and what they shared is no longer theirs: append_rows writes nothing there, and such a sequence is cut
-    (free_pages) and taken up again when there is room. Tokens past the table's places have none, and lack none."""
+    (free_pages) and taken up again when there is room. But a page that all of its holders would leave so stays with the last of
+    those that found none, and is its own. Tokens past the table's places have none, and lack none."""
     fn = "take_pages"
     pages, n, places = _pool(fn, refs, table)
     _page(fn, page)

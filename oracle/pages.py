@@ -23,6 +23,8 @@ def take(refs, table, lens, cu, page):
             if _held(old, refs) and before[old] <= 1:
                 continue
             new = next(free, -1)
+            if new < 0 and _held(old, refs) and refs[old] == 1:
+                continue  # the others have given it up: it is this sequence's own
             table[b][i] = new
             if new >= 0:
                 refs[new] = 1

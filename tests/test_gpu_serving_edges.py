@@ -1,10 +1,13 @@
 """GPU parity at the ends of what the norms, the pages and the chunks over the cache take, against float64 and the oracles.
 
 Tolerances: those of test_gpu_chunk.py and test_gpu_norm.py, or equality."""
+import random
+
 import numpy as np
 import pytest
 import torch
 
+from oracle import pages as pool_ref
 from test_gpu_attention import F16, ints, normal, random_cache
 from test_gpu_chunk import check
 
@@ -39,3 +42,30 @@ def test_chunk_float16_pages_far_apart(apart, heads, width, longest):
     assert torch.equal(got[0].view(heads, 3, width), first[:, None].expand(heads, 3, width).to(F16))
     alone = attention.chunk_rows(q[:32], cache, ints(table[:1, :1]), ints([32]), ints([0, 32]), longest=64)
     assert (got[:32].double() - alone.double()).abs().max() <= 2.0 ** -10 * alone.double().abs().max()
+
+
+@pytest.mark.parametrize("sequences,shared,free", [(2, 1, 0), (3, 1, 1), (40, 7, 0), (40, 7, 11), (700, 100, 300), (3000, 900, 40),
+                                                   (2500, 1, 2300)])
+def test_take_where_pages_run_out(sequences, shared, free):
+    """Groups of sequences that share their last page and all or some of whom write to it, with fewer free pages than writers."""
+    from larder_amd import pages as own
+    rng = random.Random(sequences + free)
+    page, pages = 32, shared + free
+    for writes in (1.0, 0.8, 0.5):
+        table = [[rng.randrange(shared), -1, -1] for _ in range(sequences)]
+        refs = [0] * pages
+        for row in table:
+            refs[row[0]] += 1
+        order = list(range(pages))
+        rng.shuffle(order)
+        table = [[order[p] if p >= 0 else -1 for p in row] for row in table]
+        refs = [r for _, r in sorted(zip(order, refs))]
+        refs = [r if r or p not in order[:shared] else 9 for p, r in enumerate(refs)]  # (a page that others hold)
+        rows = [rng.choice([1, 3, 40, 64]) if rng.random() < writes else 0 for _ in range(sequences)]
+        lens, cu = [7 + r for r in rows], [int(x) for x in np.cumsum([0] + rows)]
+        want = pool_ref.take(refs, table, lens, cu, page)
+        for _ in range(3):
+            r, t = ints(refs), ints(table)
+            got = own.take_pages(r, t, ints(lens), ints(cu), page=page)
+            for a, b in zip((r, t, *got), want):
+                assert a.tolist() == b
