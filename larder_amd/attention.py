@@ -105,6 +105,7 @@ def rotary_freq(width, base=10000.0, kind="default", factor=1.0, original=None, 
 
 _CODES = (torch.float8_e4m3fn, torch.uint8)
 _HALVES = (torch.float16, torch.bfloat16)
+_MOST = 2 ** 31 - 1  # of a size that the library takes as an int
 
 
 def _refuse(fn, why):
@@ -156,6 +157,8 @@ def _sequences(fn, cu, lens, table, rows):
     if table.dtype is not torch.int32 or table.dim() != 2 or table.shape[1] == 0:
         _refuse(fn, f"table is int32 [sequences, pages], not {table.dtype} {list(table.shape)}")
     n, width = table.shape
+    if n > _MOST or width > _MOST:
+        _refuse(fn, f"{n} sequences of {width} pages are more than an int counts")
     if not table.is_contiguous():
         table = table.contiguous()
     if lens is not None:

@@ -28,7 +28,7 @@ import functools
 import torch
 
 from . import _lib, attention
-from .attention import _device, _ints, _launch, _refuse
+from .attention import _MOST, _device, _ints, _launch, _refuse
 
 __all__ = ["compact_pages", "copy_pages", "fork_pages", "free_pages", "take_pages"]
 
@@ -39,7 +39,10 @@ def _pool(fn, refs, table):
         _refuse(fn, f"refs is int32 [pages], contiguous, not {refs.dtype} {list(refs.shape)}")
     if table.dtype is not torch.int32 or table.dim() != 2 or table.shape[1] == 0 or not table.is_contiguous():
         _refuse(fn, f"table is int32 [sequences, places], contiguous, not {table.dtype} {list(table.shape)}")
-    return refs.shape[0], table.shape[0], table.shape[1]
+    pages, (n, places) = refs.shape[0], table.shape
+    if pages > _MOST or n > _MOST or places > _MOST:
+        _refuse(fn, f"{pages} pages, {n} sequences of {places} places are more than an int counts")
+    return pages, n, places
 
 
 def _page(fn, page):
@@ -92,6 +95,8 @@ def copy_pages(cache, src, dst):
     if src.dim() != 1:
         _refuse(fn, f"src is int32 [pairs], not {src.dtype} {list(src.shape)}")
     n = src.shape[0]
+    if n > _MOST:
+        _refuse(fn, f"{n} pairs are more than an int counts")
     src, dst = _ints(fn, "src", src, n), _ints(fn, "dst", dst, n)
     dev = _device(fn, *cache, src, dst)
     if n:
@@ -107,6 +112,8 @@ def fork_pages(refs, table, parents):
     pages, n, places = _pool(fn, refs, table)
     if parents.dim() != 1:
         _refuse(fn, f"parents is int32 [sequences], not {parents.dtype} {list(parents.shape)}")
+    if parents.shape[0] > _MOST:
+        _refuse(fn, f"{parents.shape[0]} new sequences are more than an int counts")
     parents = _ints(fn, "parents", parents, parents.shape[0])
     dev = _device(fn, refs, table, parents)
     out = table.new_empty((parents.shape[0], places))

@@ -170,6 +170,8 @@ def norm_rows(x, weight, eps=1e-6, residual=None, group=None, total=None):
         weight = weight.contiguous()
     x, t, heads, x_row, x_head = _planes(x)
     r_row = r_head = s_row = s_head = 0
+    if h > attention._MOST or heads > attention._MOST:
+        attention._refuse(fn, f"{heads} heads of {h} channels are more than an int counts")
     if residual is not None:
         residual, _, _, r_row, r_head = _planes(residual)
     if total is not None:
@@ -200,6 +202,8 @@ def read_codes(codes, scales, dtype=torch.bfloat16):
             scales.shape[-1] == 0 or codes.shape[-1] % scales.shape[-1]):
         attention._refuse(fn, f"scales are float32 {list(codes.shape[:-1])} and a divisor of {codes.shape[-1]}, not "
                               f"{scales.dtype} {list(scales.shape)}")
+    if codes.shape[-1] > attention._MOST:
+        attention._refuse(fn, f"rows of {codes.shape[-1]} channels are more than an int counts")
     dt = dcode(dtype)
     dev = attention._device(fn, codes, scales)
     codes, scales = codes.contiguous(), scales.contiguous()

@@ -2,8 +2,9 @@
 import ctypes
 
 import pytest
+import torch
 
-from larder_amd import _lib
+from larder_amd import _lib, attention, pages, trunk
 
 P = ctypes.c_void_p(16)  # never dereferenced: every call below is refused while its arguments are checked
 
@@ -15,3 +16,39 @@ def test_chunks_of_more_threads_than_a_launch_takes_are_refused(built_lib, T, he
     rc = built_lib.lmoe_kv_chunk(P, 1, 128 * heads, 128, T, heads, heads, 128, P, P, 1, P, 2000, P, P, P, P, 1, 64, 100000, 0.1,
                                  None, 0, P, None)
     assert rc == _lib.ESHAPE and b"more than a launch" in built_lib.lmoe_error(), (rc, built_lib.lmoe_error())
+
+
+def test_sizes_past_an_int_are_refused(monkeypatch):
+    """What the library takes as an int would wrap: 2^32 + 64 channels would be 64 of them. (Tensors without memory.)"""
+    def empty(*shape, dtype=torch.int32):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    launched = []
+    monkeypatch.setattr(attention, "_device", lambda *a: 0)
+    monkeypatch.setattr(attention, "_launch", lambda *a: launched.append(a))
+    monkeypatch.setattr(pages, "_device", lambda *a: 0)
+    monkeypatch.setattr(pages, "_launch", lambda *a: launched.append(a))
+    monkeypatch.setattr(trunk, "call", lambda *a: launched.append(a))
+    far, bf = 2 ** 32 + 64, torch.bfloat16
+    cache = attention.KVCache.empty(2, 1, 64, device="meta")
+    q = empty(1, 1, 64, dtype=bf)
+    for call in (lambda: trunk.norm_rows(empty(1, far, dtype=bf), empty(far, dtype=bf)),
+                 lambda: trunk.norm_rows(empty(1, far, dtype=bf), empty(far, dtype=bf), group=32),
+                 lambda: trunk.norm_rows(empty(1, far, 1, dtype=bf), empty(1, dtype=bf)),
+                 lambda: trunk.read_codes(empty(1, far, dtype=torch.float8_e4m3fn), empty(1, 1, dtype=torch.float32)),
+                 lambda: pages.take_pages(empty(far), empty(1, 1), empty(1)),
+                 lambda: pages.take_pages(empty(4), empty(far, 1), empty(far)),
+                 lambda: pages.free_pages(empty(4), empty(1, far), empty(1)),
+                 lambda: pages.fork_pages(empty(4), empty(1, 1), empty(far)),
+                 lambda: pages.compact_pages(empty(4), empty(1, 1), empty(far, 1)),
+                 lambda: pages.copy_pages(cache, empty(far), empty(far)),
+                 lambda: attention.chunk_rows(q, cache, empty(1, far), empty(1)),
+                 lambda: attention.attend_rows(q, cache, empty(1, far), empty(1)),
+                 lambda: attention.append_rows(cache, None, q, q, empty(1, far), empty(1)),
+                 lambda: attention.read_rows(cache, empty(1, far), empty(2), 1)):
+        with pytest.raises(ValueError, match="an int counts"):
+            call()
+    assert not launched
+    trunk.norm_rows(empty(1, 64, dtype=bf), empty(64, dtype=bf))  # (these stand in for the kernels' launch)
+    pages.take_pages(empty(4), empty(1, 1), empty(1))
+    assert len(launched) == 2
