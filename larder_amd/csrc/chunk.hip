@@ -353,7 +353,8 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) k_chunk_rows(ChunkA
       for (int j = 0; j < KS; ++j) qf[j] = *reinterpret_cast<const u32x4 *>(q + 16 * j);
     }
     // pages and scales of the halves of 64 tiles from `base` on, a tile a lane
-    const int tiles = keys > begin ? (keys - begin + BN - 1) / BN : 0;
+    // (here and below: a table of 32-token pages may have room for 2^31 - 32 tokens, and no end of a tile is held in an int)
+    const int tiles = keys > begin ? (keys - begin - 1) / BN + 1 : 0;
     int base = 0, number[2];
     float k_scale[2], v_scale[2];
     auto look_up = [&](int t0) {
@@ -476,7 +477,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) k_chunk_rows(ChunkA
       // (never zero: -infinity times that would be NaN)
       const float c = fmaxf(lane_value(k_scale[x], t - base) * a.scale, 0x1p-126f);
       const bool hole = __builtin_amdgcn_readlane(number[x], t - base) < 0;
-      if (at + 32 > all || hole) {
+      if (all - 32 < at || hole) {
         const int left = opaque(hole ? 0 : sees - at - 4 * h);  // opaque: a branch, not selects in every half
   #pragma unroll
         for (int e = 0; e < 16; ++e)
@@ -567,7 +568,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) k_chunk_rows(ChunkA
       const int at = begin + t * BN;
       uint8_t *vt = v_lds + stage * kTileBytes;
       bool bad = false;
-      if (at + BN > all_rows) {  // the workgroup's first row does not see all of it
+      if (all_rows - BN < at) {  // the workgroup's first row does not see all of it
         const bool found = __any(any_bad<D, BF, THREADS>(vt));
         if (lane == 0) flags[wave] = found;
         barrier_lds();

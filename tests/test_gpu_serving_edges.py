@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import pages as pool_ref
-from test_gpu_attention import F16, ints, normal, random_cache
+from test_gpu_attention import BF16, F16, ints, normal, random_cache
 from test_gpu_chunk import check
 
 pytestmark = pytest.mark.gpu
@@ -69,3 +69,28 @@ def test_take_where_pages_run_out(sequences, shared, free):
             got = own.take_pages(r, t, ints(lens), ints(cu), page=page)
             for a, b in zip((r, t, *got), want):
                 assert a.tolist() == b
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_chunk_of_a_table_with_room_for_2_31_tokens(dtype):
+    """The last 32-token page of the longest table there is: its tokens are seen, and a NaN in the very last by the last row alone."""
+    from larder_amd import attention
+    rng = np.random.default_rng(31)
+    places = (2 ** 31 - 1) // 32
+    cache = random_cache(rng, 2, 1, 64, 32)
+    cache.k_scale.fill_(1.0), cache.v_scale.fill_(0.5)
+    cache.k.view(torch.uint8)[0] = 0xc0  # -2: scores of -128 against the last page's 128
+    cache.k.view(torch.uint8)[1] = 0x40
+    cache.v.view(torch.uint8)[1, 0, 31, 5] = 0x7f
+    table = torch.zeros((1, places), dtype=torch.int32, device="cuda")
+    table[0, -1] = 1
+    q = torch.ones(2, 3, 64, dtype=dtype, device="cuda")
+    got = attention.chunk_rows(q, cache, table, ints([32 * places]), ints([0, 2]), scale=1.0).double()
+    v = cache.v[1, 0].double() * 0.5
+    for row, n in ((0, 31), (1, 32)):
+        want, spread = v[:n].mean(0), v[:n].abs().mean(0)
+        off = (got[row] - want).abs()
+        # (equal weights, sums of 32 values at most: the result's rounding and a few of float32; float16 has steps of 2^-24)
+        ok = off <= torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -18 * spread + 2.0 ** -25
+        assert (ok | torch.isnan(want)).all(), (row, off.max())
+        assert torch.isnan(got[row]).any(0).tolist() == [n == 32 and c == 5 for c in range(64)]
