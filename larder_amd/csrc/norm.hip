@@ -120,8 +120,9 @@ __device__ __forceinline__ float lanes_max(float v, int lanes) {
   return v;
 }
 
-// Where squares overflow: rows are scaled by this first (2^128 of the largest sum becomes 2^48, its square 2^96)
-constexpr float kDown = 0x1p-80f;
+// Where squares overflow: rows are scaled by kDown^2 for their sum (2^128 of the largest becomes 2^48, its square 2^96). A channel is
+// brought back by one kDown before its weight and one behind, so that what is small beside large ones is not rounded on the way
+constexpr float kDown = 0x1p-40f;
 
 // N steps of eight channels a lane in registers; N = 0: rows of any length, read twice
 template <int DT, int L, int N>
@@ -179,8 +180,9 @@ __global__ void __launch_bounds__(256) k_norm(NormArgs a) {
   const float ss = row_sum<L>(squares(1.0f), lds);
   float inv = 1.0f / sqrtf(ss / float(a.H) + a.eps), down = 1.0f;
   if (__any(!(ss < INFINITY))) {  // (for a row in four wavefronts: all of them or none)
-    const float low = row_sum<L>(squares(kDown), lds + 4);
-    if (!(ss < INFINITY)) inv = 1.0f / sqrtf(low / float(a.H)), down = kDown;
+    constexpr float kSquares = kDown * kDown;
+    const float low = row_sum<L>(squares(kSquares), lds + 4);
+    if (!(ss < INFINITY)) inv = kDown / sqrtf(low / float(a.H) + a.eps * kSquares * kSquares), down = kDown;
   }
   auto normed = [&](int i, float (&u)[8]) {  // the step's y from its sums; the sums are written
     const int c = i * L + lane, n = a.H - 8 * c;
@@ -196,7 +198,7 @@ __global__ void __launch_bounds__(256) k_norm(NormArgs a) {
     else
       load_any<LMOE_F32>(a.weight, 8 * c, n, w);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) u[e] = u[e] * down * inv * w[e];
+    for (int e = 0; e < 8; ++e) u[e] = u[e] * inv * w[e] * down;
   };
   if (!a.group) {
     for_steps<N>(steps, [&](int i) {
@@ -268,7 +270,7 @@ __global__ void __launch_bounds__(256) k_norm(NormArgs a) {
       else
         load_any<LMOE_F32>(a.weight, 8 * c, n, w);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) u[e] = u[e] * down * inv * w[e];
+      for (int e = 0; e < 8; ++e) u[e] = u[e] * inv * w[e] * down;
       most = fmaxf(most, finite(u));
     }
   }

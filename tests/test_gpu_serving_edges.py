@@ -10,6 +10,7 @@ import torch
 from oracle import pages as pool_ref
 from test_gpu_attention import BF16, F16, ints, normal, random_cache
 from test_gpu_chunk import check
+from test_gpu_norm import check as check_norm
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +95,18 @@ def test_chunk_of_a_table_with_room_for_2_31_tokens(dtype):
         ok = off <= torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -18 * spread + 2.0 ** -25
         assert (ok | torch.isnan(want)).all(), (row, off.max())
         assert torch.isnan(got[row]).any(0).tolist() == [n == 32 and c == 5 for c in range(64)]
+
+
+@pytest.mark.parametrize("h", [8, 500, 512, 2000, 16400])
+def test_norm_of_small_channels_beside_large_ones(h):
+    """Rows whose squares pass float32: channels 2^-120 of the largest keep their bits, and eps counts where it is as large."""
+    rng = torch.Generator(device="cuda").manual_seed(h)
+    x = torch.randn((7, h), generator=rng, device="cuda") * 2.0 ** 66
+    x[1:4, ::2] *= 2.0 ** -110
+    x[4, 1::3] *= 2.0 ** -120
+    x[5] *= 2.0 ** 58
+    w = 1 + torch.rand(h, generator=rng, device="cuda")
+    check_norm(x, None, w, 1e-6)
+    check_norm(x, x.flip(1), w, 1e38)
+    check_norm(x, None, w, 3e38)
+    check_norm(x, None, w, 1e38, group=h)
