@@ -165,6 +165,8 @@ def norm_rows(x, weight, eps=1e-6, residual=None, group=None, total=None):
     elif total.shape != shape or total.dtype is not dtype or (h > 1 and total.stride(-1) != 1) or (
             total.dim() > 3 and not total.is_contiguous()):
         attention._refuse(fn, "total has x's shape and type and a dense last axis")
+    elif any(s == 0 and n > 1 for s, n in zip(total.stride(), shape)):
+        attention._refuse(fn, "total has a place for every element")
     dev = attention._device(fn, x, weight, residual, total)
     if h > 1 and weight.stride(0) != 1:
         weight = weight.contiguous()

@@ -52,3 +52,16 @@ def test_sizes_past_an_int_are_refused(monkeypatch):
     trunk.norm_rows(empty(1, 64, dtype=bf), empty(64, dtype=bf))  # (these stand in for the kernels' launch)
     pages.take_pages(empty(4), empty(1, 1), empty(1))
     assert len(launched) == 2
+
+
+def test_a_broadcast_total_is_refused(monkeypatch):
+    """Rows that would all be written to one place; a dense axis of one may have any stride."""
+    monkeypatch.setattr(attention, "_device", lambda *a: 0)
+    monkeypatch.setattr(attention, "_launch", lambda *a: None)
+    x, w = torch.zeros(3, 2, 64, dtype=torch.bfloat16), torch.zeros(64, dtype=torch.bfloat16)
+    for total in (x[:1].expand(3, 2, 64), x[:, :1].expand(3, 2, 64)):
+        with pytest.raises(ValueError, match="every element"):
+            trunk.norm_rows(x, w, total=total)
+        trunk.norm_rows(total, w, residual=x)  # (read, they are rows like any)
+    trunk.norm_rows(x[:1], w, total=x[:1].as_strided((1, 2, 64), (0, 64, 1)))
+    trunk.norm_rows(x[..., :1], w[:1], total=x[..., :1].as_strided((3, 2, 1), (128, 64, 0)))
