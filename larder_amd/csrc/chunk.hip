@@ -60,9 +60,8 @@ template <int ROWS>
 __device__ __forceinline__ ChunkTile nth_chunk_tile(const ChunkArgs &a, int nth) {
   ChunkTile w = {-1, 0, 0, 0, 0};
   if (a.B > 64) {
-    const int turned = nth < (a.tiles & ~7) ? (nth & ~7) | ((nth + (nth >> 3)) & 7) : nth;
-    const int task = a.tiles - 1 - turned;
-    auto begin = [&](int c, int i) { return (long long)c * a.group / ROWS + i; };
+    const int task = a.tiles - 1 - turned_task(nth, a.tiles);
+    auto begin = [&](int c, int i) { return first_task(c, i, a.group, ROWS); };
     if (a.cu)
       w.b = last_at(a.cu, a.B, task, begin);
     else  // a row a sequence
@@ -80,15 +79,10 @@ __device__ __forceinline__ ChunkTile nth_chunk_tile(const ChunkArgs &a, int nth)
   if (lane < a.B) {
     seq_rows(a.cu, lane, a.T, &row0, &n);
     len = max(a.lens[lane], 0);
-    tiles = max(int(((long long)n * a.group + ROWS - 1) / ROWS), lane == 0 || lane == a.B - 1 ? 1 : 0);
+    tiles = max(tiles_of(n, a.group, ROWS), lane == 0 || lane == a.B - 1 ? 1 : 0);
   }
-  // A tile sees about past + tile ROWS / group keys: how many tiles of the lane's sequence see 256 x or more
   const int past = max(len - n, 0);
-  auto count = [&](int x) {
-    const long long rows = 256ll * x - past;
-    const long long at = rows <= 0 ? 0 : (rows * a.group + ROWS - 1) / ROWS;
-    return at >= tiles ? 0 : tiles - int(at);
-  };
+  auto count = [&](int x) { return tiles_that_see(x, past, tiles, a.group, ROWS); };  // of the lane's sequence
   auto from = [&](int x) { return int(wave_sum(float(count(x)))); };  // (counts below 2^24: exact in float32)
   int lo = 0, hi = !a.sorted ? 1 : (int(wave_max(tiles > 0 ? float(past) + float(tiles) * ROWS / a.group : 0.0f)) >> 8) + 2, behind = 0;
   if (nth >= from(0)) return w;
@@ -123,7 +117,7 @@ __device__ __forceinline__ ChunkTile nth_chunk_tile(const ChunkArgs &a, int nth)
 // sequence takes START, what its beginning and end cost in keys, and a key for each that its last row sees: past + (t + 1) ROWS /
 // group. START is 192 where two workgroups share a CU, which hides a part of it, and 320 where one has it alone (12 sequences of
 // 48 to 700 rows over up to 9,700 tokens, 28 heads over 4 of 128: 253 -> 232 us; the former with 320 is 1 % slower).
-constexpr int kLeastStretch = 128;  // keys: two do not begin at the same 64 keys of a tile then
+static_assert(kLineKeys == kPromptKeys, "a stretch begins with a tile of keys");
 struct LinePlace {
   int b, tile, key;  // key: a multiple of a tile of keys, below what the tile's last row sees
 };
@@ -137,13 +131,9 @@ struct TileLine {
       seq_rows(a.cu, b, a.T, &row0, &n);
       len = max(a.lens[b], 0);
     }
-    tiles = int(((long long)n * a.group + ROWS - 1) / ROWS);
+    tiles = tiles_of(n, a.group, ROWS);
   }
-  // of the first t tiles of a sequence, times group (float64: a 64-bit product is an instruction; whole numbers below 2^53, and
-  // past that places are rounded, in the same way for all)
-  __device__ __forceinline__ double cost(int past, int t) const {
-    return double(t) * (double(a.group) * (max(past, 0) + START) + double(ROWS / 2) * (t + 1));
-  }
+  __device__ __forceinline__ double cost(int past, int t) const { return line_cost(past, t, a.group, ROWS, START); }
   // of the lane's sequence and those before it in the wavefront (lanes past the last sequence: of some of them)
   __device__ __forceinline__ double ends() const {
     double x = cost(len - n, tiles);
@@ -207,8 +197,7 @@ struct TileLine {
       lo += step * (__popcll(__ballot(t < hi && cost(off, t) <= x)) - 1);
       hi = min(hi, lo + step);
     }
-    const double at = (x - cost(off, lo)) * a.per_group - START;
-    int key = int(fmin(fmax(at, 0.0), double(0x7fffffff))) & -kPromptKeys;
+    int key = line_key((x - cost(off, lo)) * a.per_group - START);
     if (key && seen(off, lo, its_n * a.group) - key < kPromptKeys) ++lo, key = 0;
     return {b + i, lo, key};
   }
@@ -218,8 +207,7 @@ struct TileLine {
     const int tile = one / per, i = one - tile * per;
     *from = *to = {a.B, 0, 0};
     if ((long long)tile * ROWS >= (long long)n * a.group) return;
-    // (pieces' ends pass 31 bits where a table has room for as many tokens)
-    const uint32_t most = max(seen(len - n, tile, n * a.group), 1), step = ((most - 1) / uint32_t(per * kPromptKeys) + 1) * kPromptKeys;
+    const uint32_t most = max(seen(len - n, tile, n * a.group), 1), step = piece_keys(most, per);
     const uint32_t begin = i * step;
     if (i > 0 && begin >= most) return;
     *first = {0, 0, row0, n, len};
@@ -228,7 +216,7 @@ struct TileLine {
   }
   // how many keys a tile's last row sees
   __device__ __forceinline__ int seen(int off, int tile, int pairs) const {
-    return min(off + (min(tile * ROWS + ROWS, pairs) - 1) / a.group + 1, a.width << a.page_shift);
+    return tile_sees(off, tile, pairs, a.group, ROWS, a.width << a.page_shift);
   }
   // the first sequence from b on that has rows, by one wavefront
   __device__ __forceinline__ int with_rows(int b) {
@@ -296,7 +284,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) k_chunk_rows(ChunkA
   };
   auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
   ChunkTile work;
-  [[maybe_unused]] TileLine<ROWS, D == 256 || NW == 8 ? 320 : 192> line_of_tiles{a};
+  [[maybe_unused]] TileLine<ROWS, line_start(D, NW)> line_of_tiles{a};
   [[maybe_unused]] LinePlace at_line, to_line;
   if constexpr (SPLIT) {
     const int one = int(blockIdx.x) / a.heads;
