@@ -8,8 +8,8 @@ import pytest
 import torch
 
 from oracle import pages as pool_ref
-from test_gpu_attention import BF16, F16, ints, normal, random_cache
-from test_gpu_chunk import check
+from test_gpu_attention import BF16, F16, ints, normal, page_table, poisoned_memory, random_cache  # noqa: F401
+from test_gpu_chunk import check, check_long
 from test_gpu_norm import check as check_norm
 
 pytestmark = pytest.mark.gpu
@@ -110,3 +110,90 @@ def test_norm_of_small_channels_beside_large_ones(h):
     check_norm(x, x.flip(1), w, 1e38)
     check_norm(x, None, w, 3e38)
     check_norm(x, None, w, 1e38, group=h)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("q_heads,heads,width", [(32, 8, 64), (32, 8, 128), (16, 8, 256)])
+@pytest.mark.parametrize("sequences", [2, 5, 12, 40, 64])
+def test_chunk_whole_tiles_of_many_sequences(dtype, q_heads, heads, width, sequences):
+    """More workgroups than places, each a whole tile, the longest tiles first: sequences of few and many rows over no and long
+    histories, the first, the last and one between without rows; rows before and behind them."""
+    from larder_amd import attention
+    rng = np.random.default_rng(100 * sequences + width)
+    parts = rng.random(sequences) ** 2
+    if sequences > 3:
+        parts[[0, sequences // 2, -1]] = 0
+    rows = [int(x) for x in np.floor(2600 * parts / parts.sum())]
+    past = [int(rng.choice([0, 1, 255, 256, 700, 1300])) for _ in rows]
+    lens = [r + p for r, p in zip(rows, past)]
+    if sequences > 3:
+        lens[1] = rows[1] // 2  # more rows than tokens
+    cu = [5] + [5 + int(x) for x in np.cumsum(rows)]
+    t, long = cu[-1] + 3, max(lens)
+    assert attention._chunk_workspace(t, q_heads, heads, width, sequences, long) == 0
+    assert (t * q_heads // heads // (256 if width == 128 else 128) + 1) * heads > (512 if width == 64 else 256)
+    table, n = page_table(rng, [-(-x // 64) for x in lens])
+    cache = random_cache(rng, n, heads, width, 64)
+    q = normal(rng, t, q_heads, width, dtype=dtype)
+    got = attention.chunk_rows(q, cache, ints(table), ints(lens), ints(cu), longest=long)
+    assert (got[:5] == 0).all() and (got[cu[-1]:] == 0).all() and not torch.isnan(got).any()
+    check_long(got, q, cache, table, lens, cu, width ** -0.5, dtype, some=[0, q_heads // 2 - 1, q_heads - 1])
+
+
+@pytest.mark.parametrize("lens", [[2 ** 31 - 1, 300], [70, 2 ** 31 - 100], [2 ** 31 - 320, 2 ** 31 - 1]])
+def test_chunk_of_lengths_at_an_ints_end(lens):
+    """Sequences of far more tokens than their table has places: every row sees all the table's, the others what they see."""
+    from larder_amd import attention
+    rng = np.random.default_rng(lens[0] % 97)
+    rows, cu, page, places = [40, 30], [0, 40, 70], 64, 400
+    table, n = page_table(rng, [places, places])
+    cache = random_cache(rng, n, 2, 128, page)
+    q = normal(rng, 70, 8, 128)
+    assert attention._chunk_workspace(70, 8, 2, 128, 2, places * page)
+    got = attention.chunk_rows(q, cache, ints(table), ints(lens), ints(cu))
+    # (all of the table, for a row each: the same sums with no length beyond it)
+    for b in range(2):
+        for r in (0, rows[b] - 1):
+            sees = min(lens[b] - rows[b] + r + 1, places * page)
+            one = q[cu[b] + r][None]
+            check_long(got[cu[b] + r][None], one, cache, table[b][None], [sees], [0, 1], 128 ** -0.5, BF16)
+    assert not torch.isnan(got).any()
+
+
+@pytest.mark.parametrize("q_heads,heads,width,rows", [(3, 1, 64, 100), (8, 2, 128, 90), (16, 1, 128, 700), (4, 2, 256, 60)])
+@pytest.mark.parametrize("fill", [-1, 0, 3, 129, 0x7fffffff, -2 ** 31])
+def test_chunk_writes_its_rows_alone(q_heads, heads, width, rows, fill):
+    """Right and wild offsets, lengths and tables; a workspace that holds small and large whole numbers beforehand: what lies around
+    the output and the workspace keeps its value."""
+    from larder_amd import _lib, attention
+    rng, pick = np.random.default_rng(width + rows), random.Random(rows)
+    page, room, around = 32, 300, 4096
+    cache = random_cache(rng, 40, heads, width, page)
+    q = normal(rng, rows, q_heads, width)
+    codes = [t.data_ptr() for t in cache]
+    wild = [-2 ** 31, -5, -1, 0, 1, 7, rows // 2, rows, 1000, 9600, 2 ** 31 - 1]
+    split = 0
+    for n in (1, 3, 65):
+        for turn in range(3):
+            if turn == 0:  # right ones, rows of no sequence at both ends
+                cu = sorted(rng.integers(1, rows, n + 1).tolist())
+                lens, table = [9000 + 7 * b for b in range(n)], rng.integers(0, 40, (n, room)).tolist()
+            else:
+                cu, lens = [pick.choice(wild) for _ in range(n + 1)], [pick.choice(wild) for _ in range(n)]
+                table = [[pick.choice(wild) for _ in range(room)] for _ in range(n)]
+            need = attention._chunk_workspace(rows, q_heads, heads, width, n, room * page)
+            split += need > 0
+            ws = torch.full((need // 4 + 2 * around,), fill, dtype=torch.int32, device="cuda")
+            out = torch.full((rows * q_heads * width // 2 + 2 * around,), 77, dtype=torch.int32, device="cuda")
+            cu_t, lens_t, table_t = ints(cu), ints(lens), ints(table)
+            print("writes", q_heads, width, fill, n, turn, flush=True)
+            _lib.call("lmoe_kv_chunk", q.data_ptr(), _lib.BF16, q_heads * width, width, rows, q_heads, heads, width, cu_t.data_ptr(),
+                      lens_t.data_ptr(), n, table_t.data_ptr(), room, codes[0], codes[1], codes[2], codes[3], 40, page, room * page,
+                      0.1, ws.data_ptr() + 4 * around, need, out.data_ptr() + 4 * around, _lib.stream())
+            torch.cuda.synchronize()
+            for t, x, inside in ((ws, fill, need // 4), (out, 77, rows * q_heads * width // 2)):
+                assert t[:around].eq(x).all() and t[around + inside:].eq(x).all(), (n, turn)
+            if turn == 0:
+                got = out[around:around + rows * q_heads * width // 2].view(torch.bfloat16).view(rows, q_heads, width)
+                assert torch.equal(got, attention.chunk_rows(q, cache, table_t, lens_t, cu_t, scale=0.1))
+    assert split
