@@ -20,12 +20,13 @@
 // Bound by the matrix cores (4 width products a visible pair), at the rate that their power allows: products alone reach 2.2-2.4
 // PFLOP/s on constant data and 1.84 on random data (the clock falls to 1.86 GHz); with six vector instructions beside each, which
 // is what the exponentials and the conversion need, 1.56; the library's largest product 1.21. Measured (2,048 rows over 34,816
-// tokens, 32 heads over 4 of 128, bf16): 1,030-1,067 us, 1.06-1.10 PFLOP/s, with float16, whose products take more power, 8 %
-// more; without LDS reads and staging 943. One after the other instead of slots 1,252; 128 pairs a workgroup 1,158; 64 pairs a
+// tokens, 32 heads over 4 of 128, bf16): 1,018-1,119 us by card, 1.01-1.11 PFLOP/s, with float16, whose products take more power,
+// 11 % more; without LDS reads and staging 943. One after the other instead of slots 1,252; 128 pairs a workgroup 1,158; 64 pairs a
 // wavefront, which halves the LDS reads and leaves one wavefront a SIMD (it issues a vector instruction every eight or nine
 // cycles, each of two every four or five), 1,156; codes two tiles ahead, or loads of single lanes' addresses, 1-3 % more. Width
-// 256: one wavefront a SIMD, 0.93-0.95 PFLOP/s where all places work. A short call's workgroup: 3.3 us to its first scores, 1.45
-// a tile, 2.5 of output.
+// 256: one wavefront a SIMD, 0.90-0.92 PFLOP/s where all places work (float16 0.83-0.85). Width 64: 0.68-0.71 (float16 0.61-0.63),
+// bound by the vector unit: a pair's exponential and the rest of its weight are the same for half of the products. A short call's
+// workgroup: 3.3 us to its first scores, 1.45 a tile, 2.5 of output.
 //
 // Weights, their sums and values that are not finite: as in prompt.hip.
 #include <cmath>
@@ -652,8 +653,9 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 1 : 2) k_chunk_rows(ChunkA
 // workgroup convert each key once for 256 pairs instead of 128 (2,048 rows over 34,816 tokens, 32 heads over 4 of 128: 1,158 ->
 // 1,067 us), but leave coarser work. Against one cut of all tiles at the same keys, sized for the longest sequence: 1,110 rows
 // over 2,291 tokens before them, 16 heads over 2 of 256, 118 -> 91 us; 100 single rows over up to 8,000, 32 over 4 of 128, 113 ->
-// 92; 64 sequences of up to 16 rows over up to 4,000 56 -> 48. 1,857 rows of three over up to 9,024, 16 over 2 of 256, 235 ->
-// 201. Beginning and end of a stretch cost 1-2 us more to find: 106 rows of four sequences over up to 948 16.4 -> 17.7.
+// 92; 64 sequences of up to 16 rows over up to 4,000 56 -> 48. Beginning and end of a stretch cost 1-2 us more to find: 106 rows of
+// four sequences over up to 948 16.4 -> 17.7. Against whole tiles: those 106 rows 27 -> 18, 1,857 rows of three sequences over up to
+// 9,024, 16 over 2 of 256, 332 -> 210, 12 sequences of 48 to 700 rows over up to 9,700, 28 over 4 of 128, 259 -> 241.
 struct ChunkPlan {
   int waves, stretches, per;  // no stretches: a workgroup a tile; per: stretches a tile
   long long tiles;

@@ -8,10 +8,10 @@
 //
 // A row is taken by `lanes` neighbouring threads, eight channels a thread and step: 8 to 64 lanes of a wavefront (up to 512
 // channels, 1,536 where rows are many; several rows a workgroup), or a workgroup of 256 (up to 16,384 in registers, longer ones
-// read twice, the second time from L2). Measured: 8,192 rows of 4,096 in bf16 with their residual 48.6-53.7 us, 5.0-5.5 TB/s
-// (with codes 51, read back 19); 2,048 rows of 32 heads of 128 7.9; one row 2.8 of kernel under 9 of the call; 4,000 rows of an
-// odd 5,001 3.6 TB/s, 2,000 of 20,000 3.1. Rows may begin anywhere: loads and stores are of 16 bytes whatever their alignment (the hardware splits what
-// crosses a line), and the last, partial eight go one by one.
+// read twice, the second time from L2). Measured: 8,192 rows of 4,096 in bf16 with their residual 53.9 us, 5.0 TB/s (with
+// codes 50, read back 20); 2,048 rows of 32 heads of 128 7.9; one row 2.8 of kernel under 9 of the call; 4,000 rows of an
+// odd 5,001 3.6 TB/s, 2,000 of 20,000 3.1. Rows may begin anywhere: loads and stores are of 16 bytes whatever their alignment (the
+// hardware splits what crosses a line), and the last, partial eight go one by one.
 #include "codes.h"
 
 namespace lmoe {

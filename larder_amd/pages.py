@@ -63,7 +63,7 @@ def _compact_workspace(pages):
 def take_pages(refs, table, lens, cu=None, page=64):
     """Gives every place of the table that the newest rows fall into a page that is its sequence's alone: the lowest free one
     (refs 0 when the call begins) where it has none, or where its page has other holders. lens, cu as append_rows takes them (the
-    rows counted in lens; one row a sequence where cu is None). refs and table are written in place.
+    rows counted in lens; one row a sequence where cu is None), page: the cache's tokens a page. refs and table are written in place.
 
     (src, dst, lacking), int32 [sequences] each: the pages to copy before the rows are appended, where a sequence had shared
     a page that holds tokens before them (-1: none; a sequence has one at most), and how many of its places found no page left.
@@ -107,7 +107,8 @@ def fork_pages(refs, table, parents):
     """A new table int32 [len(parents), places] whose sequence i goes on from sequence parents[i] (int32) of the old one and shares
     its pages; parents outside the table begin empty. The old table's places are given back in the same call: sequences
     that no parent names end, sequences named once have only moved, and the old table is not used again. Beams are reordered,
-    samples drawn from one prompt and finished sequences dropped by one call; lens follows as lens[parents]."""
+    samples drawn from one prompt and finished sequences dropped by one call; lens follows as lens[parents.long()], with 0 for
+    those that begin empty."""
     fn = "fork_pages"
     pages, n, places = _pool(fn, refs, table)
     if parents.dim() != 1:
