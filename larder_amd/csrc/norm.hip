@@ -121,7 +121,7 @@ __device__ __forceinline__ float lanes_max(float v, int lanes) {
 }
 
 // Where squares overflow: rows are scaled by kDown^2 for their sum (2^128 of the largest becomes 2^48, its square 2^96). A channel is
-// brought back by one kDown before its weight and one behind, so that what is small beside large ones is not rounded on the way
+// brought back by one kDown with its division and one after it, so that what is small beside large ones is not rounded on the way
 constexpr float kDown = 0x1p-40f;
 
 // N steps of eight channels a lane in registers; N = 0: rows of any length, read twice
@@ -184,6 +184,18 @@ __global__ void __launch_bounds__(256) k_norm(NormArgs a) {
     const float low = row_sum<L>(squares(kSquares), lds + 4);
     if (!(ss < INFINITY)) inv = kDown / sqrtf(low / float(a.H) + a.eps * kSquares * kSquares), down = kDown;
   }
+  auto divide = [&](float (&u)[8], const float (&w)[8]) {
+    if (down == 1.0f) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[e] = u[e] * inv * w[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {  // below 1 no weight overflows; from 1 on nothing is subnormal before its weight
+        const float y = u[e] * inv;
+        u[e] = fabsf(y) < 1.0f ? y * w[e] * down : y * down * w[e];
+      }
+    }
+  };
   auto normed = [&](int i, float (&u)[8]) {  // the step's y from its sums; the sums are written
     const int c = i * L + lane, n = a.H - 8 * c;
     if (n <= 0) {
@@ -197,8 +209,7 @@ __global__ void __launch_bounds__(256) k_norm(NormArgs a) {
       load_any<DT>(a.weight, 8 * c, n, w);
     else
       load_any<LMOE_F32>(a.weight, 8 * c, n, w);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) u[e] = u[e] * inv * w[e] * down;
+    divide(u, w);
   };
   if (!a.group) {
     for_steps<N>(steps, [&](int i) {
@@ -269,8 +280,7 @@ __global__ void __launch_bounds__(256) k_norm(NormArgs a) {
         load_any<DT>(a.weight, 8 * c, n, w);
       else
         load_any<LMOE_F32>(a.weight, 8 * c, n, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) u[e] = u[e] * inv * w[e] * down;
+      divide(u, w);
       most = fmaxf(most, finite(u));
     }
   }

@@ -197,3 +197,15 @@ def test_chunk_writes_its_rows_alone(q_heads, heads, width, rows, fill):
                 got = out[around:around + rows * q_heads * width // 2].view(torch.bfloat16).view(rows, q_heads, width)
                 assert torch.equal(got, attention.chunk_rows(q, cache, table_t, lens_t, cu_t, scale=0.1))
     assert split
+
+
+@pytest.mark.parametrize("h", [8, 512, 2000, 16400])
+@pytest.mark.parametrize("power", [-120, -60, 60, 110, 120])
+def test_norm_of_large_rows_with_weights_of_all_sizes(h, power):
+    """Rows whose squares pass float32, with weights down to 2^-120 and up to 2^120: results that float32 holds are right."""
+    rng = torch.Generator(device="cuda").manual_seed(h)
+    x = torch.randn((5, h), generator=rng, device="cuda").clamp(-4, 4) * 2.0 ** 70
+    x[1:3, ::2] *= 2.0 ** -100
+    x[3] *= 2.0 ** 50
+    w = (1 + torch.rand(h, generator=rng, device="cuda")) * 2.0 ** power
+    check_norm(x, None, w, 1e-6)
